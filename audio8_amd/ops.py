@@ -368,7 +368,7 @@ class LinearFn(torch.autograd.Function):
 
 def linear(x, weight, bias, out_f32=False):
     shp = x.shape
-    y = LinearFn.apply(x.reshape(-1, shp[-1]), weight, bias, out_f32)
+    y = LinearFn.apply(x.reshape(-1, shp[-1]).contiguous(), weight, bias, out_f32)      # (reshape keeps the row stride of an evenly spaced slice)
     return y.view(*shp[:-1], weight.shape[0])
 
 
