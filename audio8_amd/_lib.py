@@ -71,6 +71,17 @@ ARGTYPES = {
     "a8_ctc_fwd_bwd": [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p],
     "a8_log_softmax_fwd": [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p],
     "a8_log_softmax_bwd": [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p],
+    "a8_causal_conv_fwd": [C.c_void_p, C.c_void_p],
+    "a8_causal_conv_bwd_partial_floats": [C.c_void_p, C.c_void_p],
+    "a8_causal_conv_bwd": [C.c_void_p, C.c_void_p],
+    "a8_causal_conv_step": [C.c_void_p, C.c_void_p],
+    "a8_selective_scan_workspace": [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p],
+    "a8_selective_scan_fwd": [C.c_void_p, C.c_void_p],
+    "a8_selective_scan_bwd": [C.c_void_p, C.c_void_p],
+    "a8_selective_scan_step": [C.c_void_p, C.c_void_p],
+    "a8_residual_norm_fwd": [C.c_void_p, C.c_void_p],
+    "a8_residual_norm_bwd_workspace": [C.c_void_p, C.c_void_p],
+    "a8_residual_norm_bwd": [C.c_void_p, C.c_void_p],
     "a8_sumsq": [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p],
     "a8_adamw": [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int, C.c_void_p, C.c_float, C.c_float, C.c_void_p, C.c_int, C.c_void_p],
 }
@@ -120,8 +131,31 @@ class WPrepDesc(C.Structure):
                 ("tap", C.c_int), ("ld_dst", C.c_int), ("ld_dstT", C.c_int)]
 
 
+def _fields(spec):
+    """ctypes fields from "type name name; type name ..." (i int, f float, l int64, p pointer)."""
+    kinds = {"i": C.c_int, "f": C.c_float, "l": C.c_int64, "p": C.c_void_p}
+    return [(n, kinds[part.split()[0]]) for part in spec.split(";") for n in part.split()[1:]]
+
+
+class CausalConvDesc(C.Structure):
+    _fields_ = _fields("i size dtype B T C K act; p x; l x_bs x_ts; p w bias state lengths y state_out dy; l dy_bs dy_ts; "
+                       "p dstate_out dx dstate dw dbias; i add_dw add_dbias; p partials")
+
+
+class SelectiveScanDesc(C.Structure):
+    _fields_ = _fields("i size dtype B T D N G softplus; p u; l u_bs u_ts; p dt; l dt_bs dt_ts; p z; l z_bs z_ts; p Bm; l b_bs b_ts b_gs; "
+                       "p Cm; l c_bs c_ts c_gs; p A Dskip dt_bias h0 lengths y h_out ckpt ws dy; l dy_bs dy_ts; "
+                       "p dh_out du ddt dz dBm dCm dA dD ddt_bias dh0; i add_dA add_dD add_ddt_bias")
+
+
+class ResidualNormDesc(C.Structure):
+    _fields_ = _fields("i size dtype B T C kind post gate_rows; f eps; p x; l x_ld; p o; l o_ld; p gate; l g_bs g_ts; p scale w b post_w post_b r n stats "
+                       "dr dn dx d_o dgate dw db dpost_w dpost_b dscale; i add_dw add_db add_dpost_w add_dpost_b add_dscale; p ws")
+
+
 GEMM_DESC_SIZE, ENC_DESC_SIZE, ENC_BWD_DESC_SIZE = C.sizeof(GemmDesc), C.sizeof(EncoderLayerDesc), C.sizeof(EncoderLayerBwdDesc)
 ENC_BWD_FULL_DESC_SIZE = C.sizeof(EncoderLayerBwdFullDesc)
+CONV_DESC_SIZE, SCAN_DESC_SIZE, RNORM_DESC_SIZE = C.sizeof(CausalConvDesc), C.sizeof(SelectiveScanDesc), C.sizeof(ResidualNormDesc)
 ABI_VERSION = 120            # include/a8hip.h: A8HIP_VERSION
 
 
@@ -192,5 +226,8 @@ EXPORTS = [
     "a8_vq_select", "a8_vq_gather", "a8_vq_ppl", "a8_vq_bwd",
     "a8_contrastive_fwd", "a8_contrastive_bwd", "a8_loss_combine", "a8_loss_combine_bwd", "a8_ctc_greedy_decode",
     "a8_ctc_pack_targets", "a8_ctc_fwd_bwd", "a8_log_softmax_fwd", "a8_log_softmax_bwd",
+    "a8_causal_conv_fwd", "a8_causal_conv_bwd_partial_floats", "a8_causal_conv_bwd", "a8_causal_conv_step",
+    "a8_selective_scan_workspace", "a8_selective_scan_fwd", "a8_selective_scan_bwd", "a8_selective_scan_step",
+    "a8_residual_norm_fwd", "a8_residual_norm_bwd_workspace", "a8_residual_norm_bwd",
     "a8_sumsq", "a8_adamw", "a8_zero", "a8_conv_wgrad_fold", "a8_host_negative_indices",
 ]

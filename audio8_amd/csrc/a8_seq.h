@@ -1,0 +1,43 @@
+// a8hip -- what the causal sequence kernels (causal_conv.hip, selective_scan.hip, residual_norm.hip) share.
+#pragma once
+#include "a8_common.h"
+
+constexpr float SEQ_LOG2E = 1.4426950408889634f;
+
+A8_DEV float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * SEQ_LOG2E); }
+A8_DEV float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x)); }
+A8_DEV float silu_f(float x) { return x * sigmoid_f(x); }
+// d/dx [x s(x)] = s (1 + x (1 - s)).  1 - s(x) is taken as s(-x): the difference loses all its bits for large x.
+A8_DEV float silu_grad_f(float x) {
+    const float e = exp_fast(-fabsf(x)), r = __builtin_amdgcn_rcpf(1.0f + e);
+    const float big = r, small = e * r;                       // s(|x|), s(-|x|)
+    const float s = x >= 0.f ? big : small, c = x >= 0.f ? small : big;
+    return s * fmaf(x, c, 1.0f);
+}
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1].  log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, by its odd series up to
+// s^15 (the first term left out is < 2 (1/3)^17 / 17 = 9e-10): no 1 + e is rounded, so small step lengths keep their relative precision.
+A8_DEV float softplus_f(float x) {
+    const float e = exp_fast(-fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+    float r = 2.0f / 15.0f;
+    r = fmaf(r, q, 2.0f / 13.0f);
+    r = fmaf(r, q, 2.0f / 11.0f);
+    r = fmaf(r, q, 2.0f / 9.0f);
+    r = fmaf(r, q, 2.0f / 7.0f);
+    r = fmaf(r, q, 2.0f / 5.0f);
+    r = fmaf(r, q, 2.0f / 3.0f);
+    r = fmaf(r, q, 2.0f);
+    return fmaf(s, r, fmaxf(x, 0.f));
+}
+
+// `planes` column sums over `rows` partial rows [rows][planes][C]: plane q < np goes to major[c * np + q] (a [C][np] matrix), plane np + i to
+// minor[i][c]; null targets are skipped.  add = 1 accumulates.  Summed in a fixed order: the same inputs give the same bits.
+struct A8SeqReduce {
+    const float* in; int rows, planes, C, np;
+    float* major; float* minor[6];
+    int add_major, add_minor[6];
+};
+int a8i_seq_reduce(const A8SeqReduce& r, void* stream);
+
+// a descriptor's frame count of utterance b: lengths[b] clamped to [0, T]
+A8_DEV int seq_len(const int32_t* lengths, int b, int T) { return lengths ? min(max(lengths[b], 0), T) : T; }

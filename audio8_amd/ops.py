@@ -488,6 +488,178 @@ class ZeroFn(torch.autograd.Function):
         return dx, None, None
 
 
+# ------------------------------------------------------------------ causal sequence operators
+# What mixes frames without looking ahead (a short convolution, a selective state space scan) and the norms around such a block: forward and
+# backward over [B, T, C], and a step for one frame per utterance that carries the state in place.  See include/a8hip.h for the formulas.
+def _param_grads(ctx, params):
+    """Targets of the parameter gradients, per parameter (position in the forward's arguments, tensor): p.grad when gradients go there
+    directly, a fresh tensor otherwise, None when not needed.  -> (targets, add flags, gradients to return)."""
+    tgts, add, ret = [], [], []
+    for at, p in params:
+        t = g = None
+        if p is not None and ctx.needs_input_grad[at]:
+            t = _target(p) if p.is_leaf else None
+            add.append(t is not None)
+            if t is None:
+                t = g = torch.empty(p.shape, device=p.device, dtype=torch.float32)
+        else:
+            add.append(False)
+        tgts.append(t)
+        ret.append(g)
+    return tgts, add, ret
+
+
+def _ready_direct(params, add):
+    for (_, p), a in zip(params, add):
+        if a:
+            _ready(p)
+
+
+def _rows(t):
+    """t with contiguous channels (a copy only where it has none)."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _step_only(what, *ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"a8hip {what}: a step updates its state in place and has no gradient; call it under torch.no_grad()")
+
+
+class CausalConvFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, lengths, act, want_state):
+        y, out = K.causal_conv_fwd(x.detach(), weight.detach(), bias.detach() if bias is not None else None, act, state, lengths, want_state)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, state, lengths, weight, bias)
+        ctx.act, ctx.params = act, ((1, weight), (2, bias))
+        return y, out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dout):
+        x, state, lengths, weight, bias = ctx.saved_tensors
+        dy = torch.zeros(x.shape, device=x.device, dtype=x.dtype) if dy is None else _rows(dy)
+        dout = dout.contiguous() if dout is not None else None
+        (dw, db), add, ret = _param_grads(ctx, ctx.params)
+        dx, dstate = K.causal_conv_bwd(dy, x, weight, bias, ctx.act, state, lengths, dout, ctx.needs_input_grad[3], dw, db, add)
+        _ready_direct(ctx.params, add)
+        return dx, ret[0], ret[1], dstate, None, None, None
+
+
+def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=None, return_state=False):
+    """Depthwise causal convolution over the last K = 2 .. 4 frames: y[b, t, c] = act(bias[c] + sum_k weight[c, k] x[b, t - K + 1 + k, c]).
+
+    x [B, T, C] bf16 or f32, read in place where its channels are contiguous; weight f32 [C, K] or [C, 1, K]; bias f32 [C]; activation None or
+    "silu".  state [B, K - 1, C]: the frames before x (zeros without it).  lengths int32 [B] on the device: frames of each utterance; what lies
+    behind is not read, comes out as zero and gets a zero gradient.  return_state: also return the last K - 1 frames of each utterance
+    (with `state` in front of short ones), with which the next call or causal_conv_step goes on.  Differentiable in x, weight, bias, state."""
+    y, out = CausalConvFn.apply(_rows(x), weight, bias, state, lengths, activation, return_state)
+    return (y, out) if return_state else y
+
+
+def causal_conv_step(x, state, weight, bias=None, *, activation="silu"):
+    """One frame of causal_conv for each utterance: x [B, C], state [B, K - 1, C] updated in place -> y [B, C].  No gradient."""
+    _step_only("causal_conv_step", x, state)
+    y = K.causal_conv_step(_rows(x), state, weight.detach(), bias.detach() if bias is not None else None, activation)
+    torch.autograd.graph.increment_version(state)
+    return y
+
+
+class SelectiveScanFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state):
+        grad = any(ctx.needs_input_grad)
+        y, out, ckpt = K.selective_scan_fwd(u.detach(), dt, A.detach(), B, C, D.detach() if D is not None else None, z,
+                                            dt_bias.detach() if dt_bias is not None else None, softplus, state, lengths, want_state, grad)
+        ctx.set_materialize_grads(False)
+        if grad:
+            ctx.save_for_backward(u, dt, A, B, C, D, z, dt_bias, state, lengths, ckpt)
+            ctx.softplus, ctx.params = softplus, ((2, A), (5, D), (7, dt_bias))
+        return y, out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dout):
+        u, dt, A, B, C, D, z, dt_bias, state, lengths, ckpt = ctx.saved_tensors
+        dy = torch.zeros(u.shape, device=u.device, dtype=u.dtype) if dy is None else _rows(dy)
+        dout = dout.contiguous() if dout is not None else None
+        (dA, dD, db), add, ret = _param_grads(ctx, ctx.params)
+        du, ddt, dz, dB, dC, dstate = K.selective_scan_bwd(dy, ckpt, u, dt, A, B, C, D, z, dt_bias, ctx.softplus, state, lengths, dout,
+                                                           ctx.needs_input_grad[8], dA, dD, db, add)
+        _ready_direct(ctx.params, add)
+        return du, ddt, ret[0], dB, dC, ret[1], dz, ret[2], dstate, None, None, None
+
+
+def selective_scan(u, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=True, state=None, lengths=None, return_state=False):
+    """Selective state space scan over frames, N = 1 .. 32 states per channel:
+        s = softplus(dt + dt_bias);  h_t = exp(s_t A) h_{t-1} + s_t u_t B_t;  y = (sum_n C_t h_t + D u) silu(z)
+
+    u, dt, z [B, T, Dm] and B, C [B, T, G, N] (or [B, T, N]: one group) in one dtype, bf16 or f32, read in place where their last axis is
+    contiguous; the Dm / G channels of a group share B and C.  A f32 [Dm, N] (negative for decaying states), D and dt_bias f32 [Dm].
+    state f32 [B, Dm, N]: the state before the first frame.  lengths and return_state as in causal_conv.
+    Differentiable in everything but lengths; the forward then keeps every 16th frame's states (B Dm N / 16 floats per frame)."""
+    if B.dim() == 3 and C.dim() == 3:
+        B, C = B.unsqueeze(2), C.unsqueeze(2)
+    y, out = SelectiveScanFn.apply(_rows(u), _rows(dt), A, _rows(B), _rows(C), D, _rows(z), dt_bias, state, lengths, softplus, return_state)
+    return (y, out) if return_state else y
+
+
+def selective_scan_step(u, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, softplus=True):
+    """One frame of selective_scan for each utterance: u, dt, z [B, Dm], B and C [B, G, N] (or [B, N]), state f32 [B, Dm, N] updated in place
+    -> y [B, Dm].  No gradient."""
+    _step_only("selective_scan_step", u, dt, B, C, z, state)
+    if B.dim() == 2 and C.dim() == 2:
+        B, C = B.unsqueeze(1), C.unsqueeze(1)
+    y = K.selective_scan_step(_rows(u), _rows(dt), A.detach(), _rows(B), _rows(C), state, D.detach() if D is not None else None, _rows(z),
+                              dt_bias.detach() if dt_bias is not None else None, softplus)
+    torch.autograd.graph.increment_version(state)
+    return y
+
+
+class GatedResidualNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, o, weight, bias, post_weight, post_bias, gate, scale, eps, kind):
+        grad = any(ctx.needs_input_grad)
+        r, n, stats = K.residual_norm_fwd(x, o, *(p.detach() if p is not None else None for p in (weight, bias, post_weight, post_bias)), gate,
+                                          scale.detach() if scale is not None else None, eps, kind, grad)
+        ctx.set_materialize_grads(False)
+        if grad:
+            ctx.save_for_backward(x, o, weight, bias, post_weight, post_bias, gate, scale, stats)
+            ctx.eps, ctx.kind = eps, kind
+            ctx.params = ((2, weight), (3, bias), (4, post_weight), (5, post_bias), (7, scale))
+        return r, n
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dr, dn):
+        x, o, w, b, pw, pb, gate, scale, stats = ctx.saved_tensors
+        tgts, add, ret = _param_grads(ctx, ctx.params)
+        dx, do, dgate = K.residual_norm_bwd(dr.contiguous() if dr is not None else None, dn.contiguous() if dn is not None else None, stats, x, o,
+                                            w, b, pw, pb, gate, scale, ctx.eps, ctx.kind, *tgts, add=add)
+        _ready_direct(ctx.params, add)
+        return dx, do, ret[0], ret[1], ret[2], ret[3], dgate, ret[4], None, None
+
+
+def _even_rows(t):
+    t = _rows(t)
+    return t if t.shape[0] == 1 or t.shape[1] == 1 or t.stride(0) == t.shape[1] * t.stride(1) else t.contiguous()
+
+
+def gated_residual_norm(x, o, weight=None, bias=None, *, post_weight=None, post_bias=None, gate=None, scale=None, eps=1e-6, kind="layer"):
+    """The end of one block and the norm in front of the next: r = x + scale * gate * N(o; post_weight, post_bias), n = N(r; weight, bias) -> (r, n).
+
+    x (residual stream) and o (the block's output) [B, T, C] or [T, C] in bf16 or f32, up to 8192 channels; gate [B, T, C] or one row per
+    utterance [B, 1, C] in the same dtype; norm parameters and scale f32 [C].  kind "layer" (LayerNorm) or "rms".  Without post_weight o is
+    taken as it is; without weight n is None.  n is formed from the sum before it is rounded to r.  Differentiable in every tensor."""
+    if x.dim() == 2 and o.dim() == 2 and (gate is None or gate.dim() == 2):
+        r, n = gated_residual_norm(x.unsqueeze(0), o.unsqueeze(0), weight, bias, post_weight=post_weight, post_bias=post_bias,
+                                   gate=gate.unsqueeze(0) if gate is not None else None, scale=scale, eps=eps, kind=kind)
+        return r[0], n[0] if n is not None else None
+    if x.dim() != 3 or o.dim() != 3:
+        raise ValueError(f"a8hip gated_residual_norm: x and o have {x.dim()} and {o.dim()} axes, expected [batch, frames, channels]")
+    return GatedResidualNormFn.apply(_even_rows(x), _even_rows(o), weight, bias, post_weight, post_bias, _rows(gate), scale, eps, kind)
+
+
 # ------------------------------------------------------------------ conv feature extractor
 _CONV_DX_CACHE = {}       # (utterances, padded rows, channels, dtype, device, layer) -> data-gradient buffer whose pad rows are zero
 

@@ -349,6 +349,91 @@ int a8_adamw(float* p, float* g, float* m, float* v, int64_t n, float lr, float 
              float weight_decay, int step, const float* gnorm_sq, float max_norm, float grad_scale, const int64_t* grad_denom,
              int zero_grad, void* stream);
 
+/* ---- causal sequence operators (streaming encoders): what mixes frames without looking ahead, and the norms around such a block ----
+ * Channels-last like everything else: element (b, t, c) of a strided input at b * bs + t * ts + c (strides in elements, channels contiguous:
+ * a slice of a wider projection is read in place); outputs are contiguous.  Activations (x, u, dt, z, B, C, o, gate, y ...) are `dtype`;
+ * weights, A, skips, biases, scan states and all parameter gradients are f32.
+ * lengths (int32 [B] on the device, or NULL): utterance b has lengths[b] frames (clamped to 0 .. T).  Frames behind its end are not read; their
+ * outputs and gradients are zero and the final state is the state at its end.
+ * add_*: 1 adds the parameter gradient to its target, 0 stores it.  All sums are taken in a fixed order: the same call gives the same bits. */
+enum { A8_CONV_ACT_NONE = 0, A8_CONV_ACT_SILU = 1 };
+enum { A8_NORM_LAYER = 0, A8_NORM_RMS = 1 };
+
+/* Depthwise causal convolution over K = 2 .. 4 frames: with e = (state[b, 0 .. K-2], x[b, 0 .. T-1]),
+ *   y[b, t, c] = act(bias[c] + sum_k w[c, k] e[b, t + k, c]),   state_out[b, j] = e[b, len + j]   (state NULL: zeros; state_out may be NULL).
+ * bwd: dy and the optional dstate_out -> dx, dstate, dw, dbias (each may be NULL); partials: a8_causal_conv_bwd_partial_floats() floats.
+ * step: one frame (T = 1) per utterance, state_out is the history, read and updated in place; lengths is not used. */
+typedef struct a8_causal_conv_desc {
+    int size;                             /* sizeof(a8_causal_conv_desc) */
+    int dtype, B, T, C, K, act;
+    const void* x; int64_t x_bs, x_ts;
+    const float* w; const float* bias;    /* [C][K], [C] or NULL */
+    const void* state;                    /* [B][K-1][C] or NULL */
+    const int32_t* lengths;
+    void* y; void* state_out;             /* [B][T][C], [B][K-1][C] */
+    const void* dy; int64_t dy_bs, dy_ts;
+    const void* dstate_out;
+    void* dx; void* dstate;
+    float* dw; float* dbias; int add_dw, add_dbias;
+    float* partials;
+} a8_causal_conv_desc;
+int a8_causal_conv_fwd(const a8_causal_conv_desc* d, void* stream);
+int a8_causal_conv_bwd_partial_floats(const a8_causal_conv_desc* d, int64_t* floats);
+int a8_causal_conv_bwd(const a8_causal_conv_desc* d, void* stream);
+int a8_causal_conv_step(const a8_causal_conv_desc* d, void* stream);
+
+/* Selective state space scan over N = 1 .. 32 states per channel, B and C shared by the D / G channels of a group:
+ *   s_t = softplus(dt + dt_bias) (softplus = 0: dt + dt_bias);  h_t = exp(s_t A) h_{t-1} + s_t u_t B_t;
+ *   y = (sum_n C_t h_t + Dskip u) silu(z)                           (Dskip, dt_bias, z, h0 may be NULL; h0 NULL: zeros)
+ * h_out [B][D][N] receives the state at each utterance's end.  ckpt (saved for bwd, or NULL) and ws: a8_selective_scan_workspace() floats.
+ * bwd: dy and the optional dh_out -> du, ddt, dz, dBm, dCm (contiguous) and dA, dD, ddt_bias, dh0 (these may be NULL).
+ * step: one frame (T = 1) per utterance, h_out is the state, read and updated in place. */
+typedef struct a8_selective_scan_desc {
+    int size;                             /* sizeof(a8_selective_scan_desc) */
+    int dtype, B, T, D, N, G, softplus;
+    const void* u;  int64_t u_bs, u_ts;
+    const void* dt; int64_t dt_bs, dt_ts;
+    const void* z;  int64_t z_bs, z_ts;
+    const void* Bm; int64_t b_bs, b_ts, b_gs;      /* element (b, t, g, n) at b * bs + t * ts + g * gs + n */
+    const void* Cm; int64_t c_bs, c_ts, c_gs;
+    const float* A; const float* Dskip; const float* dt_bias;      /* [D][N], [D], [D] */
+    const float* h0; const int32_t* lengths;
+    void* y; float* h_out; float* ckpt; float* ws;
+    const void* dy; int64_t dy_bs, dy_ts;
+    const float* dh_out;
+    void* du; void* ddt; void* dz; void* dBm; void* dCm;
+    float* dA; float* dD; float* ddt_bias; float* dh0;
+    int add_dA, add_dD, add_ddt_bias;
+} a8_selective_scan_desc;
+int a8_selective_scan_workspace(const a8_selective_scan_desc* d, int backward, int64_t* ckpt_floats, int64_t* ws_floats);
+int a8_selective_scan_fwd(const a8_selective_scan_desc* d, void* stream);
+int a8_selective_scan_bwd(const a8_selective_scan_desc* d, void* stream);
+int a8_selective_scan_step(const a8_selective_scan_desc* d, void* stream);
+
+/* The norms before and after a block with its gate and residual scale: p = N(o; post_w, post_b) (post = 0: o);  r = x + scale gate p;
+ * n = N(r; w, b) (n NULL: left out).  N over C <= 8192 channels: LayerNorm or RMS norm (kind); biases, gate and scale may be NULL.
+ * gate: [B][T][C] (gate_rows = 1) or one row per utterance [B][1][C].  x and o: rows of B * T with leading dimension ld.
+ * stats f32 [4][B * T] (mean and 1/std of o, then of r) is written by fwd when not NULL and read by bwd.
+ * bwd: dr and dn (either may be NULL) -> dx, d_o, dgate (shaped as gate, contiguous) and the parameter gradients (each may be NULL). */
+typedef struct a8_residual_norm_desc {
+    int size;                             /* sizeof(a8_residual_norm_desc) */
+    int dtype, B, T, C, kind, post, gate_rows;
+    float eps;
+    const void* x; int64_t x_ld;
+    const void* o; int64_t o_ld;
+    const void* gate; int64_t g_bs, g_ts;
+    const float* scale; const float* w; const float* b; const float* post_w; const float* post_b;      /* [C] */
+    void* r; void* n; float* stats;
+    const void* dr; const void* dn;
+    void* dx; void* d_o; void* dgate;
+    float* dw; float* db; float* dpost_w; float* dpost_b; float* dscale;
+    int add_dw, add_db, add_dpost_w, add_dpost_b, add_dscale;
+    float* ws;                            /* a8_residual_norm_bwd_workspace() floats */
+} a8_residual_norm_desc;
+int a8_residual_norm_fwd(const a8_residual_norm_desc* d, void* stream);
+int a8_residual_norm_bwd_workspace(const a8_residual_norm_desc* d, int64_t* floats);
+int a8_residual_norm_bwd(const a8_residual_norm_desc* d, void* stream);
+
 /* ---- host side of the boundary (no GPU work) ----
  * Negative indices of the contrastive loss exactly as the reference draws them: np.random.randint(0, T - 1, (B, n_neg * T)), the
  * ">= own frame -> +1" shift and the per-utterance row offset (audio8/wav2vec2.py:955-976), on a copy of numpy's global MT19937 state

@@ -1,0 +1,548 @@
+"""Causal convolution, selective scan and gated residual norms on the GPU against their float64 definitions (oracle/seq_ref.py).
+
+Tolerances, per element: half a step of the output's type relative to the value (bf16 2^-8, f32 2^-24), plus F 2^-24 of the largest sum of term
+magnitudes in the tensor (the oracle's `mag` evaluation), F = the number of f32 roundings an element of that output can collect on its way:
+  convolution  F = K + 12 (K products, about 10 in the activation: exp2's argument up to 8, rcp, products); weight gradients + B T (a sum of B T terms)
+  scan         a state collects about 8 per frame (step length and its exponent, product, fma), the adjoint as many: F = 16 T + 40;
+               sums over channels or frames add their length
+  norms        statistics are sums of C terms over 64 lanes: F = C / 32 + 40, and column sums + B T
+"""
+import pytest
+import torch
+
+from oracle import seq_ref as R
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+def rnd(*shape, seed, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def check(name, got, ref, mag, F):
+    assert got is not None, name
+    assert tuple(got.shape) == tuple(ref.shape), (name, got.shape, ref.shape)
+    g = got.detach().double().cpu()
+    assert torch.isfinite(g).all(), name
+    if not g.numel():
+        return
+    tol = HALF_STEP[got.dtype] * ref.abs() + F * 2.0 ** -24 * mag.abs().max()
+    bad = (g - ref).abs() - tol
+    assert bad.max() <= 0, f"{name}: off by {float((g - ref).abs().max()):.3e}, {float(bad.max()):.3e} over its tolerance"
+
+
+def cu(t, grad=False):
+    return None if t is None else t.cuda().requires_grad_(grad)
+
+
+def wide(t, left, right):
+    """The same values as a slice of a wider tensor: last axis contiguous, every other stride odd."""
+    full = torch.full((*t.shape[:-1], left + t.shape[-1] + right), float("nan"), dtype=t.dtype)
+    full[..., left:left + t.shape[-1]] = t
+    return full.cuda()[..., left:left + t.shape[-1]]
+
+
+# ------------------------------------------------------------------------------------------------ causal convolution
+CONV = [  # B, T, C, K, act, state, lengths, strided
+    (2, 37, 64, 4, "silu", True, None, False),
+    (1, 1, 1, 2, "silu", True, None, False),
+    (3, 2, 7, 4, None, True, [2, 0, 1], False),
+    (2, 130, 72, 3, "silu", False, [130, 67], True),
+    (4, 65, 129, 4, "silu", True, [65, 64, 1, 3], True),
+    (1, 300, 24, 2, None, False, None, True),
+    (2, 33, 1536, 4, "silu", False, None, False),
+    (5, 16, 520, 3, "silu", True, [16, 15, 2, 17, -4], False),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", CONV, ids=str)
+def test_causal_conv(case, dtype):
+    from audio8_amd import ops
+    B, T, C, K, act, has_state, lengths, strided = case
+    x, w, b = rnd(B, T, C, seed=1, dtype=dtype), rnd(C, 1, K, seed=2), rnd(C, seed=3)
+    state = rnd(B, K - 1, C, seed=4, dtype=dtype) if has_state else None
+    dy, dst = rnd(B, T, C, seed=5, dtype=dtype), rnd(B, K - 1, C, seed=6, dtype=dtype)
+    n = torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None
+    xg = (wide(x, 3, 2) if strided else x.cuda()).requires_grad_()
+    wg, bg, sg = cu(w, True), cu(b, True), cu(state, True)
+    y, out = ops.causal_conv(xg, wg, bg, activation=act, state=sg, lengths=cu(n), return_state=True)
+    leaves = [xg, wg, bg] + ([sg] if has_state else [])
+    got = torch.autograd.grad([y, out], leaves, [wide(dy, 1, 4) if strided else dy.cuda(), dst.cuda()])
+    ref, mag = (R.conv(x, w, b, act, state, n, dy, dst, mag=m) for m in (False, True))
+    F = K + 12
+    check("y", y, ref["y"], mag["y"], F)
+    assert torch.equal(out.cpu().double(), ref["state"])
+    check("dx", got[0], ref["dx"], mag["dx"], F + K)
+    check("dw", got[1].reshape(C, K), ref["dw"], mag["dw"], F + B * T)
+    check("dbias", got[2], ref["dbias"], mag["dbias"], F + B * T)
+    if has_state:
+        check("dstate", got[3], ref["dstate"], mag["dstate"], F + K)
+    if n is not None:                      # what lies behind an utterance's end is zero, whatever x and dy hold there
+        for i, e in enumerate(lengths):
+            e = min(max(e, 0), T)
+            assert not y[i, e:].any() and not got[0][i, e:].any()
+
+
+def test_causal_conv_does_not_read_behind_the_end():
+    from audio8_amd import ops
+    x, w = rnd(2, 40, 16, seed=1), cu(rnd(16, 4, seed=2), True)
+    n = torch.tensor([40, 9], dtype=torch.int32, device="cuda")
+    dirty = x.clone()
+    dirty[1, 9:] = float("nan")
+    dy = rnd(2, 40, 16, seed=3).cuda()
+    dirty_dy = dy.clone()
+    dirty_dy[1, 9:] = float("inf")
+    res = []
+    for a, d in ((x, dy), (dirty, dirty_dy)):
+        xg = cu(a.clone(), True)
+        y, st = ops.causal_conv(xg, w, lengths=n, return_state=True)
+        res.append([y, st, *torch.autograd.grad(y, [xg, w], d)])
+    for p, q in zip(*res):
+        assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1, 2), (1, 1536, 4), (7, 130, 3), (33, 65, 4)])
+def test_causal_conv_step_continues_a_prompt(shape, dtype):
+    from audio8_amd import ops
+    B, C, K = shape
+    x, w, b = rnd(B, 9, C, seed=1, dtype=dtype), rnd(C, K, seed=2), rnd(C, seed=3)
+    n = torch.arange(B, dtype=torch.int32) % 5
+    xg, wg, bg = wide(x, 1, 2), cu(w), cu(b)
+    _, state = ops.causal_conv(xg[:, :4], wg, bg, lengths=cu(n), return_state=True)
+    ys = [ops.causal_conv_step(xg[:, t], state, wg, bg) for t in range(4, 9)]
+    for i in range(B):
+        seq = torch.cat([x[i, :n[i].clamp(max=4)], x[i, 4:]])[None]
+        ref, mag = (R.conv(seq, w, b, mag=m) for m in (False, True))
+        check(f"y of {i}", torch.stack([y[i] for y in ys]), ref["y"][0, -5:], mag["y"][0, -5:], K + 12)
+        assert torch.equal(state[i].cpu().double(), ref["state"][0])
+
+
+# ---------------------------------------------------------------------------------------------- selective scan
+SCAN = [  # B, T, D, N, G, z, softplus, skip and bias, state, lengths, strided
+    (2, 37, 64, 16, 1, True, True, True, True, None, False),
+    (1, 1, 1, 1, 1, True, True, True, True, None, False),
+    (2, 16, 65, 4, 1, False, True, True, False, None, True),
+    (3, 33, 130, 11, 2, True, True, True, True, [33, 0, 17], True),
+    (2, 50, 24, 32, 3, True, True, False, True, [50, 16], False),
+    (1, 200, 70, 8, 1, False, False, True, False, None, False),
+    (4, 17, 96, 5, 4, True, True, True, True, [1, 16, 17, -3], True),
+    (1, 600, 64, 16, 1, True, True, True, True, None, True),
+    (2, 400, 40, 17, 1, True, True, True, True, [400, 129], False),
+]
+
+
+def scan_inputs(case, dtype):
+    B, T, D, N, G, z, softplus, extras, state, lengths, strided = case
+    a = dict(u=rnd(B, T, D, seed=1, dtype=dtype), dt=rnd(B, T, D, seed=2, dtype=dtype, scale=0.5), A=-torch.exp(rnd(D, N, seed=3)),
+             B=rnd(B, T, G, N, seed=4, dtype=dtype), C=rnd(B, T, G, N, seed=5, dtype=dtype), D=rnd(D, seed=6) if extras else None,
+             z=rnd(B, T, D, seed=7, dtype=dtype) if z else None, dt_bias=rnd(D, seed=8) - 2 if extras else None,
+             state=rnd(B, D, N, seed=9) if state else None)
+    if not softplus:
+        a["dt"], a["dt_bias"] = a["dt"].abs() * 0.1, a["dt_bias"].abs() * 0.1 if extras else None      # (steps as they are: positive, or states grow without bound)
+    return a, torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", SCAN, ids=str)
+def test_selective_scan(case, dtype):
+    from audio8_amd import ops
+    B, T, D, N, G, _, softplus, _, _, lengths, strided = case
+    a, n = scan_inputs(case, dtype)
+    dy, dst = rnd(B, T, D, seed=10, dtype=dtype), rnd(B, D, N, seed=11)
+    g = {}
+    for k, v in a.items():
+        if v is not None:
+            if strided and k in ("B", "C"):
+                g[k] = wide(v.flatten(2), 5, 2).unflatten(-1, (G, N)).requires_grad_()
+            else:
+                g[k] = (wide(v, 1, 2) if strided and k in ("u", "dt", "z") else v.cuda()).requires_grad_()
+    args = [g[k] for k in ("u", "dt", "A", "B", "C")]
+    kw = {k: g.get(k) for k in ("D", "z", "dt_bias", "state")}
+    y, out = ops.selective_scan(*args, **kw, softplus=softplus, lengths=cu(n), return_state=True)
+    got = dict(zip(g, torch.autograd.grad([y, out], list(g.values()), [wide(dy, 2, 1) if strided else dy.cuda(), dst.cuda()])))
+    ref, mag = (R.scan(**a, softplus=softplus, lengths=n, dy=dy, dstate_out=dst, mag=m) for m in (False, True))
+    F = 16 * T + 40
+    check("y", y, ref["y"], mag["y"], F + N)
+    check("state", out, ref["state"], mag["state"], F)
+    more = {"B": D // G, "C": D // G, "A": B * T, "D": B * T, "dt_bias": B * T}
+    for k in g:
+        key = "d" + k
+        check(key, got[k], ref[key], mag[key], F + N + more.get(k, 0))
+    with torch.no_grad():                  # the inference call gives the same bits
+        y2, out2 = ops.selective_scan(*args, **kw, softplus=softplus, lengths=cu(n), return_state=True)
+    assert torch.equal(y, y2) and torch.equal(out, out2)
+
+
+def test_selective_scan_does_not_read_behind_the_end():
+    from audio8_amd import ops
+    case = (2, 50, 64, 16, 1, True, True, True, False, [50, 21], False)
+    a, n = scan_inputs(case, torch.float32)
+    dy = rnd(2, 50, 64, seed=10)
+    res = []
+    for dirty in (False, True):
+        v = {k: t.clone() if t is not None else None for k, t in a.items()}
+        d = dy.clone()
+        if dirty:
+            for k in ("u", "dt", "B", "C", "z"):
+                v[k][1, 21:] = float("nan")
+            d[1, 21:] = float("inf")
+        g = {k: cu(t, True) for k, t in v.items() if t is not None}
+        y, st = ops.selective_scan(g["u"], g["dt"], g["A"], g["B"], g["C"], D=g["D"], z=g["z"], dt_bias=g["dt_bias"], lengths=cu(n), return_state=True)
+        res.append([y, st, *torch.autograd.grad(y, list(g.values()), d.cuda())])
+    for p, q in zip(*res):
+        assert torch.equal(p, q)
+
+
+def test_selective_scan_strong_decay_and_large_steps():
+    """Steps up to 20 and decays down to exp(-320): states forget within a frame; gradients of A come from products that are tiny next to the states."""
+    from audio8_amd import ops
+    B, T, D, N = 1, 40, 64, 16
+    a = dict(u=rnd(B, T, D, seed=1), dt=rnd(B, T, D, seed=2, scale=8.0), A=-torch.arange(1, N + 1).float().repeat(D, 1), B=rnd(B, T, 1, N, seed=3), C=rnd(B, T, 1, N, seed=4))
+    dy = rnd(B, T, D, seed=5)
+    g = {k: cu(t, True) for k, t in a.items()}
+    y = ops.selective_scan(*g.values())
+    got = dict(zip(g, torch.autograd.grad(y, list(g.values()), dy.cuda())))
+    ref, mag = (R.scan(**a, dy=dy, mag=m) for m in (False, True))
+    F = 16 * T + 40 + 2 * 320              # exp2's argument is rounded at up to 320 / ln 2: as many roundings of the decay, where the decay is not zero
+    check("y", y, ref["y"], mag["y"], F)
+    for k in g:
+        check("d" + k, got[k], ref["d" + k], mag["d" + k], F + N + {"B": D, "C": D, "A": T}.get(k, 0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1), (2, 130, 16, 2), (5, 70, 11, 1), (3, 64, 32, 1), (40, 96, 8, 4)])
+def test_selective_scan_step_continues_a_prompt(shape, dtype):
+    from audio8_amd import ops
+    B, D, N, G = shape
+    case = (B, 9, D, N, G, True, True, True, True, (torch.arange(B) % 5).tolist(), False)
+    a, n = scan_inputs(case, dtype)
+    g = {k: (wide(v, 1, 1) if k in ("u", "dt", "z") else v.cuda()) for k, v in a.items()}
+    par = dict(D=g["D"], dt_bias=g["dt_bias"])
+    _, state = ops.selective_scan(g["u"][:, :4], g["dt"][:, :4], g["A"], g["B"][:, :4], g["C"][:, :4], z=g["z"][:, :4], state=g["state"], lengths=cu(n), return_state=True, **par)
+    ys = [ops.selective_scan_step(g["u"][:, t], g["dt"][:, t], g["A"], g["B"][:, t], g["C"][:, t], state, z=g["z"][:, t], **par) for t in range(4, 9)]
+    for i in range(B):
+        keep = torch.cat([torch.arange(min(int(n[i]), 4)), torch.arange(4, 9)])
+        seq = {k: (v[i:i + 1, keep] if k in ("u", "dt", "z", "B", "C") else v[i:i + 1] if k == "state" else v) for k, v in a.items()}
+        ref, mag = (R.scan(**seq, mag=m) for m in (False, True))
+        check(f"y of {i}", torch.stack([y[i] for y in ys]), ref["y"][0, -5:], mag["y"][0, -5:], 16 * 9 + 40 + N)
+        check(f"state of {i}", state[i], ref["state"][0], mag["state"][0], 16 * 9 + 40)
+
+
+# ------------------------------------------------------------------------------------------------ gated residual norms
+NORM = [  # B, T, C, kind, gate, post, bias, scale, next norm, strided
+    (2, 5, 768, "layer", "rows", True, True, True, True, False),
+    (2, 37, 1024, "rms", "utterance", True, False, True, True, False),
+    (1, 1, 1, "layer", "rows", True, True, True, True, False),
+    (3, 7, 65, "layer", "utterance", True, True, True, True, True),
+    (2, 9, 2048, "rms", "none", True, False, False, True, True),
+    (1, 3, 1030, "layer", "rows", False, True, True, True, False),
+    (4, 2, 2600, "layer", "utterance", True, True, False, True, False),
+    (2, 2, 8192, "rms", "rows", True, True, True, True, False),
+    (2, 70, 512, "layer", "none", False, False, False, True, False),
+    (3, 41, 520, "rms", "utterance", True, False, True, False, True),
+    (1, 130, 8, "layer", "rows", True, False, True, True, True),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", NORM, ids=str)
+def test_gated_residual_norm(case, dtype):
+    from audio8_amd import ops
+    B, T, C, kind, gate, post, bias, scale, nxt, strided = case
+    v = lambda s: 1 + rnd(C, seed=s, scale=0.2)  # noqa: E731
+    a = dict(x=rnd(B, T, C, seed=1, dtype=dtype) + 1, o=rnd(B, T, C, seed=2, dtype=dtype, scale=3.0) - 2, w=v(3) if nxt else None, b=v(4) if nxt and bias else None,
+             pw=v(5) if post else None, pb=v(6) if post and bias else None,
+             gate={"none": None, "rows": rnd(B, T, C, seed=7, dtype=dtype), "utterance": rnd(B, 1, C, seed=7, dtype=dtype)}[gate], scale=v(8) if scale else None)
+    dr, dn = rnd(B, T, C, seed=9, dtype=dtype), rnd(B, T, C, seed=10, dtype=dtype)
+    g = {k: (wide(t, 3, 4) if strided and k in ("x", "gate") else t.cuda()).requires_grad_() for k, t in a.items() if t is not None}
+    r, n = ops.gated_residual_norm(g["x"], g["o"], g.get("w"), g.get("b"), post_weight=g.get("pw"), post_bias=g.get("pb"), gate=g.get("gate"), scale=g.get("scale"),
+                                   kind=kind)
+    outs, ups = ([r, n], [dr.cuda(), dn.cuda()]) if nxt else ([r], [dr.cuda()])
+    got = dict(zip(g, torch.autograd.grad(outs, list(g.values()), ups)))
+    ref, mag = (R.residual_norm(**a, kind=kind, dr=dr, dn=dn if nxt else None, mag=m) for m in (False, True))
+    F = C / 32 + 40
+    check("r", r, ref["r"], mag["r"], F)
+    if nxt:
+        check("n", n, ref["n"], mag["n"], 2 * F)
+    else:
+        assert n is None
+    for k in g:
+        check("d" + k, got[k], ref["d" + k], mag["d" + k], 4 * F + (B * T if k not in ("x", "o") else 0))
+    with torch.no_grad():
+        r2, n2 = ops.gated_residual_norm(*(g.get(k) for k in ("x", "o", "w", "b")), post_weight=g.get("pw"), post_bias=g.get("pb"), gate=g.get("gate"), scale=g.get("scale"), kind=kind)
+    assert torch.equal(r, r2) and (n2 is None or torch.equal(n, n2))
+
+
+def test_gated_residual_norm_one_output_used_and_two_axes():
+    """Only r, or only n, carries a gradient; [frames, channels] inputs are one utterance."""
+    from audio8_amd import ops
+    T, C = 9, 96
+    a = dict(x=rnd(1, T, C, seed=1), o=rnd(1, T, C, seed=2), w=rnd(C, seed=3), b=rnd(C, seed=4), pw=rnd(C, seed=5), pb=rnd(C, seed=6), gate=rnd(1, T, C, seed=7), scale=rnd(C, seed=8))
+    up = rnd(1, T, C, seed=9)
+    for use in ("dr", "dn"):
+        g = {k: cu(t[0] if k in ("x", "o", "gate") else t, True) for k, t in a.items()}
+        r, n = ops.gated_residual_norm(g["x"], g["o"], g["w"], g["b"], post_weight=g["pw"], post_bias=g["pb"], gate=g["gate"], scale=g["scale"])
+        assert r.shape == (T, C)
+        got = dict(zip(g, torch.autograd.grad(r if use == "dr" else n, list(g.values()), up[0].cuda())))
+        ref, mag = (R.residual_norm(**a, mag=m, dr=up if use == "dr" else torch.zeros_like(up), dn=torch.zeros_like(up) if use == "dr" else up) for m in (False, True))
+        for k in g:
+            check(use + " d" + k, got[k].reshape(ref["d" + k].shape), ref["d" + k], mag["d" + k], 4 * (C / 32 + 40) + T)
+
+
+# ------------------------------------------------------------------------------------------------ empty calls
+def test_no_frames_and_no_utterances():
+    from audio8_amd import ops
+    for B, T in ((2, 0), (0, 5)):
+        x = torch.zeros(B, T, 8, device="cuda", requires_grad=True)
+        w, b = cu(rnd(8, 4, seed=1), True), cu(rnd(8, seed=2), True)
+        st = cu(rnd(B, 3, 8, seed=3), True)
+        y, out = ops.causal_conv(x, w, b, state=st, return_state=True)
+        assert y.shape == x.shape and torch.equal(out, st)
+        up = rnd(B, 3, 8, seed=4).cuda()
+        dx, dw, db, ds = torch.autograd.grad([y, out], [x, w, b, st], [torch.zeros_like(y), up])
+        assert not dw.any() and not db.any() and torch.equal(ds, up) and dx.shape == x.shape
+        A, h = cu(-torch.ones(8, 16), True), cu(rnd(B, 8, 16, seed=5), True)
+        bc = torch.zeros(B, T, 1, 16, device="cuda", requires_grad=True)
+        y, out = ops.selective_scan(x, x, A, bc, bc, state=h, return_state=True)
+        assert torch.equal(out, h)
+        up = rnd(B, 8, 16, seed=6).cuda()
+        dA, dh = torch.autograd.grad([y, out], [A, h], [torch.zeros_like(y), up])
+        assert not dA.any() and torch.equal(dh, up)
+        v = cu(rnd(8, seed=7), True)
+        r, n = ops.gated_residual_norm(x, x, v, scale=b)
+        g = torch.autograd.grad([r, n], [v, b], [torch.zeros_like(r), torch.zeros_like(n)])
+        assert not any(t.any() for t in g)
+
+
+# ------------------------------------------------------------------------------------------------ together, as a block uses them
+class Block:
+    """norm -> projection -> convolution -> scan -> projection -> gated residual norm, with the framework's own linear layers."""
+
+    def __init__(self, d=128, inner=192, N=16, K=4, rank=8):
+        self.d, self.inner, self.N, self.rank = d, inner, N, rank
+        p = lambda s, *shape, scale=1.0, at=0.0: torch.nn.Parameter(at + rnd(*shape, seed=s, scale=scale).cuda())  # noqa: E731
+        self.p = dict(w_in=p(1, 2 * inner, d, scale=d ** -0.5), conv_w=p(2, inner, K, scale=0.5), conv_b=p(3, inner, scale=0.1),
+                      w_x=p(4, rank + 2 * N, inner, scale=inner ** -0.5), w_dt=p(5, inner, rank, scale=rank ** -0.5), dt_bias=p(6, inner, scale=0.5, at=-3.0),
+                      A_log=p(7, inner, N, scale=0.5), D=p(8, inner, at=1.0, scale=0.1), w_out=p(9, d, inner, scale=inner ** -0.5),
+                      post=p(10, d, at=1.0, scale=0.1), scale=p(11, d, at=0.5, scale=0.1), nxt=p(12, d, at=1.0, scale=0.1))
+
+    def mix(self, xc, z):
+        from audio8_amd import ops
+        p, R_, N = self.p, self.rank, self.N
+        proj = ops.linear(xc, p["w_x"], None)
+        return ops.linear(proj[..., :R_], p["w_dt"], None), proj[..., R_:R_ + N], proj[..., R_ + N:], dict(D=p["D"], z=z, dt_bias=p["dt_bias"])
+
+    def ends(self, r, y, gate):
+        from audio8_amd import ops
+        return ops.gated_residual_norm(r, ops.linear(y, self.p["w_out"], None), self.p["nxt"], post_weight=self.p["post"], gate=gate, scale=self.p["scale"], kind="rms")
+
+    def forward(self, r, n, gate, states=None, lengths=None):
+        from audio8_amd import ops
+        p = self.p
+        xz = ops.linear(n, p["w_in"], None)
+        x, z = xz[..., :self.inner], xz[..., self.inner:]
+        xc, conv = ops.causal_conv(x, p["conv_w"], p["conv_b"], state=states[0] if states else None, lengths=lengths, return_state=True)
+        dt, B, C, kw = self.mix(xc, z)
+        y, h = ops.selective_scan(xc, dt, -torch.exp(p["A_log"]), B, C, state=states[1] if states else None, lengths=lengths, return_state=True, **kw)
+        return (*self.ends(r, y, gate), (conv, h))
+
+    def step(self, r, n, gate, states):
+        from audio8_amd import ops
+        p = self.p
+        xz = ops.linear(n, p["w_in"], None)
+        xc = ops.causal_conv_step(xz[:, :self.inner], states[0], p["conv_w"], p["conv_b"])
+        dt, B, C, kw = self.mix(xc, xz[:, self.inner:])
+        y = ops.selective_scan_step(xc, dt, -torch.exp(p["A_log"]), B, C, states[1], **kw)
+        return self.ends(r, y, gate)
+
+
+def test_a_block_in_chunks_and_frame_by_frame_is_the_block():
+    """One stream three ways: at once, in two chunks, frame by frame.  Same inputs per frame, f32: what differs is the order of f32 sums; two
+    applications of products over 128 .. 192 terms, 16 states and 40 frames stay within 1e-4 of the largest value (2^-24 x (16 x 40 + 200) x ~2)."""
+    blk = Block()
+    B, T = 3, 40
+    r, n, gate = (rnd(B, T, blk.d, seed=s).cuda() for s in (20, 21, 22))
+    with torch.no_grad():
+        R1, N1, (c1, h1) = blk.forward(r, n, gate)
+        parts, st = [], None
+        for a, b in ((0, 23), (23, T)):
+            pr, pn, st = blk.forward(r[:, a:b], n[:, a:b].contiguous(), gate[:, a:b], st)
+            parts.append((pr, pn))
+        s = [torch.zeros_like(c1), torch.zeros_like(h1)]
+        steps = [blk.step(r[:, t], n[:, t].contiguous(), gate[:, t], s) for t in range(T)]
+    for Rk, Nk, ck, hk in ((torch.cat([q[0] for q in parts], 1), torch.cat([q[1] for q in parts], 1), *st),
+                           (torch.stack([q[0] for q in steps], 1), torch.stack([q[1] for q in steps], 1), *s)):
+        for p, q in ((R1, Rk), (N1, Nk), (c1, ck), (h1, hk)):
+            assert (p - q).abs().max() < 1e-4 * p.abs().max()
+
+
+def test_a_block_trains_with_the_oracles_gradients_and_padding_changes_nothing():
+    """Gradients of every parameter of a block against float64, and a padded batch against its utterances one by one.  f32 throughout; a gradient is
+    a sum over B T = 60 frames through three products and the scan: 2^-24 x (16 T + 3 x 192 + B T + 100) x 4 (its chain of magnitudes) < 4e-4."""
+    import audio8_amd.ops as ops
+    blk = Block()
+    lengths = [30, 11, 19]
+    B, T = 3, 30
+    r, n, gate, ur, un = (rnd(B, T, blk.d, seed=s) for s in (20, 21, 22, 23, 24))
+    live = torch.arange(T)[None] < torch.tensor(lengths)[:, None]
+    ur, un = ur * live[..., None], un * live[..., None]
+    was = ops.compute_dtype()
+    ops.set_compute_dtype(torch.float32)
+    try:
+        Rg, Ng, _ = blk.forward(r.cuda(), n.cuda(), gate.cuda(), lengths=torch.tensor(lengths, dtype=torch.int32).cuda())
+        got = dict(zip(blk.p, torch.autograd.grad([Rg, Ng], list(blk.p.values()), [ur.cuda(), un.cuda()])))
+    finally:
+        ops.set_compute_dtype(was)
+    p = {k: v.detach().double().cpu().requires_grad_() for k, v in blk.p.items()}
+    loss = 0.0
+    for i, e in enumerate(lengths):
+        x_, z_ = (n[i, :e].double() @ p["w_in"].t()).split(blk.inner, -1)
+        ext = torch.cat([torch.zeros(3, blk.inner, dtype=torch.float64), x_])
+        xc = R.silu((ext.unfold(0, 4, 1) * p["conv_w"]).sum(-1) + p["conv_b"])
+        dt, Bm, Cm = (xc @ p["w_x"].t()).split([blk.rank, blk.N, blk.N], -1)
+        s = torch.logaddexp(dt @ p["w_dt"].t() + p["dt_bias"], torch.zeros((), dtype=torch.float64))
+        A, h, ys = -torch.exp(p["A_log"]), torch.zeros(blk.inner, blk.N, dtype=torch.float64), []
+        for t in range(e):
+            h = torch.exp(s[t][:, None] * A) * h + (s[t] * xc[t])[:, None] * Bm[t]
+            ys.append((h @ Cm[t] + p["D"] * xc[t]) * R.silu(z_[t]))
+        o = torch.stack(ys) @ p["w_out"].t()
+        rr = r[i, :e].double() + p["scale"] * gate[i, :e].double() * o * torch.rsqrt((o * o).mean(-1, keepdim=True) + 1e-6) * p["post"]
+        nn_ = rr * torch.rsqrt((rr * rr).mean(-1, keepdim=True) + 1e-6) * p["nxt"]
+        for k, v, w in (("r", rr, Rg), ("n", nn_, Ng)):
+            assert (w[i, :e].double().cpu() - v).abs().max() < 1e-4 * v.abs().max(), (k, i)
+        loss = loss + (rr * ur[i, :e].double()).sum() + (nn_ * un[i, :e].double()).sum()
+    for (k, v), g in zip(p.items(), torch.autograd.grad(loss, list(p.values()))):
+        assert (got[k].double().cpu() - g).abs().max() < 4e-4 * g.abs().max(), k
+
+
+def test_parameter_gradients_go_straight_into_grad_when_the_stepper_asks():
+    import audio8_amd.ops as ops
+    p = {k: torch.nn.Parameter(v.cuda()) for k, v in dict(w=rnd(24, 4, seed=1), b=rnd(24, seed=2), A=-rnd(24, 16, seed=3).abs(), D=rnd(24, seed=4), db=rnd(24, seed=5),
+                                                          n=rnd(24, seed=6), s=rnd(24, seed=7)).items()}
+    x, bc = rnd(2, 20, 24, seed=8).cuda(), rnd(2, 20, 16, seed=9).cuda()
+
+    def loss():
+        y = ops.causal_conv(x, p["w"], p["b"])
+        y = ops.selective_scan(y, y, p["A"], bc, bc, D=p["D"], dt_bias=p["db"])
+        r, n = ops.gated_residual_norm(x, y, p["n"], scale=p["s"], kind="rms")
+        return (r * n).sum()
+    want = torch.autograd.grad(loss(), list(p.values()))
+    for v in p.values():
+        v.grad = torch.ones_like(v)
+    seen = []
+    was = ops.DIRECT_GRADS, ops.GRAD_READY_HOOK
+    ops.DIRECT_GRADS, ops.GRAD_READY_HOOK = True, seen.append
+    try:
+        loss().backward()
+    finally:
+        ops.DIRECT_GRADS, ops.GRAD_READY_HOOK = was
+    assert {id(v) for v in seen} == {id(v) for v in p.values()} and len(seen) == len(p)
+    for v, g in zip(p.values(), want):
+        assert torch.allclose(v.grad, 1 + g, rtol=2.0 ** -22, atol=2.0 ** -22 * float(g.abs().max() + 1))
+
+
+# ------------------------------------------------------------------------------------------------ streams, graphs, repeated calls
+def _train(ops, v):
+    y = ops.causal_conv(v["x"], v["w"], v["b"], lengths=v["n"])
+    y = ops.selective_scan(y, v["dt"], v["A"], v["B"], v["C"], D=v["D"], z=v["z"], dt_bias=v["db"], lengths=v["n"])
+    r, n = ops.gated_residual_norm(v["x"], y, v["g"], gate=v["gate"], scale=v["s"], kind="rms")
+    leaves = [v[k] for k in ("x", "w", "b", "dt", "A", "B", "C", "D", "z", "db", "g", "gate", "s")]
+    return [r, n, *torch.autograd.grad([r, n], leaves, [v["ur"], v["un"]])]
+
+
+def _train_inputs(seed, dtype=torch.bfloat16, B=2, T=75, D=136):
+    f = lambda k, *s, d=dtype: rnd(*s, seed=seed * 100 + k, dtype=d).cuda().requires_grad_()  # noqa: E731
+    f32 = torch.float32
+    v = dict(x=f(1, B, T, D), w=f(2, D, 4, d=f32), b=f(3, D, d=f32), dt=f(4, B, T, D), B=f(6, B, T, 16), C=f(7, B, T, 16), D=f(8, D, d=f32), z=f(9, B, T, D),
+             db=f(10, D, d=f32), g=f(11, D, d=f32), gate=f(12, B, 1, D), s=f(13, D, d=f32))
+    v["A"] = (-rnd(D, 16, seed=seed * 100 + 5).exp()).cuda().requires_grad_()
+    v["ur"], v["un"] = rnd(B, T, D, seed=seed * 100 + 14, dtype=dtype).cuda(), rnd(B, T, D, seed=seed * 100 + 15, dtype=dtype).cuda()
+    v["n"] = torch.tensor([T, T // 3], dtype=torch.int32).cuda()
+    return v
+
+
+def test_the_same_call_gives_the_same_bits_on_any_stream():
+    from audio8_amd import ops
+    v = _train_inputs(1)
+    want = _train(ops, v)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = [t for _ in range(3) for t in _train(ops, v)]
+    here = [t for _ in range(3) for t in _train(ops, v)]           # two streams at once: no workspace is shared
+    torch.cuda.synchronize()
+    for got in (there, here):
+        for i, t in enumerate(got):
+            assert torch.equal(t, want[i % len(want)])
+
+
+def test_two_captured_training_steps_replay_with_new_inputs():
+    from audio8_amd import ops
+    vs = [_train_inputs(2), _train_inputs(3)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for v in vs:
+            _train(ops, v)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for v in vs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_train(ops, v))
+        graphs.append(g)
+    for turn in range(3):
+        with torch.no_grad():
+            for i, v in enumerate(vs):
+                fresh = _train_inputs(10 + 2 * turn + i)
+                for k in v:
+                    v[k].copy_(fresh[k])
+        want = [_train(ops, v) for v in vs]
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for got, w in zip(outs, want):
+            for p, q in zip(got, w):
+                assert torch.equal(p, q)
+
+
+def test_captured_steps_carry_their_state():
+    from audio8_amd import ops
+    B, D, N, K = 3, 70, 16, 4
+    x, w = rnd(B, D, seed=1).cuda(), rnd(D, K, seed=2).cuda()
+    dt, A = rnd(B, D, seed=3).cuda(), -rnd(D, N, seed=4).exp().cuda()
+    bm = rnd(B, 1, N, seed=5).cuda()
+
+    def step(conv, h):
+        y = ops.causal_conv_step(x, conv, w)
+        return ops.selective_scan_step(y, dt, A, bm, bm, h)
+    fresh = lambda: (torch.zeros(B, K - 1, D, device="cuda"), torch.zeros(B, D, N, device="cuda"))  # noqa: E731
+    a, b = fresh(), fresh()
+    step(*fresh())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = step(*a)
+    for t in a:
+        t.zero_()
+    for t in range(4):
+        x.copy_(rnd(B, D, seed=30 + t))
+        want = step(*b)
+        g.replay()
+        assert torch.equal(y, want) and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_a_step_marks_its_state_as_changed():
+    """A state that a training call saved for its backward and a step then changed is refused by the tape, not silently used."""
+    from audio8_amd import ops
+    x, w = cu(rnd(1, 5, 8, seed=1), True), rnd(8, 4, seed=2).cuda()
+    st = torch.zeros(1, 3, 8, device="cuda")
+    y = ops.causal_conv(x, w, state=st)
+    with torch.no_grad():
+        ops.causal_conv_step(x[:, 0], st, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
