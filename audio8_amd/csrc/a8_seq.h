@@ -30,6 +30,14 @@ A8_DEV float softplus_f(float x) {
     return fmaf(s, r, fmaxf(x, 0.f));
 }
 
+// A block barrier for LDS only: __syncthreads also drains the wave's global loads and stores, which would put the latency of every prefetch and
+// of every output store on the path of each tile.
+A8_DEV void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // `planes` column sums over `rows` partial rows [rows][planes][C]: plane q < np goes to major[c * np + q] (a [C][np] matrix), plane np + i to
 // minor[i][c]; null targets are skipped.  add = 1 accumulates.  Summed in a fixed order: the same inputs give the same bits.
 struct A8SeqReduce {

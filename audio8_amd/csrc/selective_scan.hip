@@ -6,131 +6,208 @@
 //   dD = u sum_n q B + sum_n A k_t,  k_t = exp(D_t A) q_t h_{t-1};   dA = sum_t k_t D_t;   d dt = dD sigmoid(dt + dt_bias)
 // (c_{t-1} = exp(D_t A) q_t, so k_t = c_{t-1} h_{t-1}: the adjoint's own product is reused).
 //
-// Layout: a lane is a channel, a wave is 4 states of 64 channels, a block is ceil(N / 4) waves of the same 64 channels: the frame inputs are
-// read along the channels (64 lanes, 128 B in bf16, any alignment), B and C are LDS broadcasts, no state is ever exchanged between lanes, and
-// only the sums over states (y; q B, A k) cross waves, through LDS once per tile of 16 frames.  softplus / silu run once per (frame, channel),
-// split over the block's waves, not once per state.
+// Layout: a lane is a channel, a wave is NS states of 64 channels, a block is ceil(N / NS) waves of the same 64 channels: the frame inputs are
+// read along the channels (64 lanes, 128 B in bf16, any alignment), no state is ever exchanged between lanes, and only the sums over states
+// (y; q B, A k) cross waves, through LDS once per tile of 16 frames.  softplus / silu run once per (frame, channel), split over the block's
+// waves, not once per state.  A wave's B and C of a tile (16 NS values each) sit in NS VGPRs, the same 16 values in each row of 16 lanes: the
+// row broadcast of a DPP operand hands them to the multiply for nothing (read as LDS broadcasts they took 32 16-byte reads per wave and tile).
 // Everything between the inputs and the outputs is f32: steps, decays, states, adjoints and all sums.
 #include "a8_seq.h"
 #include "a8hip_internal.h"
+#include <utility>
 
 namespace {
 
-constexpr int TT = 16;      // frames of a tile: a wave's 4 states x 16 frames of a and h live in registers in the backward
+constexpr int TT = 16;      // frames of a tile
 constexpr int CH = 64;      // channels of a block
-constexpr int NS = 4;       // states of a wave
+constexpr int FNS = 2;      // states of a wave, forward: 8 waves for 16 states, two per SIMD (one wave alone issues a VALU operation every ~9 cycles, two every ~5)
+constexpr int BNS = 4;      // states of a wave, backward: 16 frames x 4 states of decays and of states live in registers
 
 struct ScanArgs {
     a8_selective_scan_desc d;
     int cpg, tpg, tiles;               // channels and channel tiles per group, frame tiles of T
-    float* part;                       // backward: [B][N + 2][D] partial dA planes, dD, ddt_bias
+    int chunks, tpc;                   // frame chunks that run side by side, tiles per chunk
+    float* ends;                       // chunks > 1: [B][chunks][N + 1][D] each chunk's own end state (backward: adjoint at its beginning) and sum of steps
+    float* part;                       // backward: [B][chunks][N + 2][D] partial dA planes, dD, ddt_bias
     float* part_b; float* part_c;      // backward: [tpg][B][T][G][N] partial dB, dC
 };
 
-struct Where { int b, g, ct, c0, ch; bool live; int64_t chan; int len; };
-A8_DEV Where locate(const ScanArgs& p, int lane) {
+struct Where { int b, g, ct, ch, len, ck, i0, i1; bool live; };      // i0 .. i1: the chunk's tiles that hold valid frames
+A8_DEV Where locate(const ScanArgs& p, int lane, int first_chunk, int nchunks) {
     Where w;
     int i = blockIdx.x;
     w.ct = i % p.tpg; i /= p.tpg;
-    w.g = i % p.d.G; w.b = i / p.d.G;
+    w.g = i % p.d.G; i /= p.d.G;
+    w.ck = first_chunk + i % nchunks; w.b = i / nchunks;
     const int c = w.ct * CH + lane;
     w.live = c < p.cpg;
     w.ch = w.g * p.cpg + min(c, p.cpg - 1);
     w.len = seq_len(p.d.lengths, w.b, p.d.T);
+    w.i0 = w.ck * p.tpc;
+    w.i1 = min(w.i0 + p.tpc, (w.len + TT - 1) / TT);
     return w;
 }
 
-template <typename T> A8_DEV float ldf(const void* p, int64_t i) { return to_f(((const T*)p)[i]); }
+// row (b, t) of a strided input: a wave-uniform address, so that a load is one scalar base and one 32-bit lane offset
+template <typename T> A8_DEV const T* row_of(const void* p, int64_t bs, int64_t ts, int b, int t) { return (const T*)p + (b * bs + t * ts); }
 
-// B or C of one tile, one value per thread (TT x 4 NW values = the block's threads): frame tid / (4 NW), state tid % (4 NW)
-template <typename T, int NW> A8_DEV float load_bc(const void* base, int64_t bs, int64_t ts, int64_t gs, const ScanArgs& p, const Where& w, int t0) {
-    const int n = threadIdx.x % (NS * NW), t = t0 + threadIdx.x / (NS * NW);
-    return t < w.len && n < p.d.N ? ldf<T>(base, w.b * bs + t * ts + w.g * gs + n) : 0.f;
+// value I of the 16 that every row of 16 lanes holds in v, as a DPP operand
+template <int I> A8_DEV float row_value(float v) { return dpp_f<0x150 + I>(v); }
+template <int... I, typename F> A8_DEV void unroll_impl(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>()), ...); }
+template <int N, typename F> A8_DEV void unroll(F f) { unroll_impl(std::make_integer_sequence<int, N>(), f); }
+
+// The inputs of one tile as a thread holds them between their loads and their use a tile later.  Loads are unconditional: a frame behind the
+// end reads the last valid one and is dropped where it is used, so nothing waits for a load before its time.
+template <typename T, int NW, int NS, bool Z, bool DY> struct TileRegs {
+    static constexpr int EP = TT / NW, BC = NS * NW;       // (frame, channel) elements per thread: frames wv, wv + NW, ...; states of the block
+    T u[EP], dt[EP], z[Z ? EP : 1], dy[DY ? EP : 1], b, c;
+    A8_DEV void load(const a8_selective_scan_desc& d, const Where& w, int wv, int t0) {
+#pragma unroll
+        for (int j = 0; j < EP; ++j) {
+            const int t = min(t0 + wv + NW * j, w.len - 1);
+            u[j] = row_of<T>(d.u, d.u_bs, d.u_ts, w.b, t)[(uint32_t)w.ch];
+            dt[j] = row_of<T>(d.dt, d.dt_bs, d.dt_ts, w.b, t)[(uint32_t)w.ch];
+            if constexpr (Z) z[j] = row_of<T>(d.z, d.z_bs, d.z_ts, w.b, t)[(uint32_t)w.ch];
+            if constexpr (DY) dy[j] = row_of<T>(d.dy, d.dy_bs, d.dy_ts, w.b, t)[(uint32_t)w.ch];
+        }
+        // B and C: one value per thread (at most: TT BC <= 64 NW), frame tid / BC, state tid % BC
+        const int n = min((int)threadIdx.x % BC, d.N - 1), t = min(t0 + (int)threadIdx.x / BC, w.len - 1);
+        b = ((const T*)d.Bm)[w.b * d.b_bs + t * d.b_ts + w.g * d.b_gs + n];
+        c = ((const T*)d.Cm)[w.b * d.c_bs + t * d.c_ts + w.g * d.c_gs + n];
+    }
+    A8_DEV void stage_bc(const a8_selective_scan_desc& d, const Where& w, int t0, float* s_b, float* s_c) const {       // -> LDS [TT][BC]
+        const int tid = threadIdx.x;
+        if (TT * BC == 64 * NW || tid < TT * BC) {
+            const bool in = tid % BC < d.N && t0 + tid / BC < w.len;
+            s_b[tid] = in ? to_f(b) : 0.f;
+            s_c[tid] = in ? to_f(c) : 0.f;
+        }
+    }
+};
+// a wave's values of an LDS tile [TT][BC]: v[k] holds frames 16 / NS * k .., frame (l & 15) / NS, state n0 + l % NS, in every row of 16 lanes
+template <int NS, int BC> A8_DEV void wave_bc(float (&v)[NS], const float* s, int n0, int lane) {
+#pragma unroll
+    for (int k = 0; k < NS; ++k) v[k] = s[(16 / NS * k + (lane & 15) / NS) * BC + n0 + lane % NS];
 }
+// acc += sum_n row value (I + n) of v * x[n], and its elementwise form x[n] += row value (I + n) of v * g: multiply-adds with the row broadcast in
+// the DPP operand (the compiler folds it into multiplies only).  A DPP operand may not be read within two wait states of a VALU write of its register,
+// which the compiler does not see here: one s_nop in front of the group covers a copy that it may have placed there.
+template <int I> A8_DEV void row_dot(float& acc, float v, const float (&x)[2]) {
+    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 row_newbcast:%4 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %0, %1, %3 row_newbcast:%5 row_mask:0xf bank_mask:0xf"
+        : "+v"(acc) : "v"(v), "v"(x[0]), "v"(x[1]), "n"(I), "n"(I + 1));
+}
+template <int I> A8_DEV void row_dot(float& acc, float v, const float (&x)[4]) {
+    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
+        : "+v"(acc) : "v"(v), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3));
+}
+template <int I> A8_DEV void row_axpy(float (&x)[4], float v, float g) {
+    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %4, %5 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
+        : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]) : "v"(v), "v"(g), "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3));
+}
+// element (t, n) of wave_bc's values
+template <int NS, int T_, int N_> A8_DEV float bc_at(const float (&v)[NS]) { return row_value<(T_ % (16 / NS)) * NS + N_>(v[T_ / (16 / NS)]); }
 
-template <typename T, int NW> __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs p) {
-    constexpr int EP = TT / NW;                            // (frame, channel) elements of a tile per thread
+// ENDS: only each chunk's own end state (from zero) and the sum of its steps; else the chunk itself, from the state that the chunks before it leave.
+template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs p) {
+    constexpr int NS = FNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dx[TT][CH];                        // {D, D u}
-    __shared__ __align__(16) float s_b[TT][NS * NW], s_c[TT][NS * NW];
-    __shared__ float s_y[NW][TT][CH];
+    __shared__ float s_b[TT * BC], s_c[TT * BC];
+    __shared__ float s_y[ENDS ? 1 : NW][TT][CH];
     const a8_selective_scan_desc& d = p.d;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, n0 = wv * NS;
-    const Where w = locate(p, lane);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = wv * NS;
+    const Where w = locate(p, lane, 0, ENDS ? p.chunks - 1 : p.chunks);
     const float bias = d.dt_bias ? d.dt_bias[w.ch] : 0.f, skip = d.Dskip ? d.Dskip[w.ch] : 0.f;
-    float A2[NS], h[NS];
+    const bool sp = d.softplus != 0;
+    float A2[NS], h[NS], sum = 0.f;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const bool has = n0 + n < d.N;
         A2[n] = has ? d.A[(int64_t)w.ch * d.N + n0 + n] * SEQ_LOG2E : 0.f;
-        h[n] = has && d.h0 ? d.h0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
+        h[n] = !ENDS && has && d.h0 ? d.h0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
     }
-    const int ntile = (w.len + TT - 1) / TT;
-    float u[EP], dt[EP], z[EP], rb = 0.f, rc = 0.f;
-    auto load = [&](int t0) {
-#pragma unroll
-        for (int j = 0; j < EP; ++j) {
-            const int t = t0 + wv + NW * j;
-            const bool in = t < w.len;
-            u[j] = in ? ldf<T>(d.u, w.b * d.u_bs + t * d.u_ts + w.ch) : 0.f;
-            dt[j] = in ? ldf<T>(d.dt, w.b * d.dt_bs + t * d.dt_ts + w.ch) : 0.f;
-            z[j] = in && d.z ? ldf<T>(d.z, w.b * d.z_bs + t * d.z_ts + w.ch) : 0.f;
-        }
-        rb = load_bc<T, NW>(d.Bm, d.b_bs, d.b_ts, d.b_gs, p, w, t0);
-        rc = load_bc<T, NW>(d.Cm, d.c_bs, d.c_ts, d.c_gs, p, w, t0);
-    };
-    if (ntile > 0) load(0);
-    for (int i = 0; i < ntile; ++i) {
-        const int t0 = i * TT;
-        float cu[EP], cz[EP];
-#pragma unroll
-        for (int j = 0; j < EP; ++j) {
-            const int t = wv + NW * j;
-            const float raw = dt[j] + bias, D = t0 + t < w.len ? (d.softplus ? softplus_f(raw) : raw) : 0.f;
-            s_dx[t][lane] = make_float2(D, D * u[j]);
-            cu[j] = u[j]; cz[j] = z[j];
-        }
-        s_b[0][threadIdx.x] = rb;                          // ([TT][4 NW] flat)
-        s_c[0][threadIdx.x] = rc;
-        if (d.ckpt && w.live)
+    if constexpr (!ENDS)
+        for (int k = 0; k < w.ck; ++k) {                   // the states that the chunks before leave: at most a few dozen, each two loads away
+            const float* const e = p.ends + ((int64_t)w.b * p.chunks + k) * (d.N + 1) * d.D + w.ch;
+            const float s = e[(int64_t)d.N * d.D];
 #pragma unroll
             for (int n = 0; n < NS; ++n)
-                if (n0 + n < d.N) d.ckpt[(((int64_t)w.b * p.tiles + i) * d.N + n0 + n) * d.D + w.ch] = h[n];
-        __syncthreads();
-        if (i + 1 < ntile) load(t0 + TT);
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const float2 dx = s_dx[t][lane];
-            float y = 0.f;
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                h[n] = fmaf(__builtin_amdgcn_exp2f(dx.x * A2[n]), h[n], dx.y * s_b[t][n0 + n]);
-                y = fmaf(s_c[t][n0 + n], h[n], y);
-            }
-            s_y[wv][t][lane] = y;
+                if (n0 + n < d.N) h[n] = fmaf(__builtin_amdgcn_exp2f(A2[n] * s), h[n], e[(int64_t)(n0 + n) * d.D]);
         }
-        __syncthreads();
+    TileRegs<T, NW, NS, Z, false> nx, cu;                  // the next tile's inputs, this tile's u and z
+    auto stage = [&](int t0) {                             // nx -> LDS
 #pragma unroll
         for (int j = 0; j < EP; ++j) {
             const int t = wv + NW * j;
-            float y = skip * cu[j];
-#pragma unroll
-            for (int v = 0; v < NW; ++v) y += s_y[v][t][lane];
-            if (d.z) y *= silu_f(cz[j]);
-            if (w.live && t0 + t < w.len) ((T*)d.y)[((int64_t)w.b * d.T + t0 + t) * d.D + w.ch] = from_f<T>(y);
+            const float raw = to_f(nx.dt[j]) + bias, s = sp ? softplus_f(raw) : raw, u = to_f(nx.u[j]);
+            const bool in = t0 + t < w.len;
+            s_dx[t][lane] = make_float2(in ? s : 0.f, in ? s * u : 0.f);
         }
+        nx.stage_bc(d, w, t0, s_b, s_c);
+    };
+    if (w.i0 < w.i1) { nx.load(d, w, wv, w.i0 * TT); stage(w.i0 * TT); }
+    for (int i = w.i0; i < w.i1; ++i) {
+        const int t0 = i * TT;
+        cu = nx;
+        if (!ENDS && d.ckpt && w.live) {
+            float* const ck = d.ckpt + (((int64_t)w.b * p.tiles + i) * d.N + n0) * d.D;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+                if (n0 + n < d.N) ck[(int64_t)n * d.D + w.ch] = h[n];
+        }
+        lds_barrier();
+        if (i + 1 < w.i1) nx.load(d, w, wv, t0 + TT);
+        float bv[NS], cv[NS];
+        wave_bc<NS, BC>(bv, s_b, n0, lane);
+        if constexpr (!ENDS) wave_bc<NS, BC>(cv, s_c, n0, lane);
+        unroll<TT>([&](auto tc) {
+            constexpr int t = decltype(tc)::value;
+            const float2 dx = s_dx[t][lane];
+            float y = 0.f;
+            if constexpr (ENDS) sum += dx.x;
+            unroll<NS>([&](auto nc) {
+                constexpr int n = decltype(nc)::value;
+                h[n] = fmaf(__builtin_amdgcn_exp2f(dx.x * A2[n]), h[n], dx.y * bc_at<NS, t, n>(bv));
+            });
+            if constexpr (!ENDS) {
+                row_dot<(t % (16 / NS)) * NS>(y, cv[t / (16 / NS)], h);
+                s_y[wv][t][lane] = y;
+            }
+        });
+        lds_barrier();
+        if (i + 1 < w.i1) stage(t0 + TT);                  // (the loads are a tile old; the stores below are not waited for)
+        if constexpr (!ENDS)
+#pragma unroll
+            for (int j = 0; j < EP; ++j) {
+                const int t = wv + NW * j;
+                float y = skip * to_f(cu.u[j]);
+#pragma unroll
+                for (int v = 0; v < NW; ++v) y += s_y[v][t][lane];
+                if constexpr (Z) y *= silu_f(to_f(cu.z[j]));
+                if (t0 + t < w.len && w.live) ((T*)d.y + ((int64_t)w.b * d.T + t0 + t) * d.D)[(uint32_t)w.ch] = from_f<T>(y);
+            }
     }
-    if (w.live) {
-        for (int t = w.len + wv; t < d.T; t += NW) ((T*)d.y)[((int64_t)w.b * d.T + t) * d.D + w.ch] = from_f<T>(0.f);
-        if (d.h_out)
+    if (!w.live) return;
+    if constexpr (ENDS) {
+        float* const e = p.ends + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 1) * d.D + w.ch;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+            if (n0 + n < d.N) e[(int64_t)(n0 + n) * d.D] = h[n];
+        if (wv == 0) e[(int64_t)d.N * d.D] = sum;
+    } else {
+        for (int t = max(w.i0 * TT, w.len) + wv; t < min((w.i0 + p.tpc) * TT, d.T); t += NW) ((T*)d.y)[((int64_t)w.b * d.T + t) * d.D + w.ch] = from_f<T>(0.f);
+        if (d.h_out && w.ck == p.chunks - 1)
 #pragma unroll
             for (int n = 0; n < NS; ++n)
                 if (n0 + n < d.N) d.h_out[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] = h[n];
     }
 }
 
-// Sum of 64 register values over the wave's 64 lanes, scattered: lane l returns the total of v[l].  Each step pairs lanes that differ in one
-// index bit, adds, and keeps the half of the values whose index has the lane's bit: 63 adds instead of 64 x 6.  The upper two bits go
-// through the half-wave and half-row register swaps (no select needed), the lower four through DPP (xor 8, mirror of 8, xor 2, xor 1).
+// Sums over a wave's 64 lanes of 64 values that come 16 at a time (4 frames x 4 states), scattered: lane l gets the total of value l.  A step pairs
+// lanes that differ in one bit of the index, adds, and keeps the half of the values whose index has the lane's bit: one add per value left instead
+// of six per value.  Inside a row of 16 lanes through DPP (two selects and an add per value left: ~11 cycles), across the rows through the
+// half-wave and half-row register swaps (~15 cycles): the rows come last, when one value per 16 is left.
 template <int CTRL, int M> A8_DEV void scatter_step(float* v, bool upper) {
 #pragma unroll
     for (int i = 0; i < M; ++i) {
@@ -138,169 +215,216 @@ template <int CTRL, int M> A8_DEV void scatter_step(float* v, bool upper) {
         v[i] = keep + dpp_f<CTRL>(send);
     }
 }
-A8_DEV float wave_sum_scatter64(float (&v)[64], int lane) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 32]), false, false);
-        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 16]), false, false);
-        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    }
+A8_DEV float row_sum_scatter16(float (&v)[16], int lane) {      // lane l: the sum of v[l & 15] over its row
     scatter_step<0x128, 8>(v, lane & 8);          // row_ror:8
-    scatter_step<0x141, 4>(v, lane & 4);          // row_half_mirror
+    scatter_step<0x141, 4>(v, lane & 4);          // row_half_mirror: flips the bits below too, on which nothing depends yet
     scatter_step<0x4E, 2>(v, lane & 2);           // quad_perm xor 2
     scatter_step<0xB1, 1>(v, lane & 1);           // quad_perm xor 1
     return v[0];
 }
+A8_DEV float rows_sum_scatter4(const float (&v)[4]) {           // row r: the sum of v[r] over the rows
+    auto swap_add32 = [](float x, float y) {
+        auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+        return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    };
+    const float lo = swap_add32(v[0], v[2]), hi = swap_add32(v[1], v[3]);
+    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
 
-template <typename T, int NW> __global__ __launch_bounds__(64 * NW) void scan_bwd_kernel(ScanArgs p) {
-    constexpr int EP = TT / NW;
-    __shared__ float2 s_dx[TT][CH];                        // {D, D u}
-    __shared__ float s_g[TT][CH];                          // dout silu(z)
-    __shared__ __align__(16) float s_b[TT][NS * NW], s_c[TT][NS * NW];
-    __shared__ float s_qb[NW][TT][CH], s_ak[NW][TT][CH], s_y[NW][TT][CH];
+// ENDS: only the adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps.
+template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void scan_bwd_kernel(ScanArgs p) {
+    constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
+    __shared__ float2 s_dxs[2][TT][CH];                    // {D, D u}, by tile parity
+    __shared__ float s_gs[2][TT][CH];                      // dout silu(z)
+    __shared__ float s_b[TT * BC], s_c[TT * BC];
+    __shared__ float s_qb[ENDS ? 1 : NW][TT][CH], s_ak[ENDS ? 1 : NW][TT][CH], s_y[Z && !ENDS ? NW : 1][TT][CH];
     const a8_selective_scan_desc& d = p.d;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, n0 = wv * NS;
-    const Where w = locate(p, lane);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = wv * NS;
+    const Where w = locate(p, lane, ENDS ? 1 : 0, ENDS ? p.chunks - 1 : p.chunks);
     const float bias = d.dt_bias ? d.dt_bias[w.ch] : 0.f, skip = d.Dskip ? d.Dskip[w.ch] : 0.f;
-    float A[NS], A2[NS], c[NS], dA[NS] = {};
+    const bool sp = d.softplus != 0;
+    float A[NS], A2[NS], c[NS], dA[NS] = {}, sum = 0.f;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const bool has = n0 + n < d.N;
         A[n] = has ? d.A[(int64_t)w.ch * d.N + n0 + n] : 0.f;
         A2[n] = A[n] * SEQ_LOG2E;
-        c[n] = has && w.live && d.dh_out ? d.dh_out[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
+        c[n] = !ENDS && has && w.live && d.dh_out ? d.dh_out[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
     }
+    if constexpr (!ENDS)
+        for (int k = p.chunks - 1; k > w.ck; --k) {
+            const float* const e = p.ends + ((int64_t)w.b * p.chunks + k) * (d.N + 1) * d.D + w.ch;
+            const float s = e[(int64_t)d.N * d.D];
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+                if (n0 + n < d.N && w.live) c[n] = fmaf(__builtin_amdgcn_exp2f(A2[n] * s), c[n], e[(int64_t)(n0 + n) * d.D]);
+        }
     float dskip = 0.f, dbias = 0.f;
-    const int ntile = (w.len + TT - 1) / TT;
-    float u[EP], dt[EP], z[EP], dy[EP], rb = 0.f, rc = 0.f, rh[NS] = {};
+    TileRegs<T, NW, NS, Z, true> nx, cu;
+    float rh[NS] = {};
     auto load = [&](int i) {
+        nx.load(d, w, wv, i * TT);
+        if constexpr (!ENDS) {
+            const float* const ck = d.ckpt + (((int64_t)w.b * p.tiles + i) * d.N + n0) * d.D;
 #pragma unroll
-        for (int j = 0; j < EP; ++j) {
-            const int t = i * TT + wv + NW * j;
-            const bool in = t < w.len && w.live;           // (an absent channel contributes nothing to dB and dC)
-            u[j] = in ? ldf<T>(d.u, w.b * d.u_bs + t * d.u_ts + w.ch) : 0.f;
-            dt[j] = in ? ldf<T>(d.dt, w.b * d.dt_bs + t * d.dt_ts + w.ch) : 0.f;
-            z[j] = in && d.z ? ldf<T>(d.z, w.b * d.z_bs + t * d.z_ts + w.ch) : 0.f;
-            dy[j] = in ? ldf<T>(d.dy, w.b * d.dy_bs + t * d.dy_ts + w.ch) : 0.f;
+            for (int n = 0; n < NS; ++n) rh[n] = n0 + n < d.N ? ck[(int64_t)n * d.D + w.ch] : 0.f;
         }
-        rb = load_bc<T, NW>(d.Bm, d.b_bs, d.b_ts, d.b_gs, p, w, i * TT);
-        rc = load_bc<T, NW>(d.Cm, d.c_bs, d.c_ts, d.c_gs, p, w, i * TT);
-#pragma unroll
-        for (int n = 0; n < NS; ++n) rh[n] = w.live && n0 + n < d.N ? d.ckpt[(((int64_t)w.b * p.tiles + i) * d.N + n0 + n) * d.D + w.ch] : 0.f;
     };
-    if (ntile > 0) load(ntile - 1);
-    for (int i = ntile - 1; i >= 0; --i) {
+    auto stage = [&](int t0) {
+#pragma unroll
+        for (int j = 0; j < EP; ++j) {
+            const int t = wv + NW * j;
+            const float raw = to_f(nx.dt[j]) + bias, s = sp ? softplus_f(raw) : raw, u = to_f(nx.u[j]);
+            const bool in = t0 + t < w.len && w.live;      // (an absent channel contributes nothing to dB and dC)
+            s_dxs[t0 / TT & 1][t][lane] = make_float2(in ? s : 0.f, in ? s * u : 0.f);
+            float g = to_f(nx.dy[j]);
+            if constexpr (Z) g *= silu_f(to_f(nx.z[j]));
+            s_gs[t0 / TT & 1][t][lane] = in ? g : 0.f;
+        }
+        nx.stage_bc(d, w, t0, s_b, s_c);
+    };
+    if (w.i0 < w.i1) { load(w.i1 - 1); stage((w.i1 - 1) * TT); }
+    for (int i = w.i1 - 1; i >= w.i0; --i) {
         const int t0 = i * TT;
-        float cu[EP], cr[EP], cz[EP], cdy[EP], a[TT][NS], h[TT + 1][NS];
+        const float2 (&s_dx)[TT][CH] = s_dxs[i & 1];
+        const float (&s_g)[TT][CH] = s_gs[i & 1];
+        cu = nx;
+        float a[TT][NS], h[TT + 1][NS], gb[4], gc[4];      // decays, states; dB's and dC's row sums of each 4 frames
 #pragma unroll
-        for (int j = 0; j < EP; ++j) {
-            const int t = wv + NW * j;
-            const float raw = dt[j] + bias, D = t0 + t < w.len ? (d.softplus ? softplus_f(raw) : raw) : 0.f;
-            s_dx[t][lane] = make_float2(D, D * u[j]);
-            s_g[t][lane] = d.z ? dy[j] * silu_f(z[j]) : dy[j];
-            cu[j] = u[j]; cr[j] = raw; cz[j] = z[j]; cdy[j] = dy[j];
-        }
-        s_b[0][threadIdx.x] = rb;
-        s_c[0][threadIdx.x] = rc;
+        for (int n = 0; n < NS; ++n) h[0][n] = w.live ? rh[n] : 0.f;
+        lds_barrier();
+        if (i > w.i0) load(i - 1);
+        float bv[NS], cv[NS];
+        wave_bc<NS, BC>(bv, s_b, n0, lane);
+        wave_bc<NS, BC>(cv, s_c, n0, lane);
+        if constexpr (!ENDS)
+            unroll<TT>([&](auto tc) {                      // the tile's states again, from the saved state before it
+                constexpr int t = decltype(tc)::value;
+                const float2 dx = s_dx[t][lane];
+                float y = 0.f;
+                unroll<NS>([&](auto nc) {
+                    constexpr int n = decltype(nc)::value;
+                    a[t][n] = __builtin_amdgcn_exp2f(dx.x * A2[n]);
+                    h[t + 1][n] = fmaf(a[t][n], h[t][n], dx.y * bc_at<NS, t, n>(bv));
+                });
+                if constexpr (Z) {
+                    row_dot<(t % 4) * 4>(y, cv[t / 4], h[t + 1]);
+                    s_y[wv][t][lane] = y;
+                }
+                if constexpr (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            });
+        unroll<TT / 4>([&](auto qc) {                      // backwards, 4 frames at a time
+            constexpr int t4 = TT - 4 - 4 * decltype(qc)::value;
+            float vb[16], vc[16];
+            unroll<4>([&](auto tc) {
+                constexpr int t = t4 + 3 - decltype(tc)::value;
+                const float2 dx = s_dx[t][lane];
+                const float g = s_g[t][lane];
+                row_axpy<(t % 4) * 4>(c, cv[t / 4], g);    // c is q_t here
+                if constexpr (ENDS) {
+                    sum += dx.x;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) h[0][n] = rh[n];
-        __syncthreads();
-        if (i > 0) load(i - 1);
+                    for (int n = 0; n < NS; ++n) c[n] *= __builtin_amdgcn_exp2f(dx.x * A2[n]);
+                } else {
+                    float qb = 0.f, ak = 0.f;
+                    row_dot<(t % 4) * 4>(qb, bv[t / 4], c);
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {                     // the tile's states again, from the saved state before it
-            const float2 dx = s_dx[t][lane];
-            float y = 0.f;
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                a[t][n] = __builtin_amdgcn_exp2f(dx.x * A2[n]);
-                h[t + 1][n] = fmaf(a[t][n], h[t][n], dx.y * s_b[t][n0 + n]);
-                y = fmaf(s_c[t][n0 + n], h[t + 1][n], y);
+                    for (int n = 0; n < NS; ++n) {
+                        vb[(t - t4) * 4 + n] = c[n] * dx.y;
+                        vc[(t - t4) * 4 + n] = h[t + 1][n] * g;
+                        c[n] *= a[t][n];
+                        const float k = c[n] * h[t][n];
+                        ak = fmaf(A[n], k, ak);
+                        dA[n] = fmaf(k, dx.x, dA[n]);
+                    }
+                    s_qb[wv][t][lane] = qb;
+                    s_ak[wv][t][lane] = ak;
+                }
+            });
+            if constexpr (!ENDS) {
+                gb[t4 / 4] = row_sum_scatter16(vb, lane);
+                gc[t4 / 4] = row_sum_scatter16(vc, lane);
+                __builtin_amdgcn_sched_barrier(0);         // (read ahead of here, the next frames' inputs cost more registers than two waves per SIMD have)
             }
-            if (d.z) s_y[wv][t][lane] = y;
+        });
+        float sb = 0.f, sc = 0.f;
+        if constexpr (!ENDS) {
+            sb = rows_sum_scatter4(gb);
+            sc = rows_sum_scatter4(gc);
         }
-        float vb[TT * NS], vc[TT * NS];
-#pragma unroll
-        for (int t = TT - 1; t >= 0; --t) {
-            const float2 dx = s_dx[t][lane];
-            const float g = s_g[t][lane];
-            float qb = 0.f, ak = 0.f;
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const float q = fmaf(s_c[t][n0 + n], g, c[n]);
-                vb[t * NS + n] = q * dx.y;
-                vc[t * NS + n] = g * h[t + 1][n];
-                qb = fmaf(q, s_b[t][n0 + n], qb);
-                c[n] = a[t][n] * q;
-                const float k = c[n] * h[t][n];
-                ak = fmaf(A[n], k, ak);
-                dA[n] = fmaf(k, dx.x, dA[n]);
+        lds_barrier();
+        if (i > w.i0) stage(t0 - TT);
+        if constexpr (!ENDS) {
+            {
+                const int t = t0 + (lane >> 2), n = n0 + (lane & 3);
+                if (t < w.len && n < d.N) {
+                    const int64_t at = ((((int64_t)w.ct * d.B + w.b) * d.T + t) * d.G + w.g) * d.N + n;
+                    p.part_b[at] = sb;
+                    p.part_c[at] = sc;
+                }
             }
-            s_qb[wv][t][lane] = qb;
-            s_ak[wv][t][lane] = ak;
-        }
-        {
-            const float sb = wave_sum_scatter64(vb, lane), sc = wave_sum_scatter64(vc, lane);
-            const int t = t0 + (lane >> 2), n = n0 + (lane & 3);
-            if (t < w.len && n < d.N) {
-                const int64_t at = ((((int64_t)w.ct * d.B + w.b) * d.T + t) * d.G + w.g) * d.N + n;
-                p.part_b[at] = sb;
-                p.part_c[at] = sc;
-            }
-        }
-        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < EP; ++j) {
-            const int t = wv + NW * j;
-            const bool in = w.live && t0 + t < w.len;
-            const float D = s_dx[t][lane].x, g = s_g[t][lane];
-            float qb = 0.f, ak = 0.f, y = skip * cu[j];
+            for (int j = 0; j < EP; ++j) {
+                const int t = wv + NW * j;
+                const float u = to_f(cu.u[j]), g = s_g[t][lane];
+                float qb = 0.f, ak = 0.f, y = skip * u;
 #pragma unroll
-            for (int v = 0; v < NW; ++v) { qb += s_qb[v][t][lane]; ak += s_ak[v][t][lane]; }
-            const int64_t at = ((int64_t)w.b * d.T + t0 + t) * d.D + w.ch;
-            float dd = fmaf(cu[j], qb, ak);
-            if (d.softplus) dd *= sigmoid_f(cr[j]);
-            if (in) {
-                dskip = fmaf(g, cu[j], dskip);
-                dbias += dd;
-                ((T*)d.du)[at] = from_f<T>(fmaf(D, qb, skip * g));
-                ((T*)d.ddt)[at] = from_f<T>(dd);
-                if (d.z) {
+                for (int k = 0; k < NW; ++k) { qb += s_qb[k][t][lane]; ak += s_ak[k][t][lane]; }
+                float dd = fmaf(u, qb, ak);
+                if (sp) dd *= sigmoid_f(to_f(cu.dt[j]) + bias);
+                float dz = 0.f;
+                if constexpr (Z) {
 #pragma unroll
-                    for (int v = 0; v < NW; ++v) y += s_y[v][t][lane];
-                    ((T*)d.dz)[at] = from_f<T>(cdy[j] * y * silu_grad_f(cz[j]));
+                    for (int k = 0; k < NW; ++k) y += s_y[k][t][lane];
+                    dz = to_f(cu.dy[j]) * y * silu_grad_f(to_f(cu.z[j]));
+                }
+                if (t0 + t < w.len && w.live) {
+                    const int64_t at = ((int64_t)w.b * d.T + t0 + t) * d.D;
+                    dskip = fmaf(g, u, dskip);
+                    dbias += dd;
+                    ((T*)d.du + at)[(uint32_t)w.ch] = from_f<T>(fmaf(s_dx[t][lane].x, qb, skip * g));
+                    ((T*)d.ddt + at)[(uint32_t)w.ch] = from_f<T>(dd);
+                    if constexpr (Z) ((T*)d.dz + at)[(uint32_t)w.ch] = from_f<T>(dz);
                 }
             }
         }
     }
-    if (w.live)
-        for (int t = w.len + wv; t < d.T; t += NW) {
-            const int64_t at = ((int64_t)w.b * d.T + t) * d.D + w.ch;
-            ((T*)d.du)[at] = from_f<T>(0.f);
-            ((T*)d.ddt)[at] = from_f<T>(0.f);
-            if (d.z) ((T*)d.dz)[at] = from_f<T>(0.f);
+    if constexpr (ENDS) {
+        if (w.live) {
+            float* const e = p.ends + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 1) * d.D + w.ch;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+                if (n0 + n < d.N) e[(int64_t)(n0 + n) * d.D] = c[n];
+            if (wv == 0) e[(int64_t)d.N * d.D] = sum;
         }
-    __syncthreads();                                       // (s_qb is read by the last tile's epilogue above)
-    s_qb[wv][0][lane] = dskip;
-    s_qb[wv][1][lane] = dbias;
-    __syncthreads();
-    float* const part = p.part + (int64_t)w.b * (d.N + 2) * d.D;
-    if (w.live) {
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-            if (n0 + n < d.N) {
-                part[(int64_t)(n0 + n) * d.D + w.ch] = dA[n];
-                if (d.dh0) d.dh0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] = c[n];
+    } else {
+        if (w.live)
+            for (int t = max(w.i0 * TT, w.len) + wv; t < min((w.i0 + p.tpc) * TT, d.T); t += NW) {
+                const int64_t at = ((int64_t)w.b * d.T + t) * d.D + w.ch;
+                ((T*)d.du)[at] = from_f<T>(0.f);
+                ((T*)d.ddt)[at] = from_f<T>(0.f);
+                if constexpr (Z) ((T*)d.dz)[at] = from_f<T>(0.f);
             }
-        if (wv == 0) {
-            float s0 = 0.f, s1 = 0.f;
+        lds_barrier();                                     // (s_qb is read by the last tile's epilogue above)
+        s_qb[wv][0][lane] = dskip;
+        s_qb[wv][1][lane] = dbias;
+        lds_barrier();
+        float* const part = p.part + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 2) * d.D + w.ch;
+        if (w.live) {
 #pragma unroll
-            for (int v = 0; v < NW; ++v) { s0 += s_qb[v][0][lane]; s1 += s_qb[v][1][lane]; }
-            part[(int64_t)d.N * d.D + w.ch] = s0;
-            part[(int64_t)(d.N + 1) * d.D + w.ch] = s1;
+            for (int n = 0; n < NS; ++n)
+                if (n0 + n < d.N) {
+                    part[(int64_t)(n0 + n) * d.D] = dA[n];
+                    if (d.dh0 && w.ck == 0) d.dh0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] = c[n];
+                }
+            if (wv == 0) {
+                float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                for (int k = 0; k < NW; ++k) { s0 += s_qb[k][0][lane]; s1 += s_qb[k][1][lane]; }
+                part[(int64_t)d.N * d.D] = s0;
+                part[(int64_t)(d.N + 1) * d.D] = s1;
+            }
         }
     }
 }
@@ -320,6 +444,7 @@ template <typename T> __global__ __launch_bounds__(256) void scan_bc_kernel(Scan
 }
 
 // One frame: 4 lanes per channel, 4 consecutive states per lane and round; the state is read and written once.
+template <typename T> A8_DEV float ldf(const void* p, int64_t i) { return to_f(((const T*)p)[i]); }
 template <typename T> __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p) {
     const a8_selective_scan_desc& d = p.d;
     const int b = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x >> 2), s4 = threadIdx.x & 3;
@@ -354,41 +479,74 @@ int scan_check(const a8_selective_scan_desc* d, const char* what) {
     A8_REQUIRE(d->A != nullptr, "%s: null A", what);
     return A8_OK;
 }
-ScanArgs scan_args(const a8_selective_scan_desc* d) {
+// Frame chunks of a launch of `waves` waves: enough for about 2048 waves (two per SIMD), none shorter than 4 tiles.
+int scan_chunks(int64_t waves, int tiles) {
+    int n = waves >= 700 ? 1 : (int)((2048 + waves) / (waves > 0 ? waves : 1));
+    if (n > tiles / 4) n = tiles / 4;
+    return n < 1 ? 1 : n;
+}
+ScanArgs scan_args(const a8_selective_scan_desc* d, int ns) {
     ScanArgs p = {};
     p.d = *d;
     p.cpg = d->D / d->G;
     p.tpg = cdiv(p.cpg, CH);
     p.tiles = cdiv(d->T, TT);
+    p.chunks = scan_chunks((int64_t)d->B * d->G * p.tpg * cdiv(d->N, ns), p.tiles);
+    p.tpc = cdiv(p.tiles, p.chunks);
+    p.chunks = p.tpc > 0 ? cdiv(p.tiles, p.tpc) : 1;         // (no empty chunks; T = 0: one without tiles)
     return p;
 }
-int64_t scan_blocks(const ScanArgs& p) { return (int64_t)p.d.B * p.d.G * p.tpg; }
+int64_t scan_blocks(const ScanArgs& p, int chunks) { return (int64_t)p.d.B * p.d.G * p.tpg * chunks; }
+int64_t ends_floats(const ScanArgs& p) { return p.chunks > 1 ? (int64_t)p.d.B * p.chunks * (p.d.N + 1) * p.d.D : 0; }
 
-#define SCAN_DISPATCH(KERNEL, STREAM)                                                                                                       \
-    do {                                                                                                                                    \
-        const dim3 grid((unsigned)scan_blocks(p));                                                                                          \
-        const hipStream_t st = (hipStream_t)STREAM;                                                                                         \
-        if (d->dtype == A8_BF16) {                                                                                                          \
-            if (d->N <= 4) hipLaunchKernelGGL((KERNEL<bf16, 1>), grid, dim3(64), 0, st, p);                                                  \
-            else if (d->N <= 8) hipLaunchKernelGGL((KERNEL<bf16, 2>), grid, dim3(128), 0, st, p);                                            \
-            else if (d->N <= 16) hipLaunchKernelGGL((KERNEL<bf16, 4>), grid, dim3(256), 0, st, p);                                           \
-            else hipLaunchKernelGGL((KERNEL<bf16, 8>), grid, dim3(512), 0, st, p);                                                           \
-        } else {                                                                                                                            \
-            if (d->N <= 4) hipLaunchKernelGGL((KERNEL<float, 1>), grid, dim3(64), 0, st, p);                                                 \
-            else if (d->N <= 8) hipLaunchKernelGGL((KERNEL<float, 2>), grid, dim3(128), 0, st, p);                                           \
-            else if (d->N <= 16) hipLaunchKernelGGL((KERNEL<float, 4>), grid, dim3(256), 0, st, p);                                          \
-            else hipLaunchKernelGGL((KERNEL<float, 8>), grid, dim3(512), 0, st, p);                                                          \
-        }                                                                                                                                   \
+#define SCAN_LAUNCH(KERNEL, T, NW, Z, ENDS) hipLaunchKernelGGL((KERNEL<T, NW, Z, ENDS>), grid, dim3(64 * NW), 0, st, p)
+#define FWD_WAVES(T, Z, ENDS)                                                                                     \
+    do {                                                                                                          \
+        if (waves <= 1) SCAN_LAUNCH(scan_fwd_kernel, T, 1, Z, ENDS);                                              \
+        else if (waves <= 2) SCAN_LAUNCH(scan_fwd_kernel, T, 2, Z, ENDS);                                         \
+        else if (waves <= 4) SCAN_LAUNCH(scan_fwd_kernel, T, 4, Z, ENDS);                                         \
+        else if (waves <= 8) SCAN_LAUNCH(scan_fwd_kernel, T, 8, Z, ENDS);                                         \
+        else SCAN_LAUNCH(scan_fwd_kernel, T, 16, Z, ENDS);                                                        \
     } while (0)
+#define BWD_WAVES(T, Z, ENDS)                                                                                     \
+    do {                                                                                                          \
+        if (waves <= 1) SCAN_LAUNCH(scan_bwd_kernel, T, 1, Z, ENDS);                                              \
+        else if (waves <= 2) SCAN_LAUNCH(scan_bwd_kernel, T, 2, Z, ENDS);                                         \
+        else if (waves <= 4) SCAN_LAUNCH(scan_bwd_kernel, T, 4, Z, ENDS);                                         \
+        else SCAN_LAUNCH(scan_bwd_kernel, T, 8, Z, ENDS);                                                         \
+    } while (0)
+
+// A chunk's own end does not look at z in the forward; in the backward it does (through dout silu(z)).
+int launch_fwd(const ScanArgs& p, bool ends, hipStream_t st) {
+    const dim3 grid((unsigned)scan_blocks(p, ends ? p.chunks - 1 : p.chunks));
+    const int waves = cdiv(p.d.N, FNS);
+    const bool bf = p.d.dtype == A8_BF16, z = p.d.z != nullptr;
+    if (ends) { if (bf) FWD_WAVES(bf16, false, true); else FWD_WAVES(float, false, true); }
+    else if (bf) { if (z) FWD_WAVES(bf16, true, false); else FWD_WAVES(bf16, false, false); }
+    else { if (z) FWD_WAVES(float, true, false); else FWD_WAVES(float, false, false); }
+    return a8_check_launch("a8_selective_scan_fwd");
+}
+int launch_bwd(const ScanArgs& p, bool ends, hipStream_t st) {
+    const dim3 grid((unsigned)scan_blocks(p, ends ? p.chunks - 1 : p.chunks));
+    const int waves = cdiv(p.d.N, BNS);
+    const bool bf = p.d.dtype == A8_BF16, z = p.d.z != nullptr;
+    if (ends) {
+        if (bf) { if (z) BWD_WAVES(bf16, true, true); else BWD_WAVES(bf16, false, true); }
+        else { if (z) BWD_WAVES(float, true, true); else BWD_WAVES(float, false, true); }
+    } else if (bf) { if (z) BWD_WAVES(bf16, true, false); else BWD_WAVES(bf16, false, false); }
+    else { if (z) BWD_WAVES(float, true, false); else BWD_WAVES(float, false, false); }
+    return a8_check_launch("a8_selective_scan_bwd");
+}
 
 }  // namespace
 
 extern "C" int a8_selective_scan_workspace(const a8_selective_scan_desc* d, int backward, int64_t* ckpt_floats, int64_t* ws_floats) {
     if (int e = scan_check(d, "a8_selective_scan_workspace")) return e;
     A8_REQUIRE(ckpt_floats != nullptr && ws_floats != nullptr, "a8_selective_scan_workspace: null result");
-    const ScanArgs p = scan_args(d);
+    const ScanArgs p = scan_args(d, backward ? BNS : FNS);
     *ckpt_floats = (int64_t)d->B * p.tiles * d->N * d->D;
-    *ws_floats = backward ? (int64_t)d->B * (d->N + 2) * d->D + 2 * (int64_t)p.tpg * d->B * d->T * d->G * d->N : 0;
+    *ws_floats = ends_floats(p);
+    if (backward) *ws_floats += (int64_t)d->B * p.chunks * (d->N + 2) * d->D + 2 * (int64_t)p.tpg * d->B * d->T * d->G * d->N;
     return A8_OK;
 }
 
@@ -396,25 +554,30 @@ extern "C" int a8_selective_scan_fwd(const a8_selective_scan_desc* d, void* stre
     if (int e = scan_check(d, "a8_selective_scan_fwd")) return e;
     if (d->B == 0) return A8_OK;
     A8_REQUIRE(d->T == 0 || (d->u && d->dt && d->Bm && d->Cm && d->y), "a8_selective_scan_fwd: null u, dt, B, C or y");
-    const ScanArgs p = scan_args(d);
-    A8_REQUIRE(scan_blocks(p) < (1 << 22), "a8_selective_scan_fwd: B x D = %d x %d is too large", d->B, d->D);
-    SCAN_DISPATCH(scan_fwd_kernel, stream);
-    return a8_check_launch("a8_selective_scan_fwd");
+    ScanArgs p = scan_args(d, FNS);
+    A8_REQUIRE(scan_blocks(p, p.chunks) < (1 << 21), "a8_selective_scan_fwd: B x D = %d x %d is too large", d->B, d->D);
+    A8_REQUIRE(p.chunks == 1 || d->ws, "a8_selective_scan_fwd: null workspace");
+    p.ends = d->ws;
+    if (p.chunks > 1)
+        if (int e = launch_fwd(p, true, (hipStream_t)stream)) return e;
+    return launch_fwd(p, false, (hipStream_t)stream);
 }
 
 extern "C" int a8_selective_scan_bwd(const a8_selective_scan_desc* d, void* stream) {
     if (int e = scan_check(d, "a8_selective_scan_bwd")) return e;
-    ScanArgs p = scan_args(d);
+    ScanArgs p = scan_args(d, BNS);
     A8_REQUIRE(d->B == 0 || d->ws, "a8_selective_scan_bwd: null workspace");
     A8_REQUIRE(d->B == 0 || d->T == 0 || (d->u && d->dt && d->Bm && d->Cm && d->dy && d->ckpt && d->du && d->ddt && d->dBm && d->dCm && (d->dz || !d->z)),
                "a8_selective_scan_bwd: null operand");
-    A8_REQUIRE(scan_blocks(p) < (1 << 22), "a8_selective_scan_bwd: B x D = %d x %d is too large", d->B, d->D);
-    p.part = d->ws;
-    p.part_b = p.part + (int64_t)d->B * (d->N + 2) * d->D;
+    A8_REQUIRE(scan_blocks(p, p.chunks) < (1 << 21), "a8_selective_scan_bwd: B x D = %d x %d is too large", d->B, d->D);
+    p.ends = d->ws;
+    p.part = p.ends + ends_floats(p);
+    p.part_b = p.part + (int64_t)d->B * p.chunks * (d->N + 2) * d->D;
     p.part_c = p.part_b + (int64_t)p.tpg * d->B * d->T * d->G * d->N;
     if (d->B > 0) {
-        SCAN_DISPATCH(scan_bwd_kernel, stream);
-        if (int e = a8_check_launch("a8_selective_scan_bwd")) return e;
+        if (p.chunks > 1)
+            if (int e = launch_bwd(p, true, (hipStream_t)stream)) return e;
+        if (int e = launch_bwd(p, false, (hipStream_t)stream)) return e;
         const int64_t total = (int64_t)d->B * d->T * d->G * d->N;
         if (total > 0) {
             const dim3 grid((unsigned)((total + 255) / 256));
@@ -423,7 +586,7 @@ extern "C" int a8_selective_scan_bwd(const a8_selective_scan_desc* d, void* stre
             if (int e = a8_check_launch("a8_selective_scan_bwd")) return e;
         }
     }
-    A8SeqReduce r = {p.part, d->B, d->N + 2, d->D, d->N, d->dA, {d->dD, d->ddt_bias}, d->add_dA, {d->add_dD, d->add_ddt_bias}};
+    A8SeqReduce r = {p.part, d->B * p.chunks, d->N + 2, d->D, d->N, d->dA, {d->dD, d->ddt_bias}, d->add_dA, {d->add_dD, d->add_ddt_bias}};
     return a8i_seq_reduce(r, stream);
 }
 
@@ -433,7 +596,7 @@ extern "C" int a8_selective_scan_step(const a8_selective_scan_desc* d, void* str
     A8_REQUIRE(d->B <= 65535, "a8_selective_scan_step: B = %d is too large", d->B);
     if (d->B == 0) return A8_OK;
     A8_REQUIRE(d->u && d->dt && d->Bm && d->Cm && d->y && d->h_out, "a8_selective_scan_step: null u, dt, B, C, y or state");
-    const ScanArgs p = scan_args(d);
+    const ScanArgs p = scan_args(d, FNS);
     const dim3 grid(cdiv(d->D, 64), d->B);
     if (d->dtype == A8_BF16) hipLaunchKernelGGL((scan_step_kernel<bf16>), grid, dim3(256), 0, (hipStream_t)stream, p);
     else hipLaunchKernelGGL((scan_step_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, p);
