@@ -89,17 +89,24 @@ template <int NS, int BC> A8_DEV void wave_bc(float (&v)[NS], const float* s, in
 #pragma unroll
     for (int k = 0; k < NS; ++k) v[k] = s[(16 / NS * k + (lane & 15) / NS) * BC + n0 + lane % NS];
 }
-// acc += sum_n row value (I + n) of v * x[n], and its elementwise form x[n] += row value (I + n) of v * g: multiply-adds with the row broadcast in
+// sum_n row value (I + n) of v * x[n], and its elementwise form x[n] += row value (I + n) of v * g: multiply-adds with the row broadcast in
 // the DPP operand (the compiler folds it into multiplies only).  A DPP operand may not be read within two wait states of a VALU write of its register,
 // which the compiler does not see here: one s_nop in front of the group covers a copy that it may have placed there.
-template <int I> A8_DEV void row_dot(float& acc, float v, const float (&x)[2]) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 row_newbcast:%4 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %0, %1, %3 row_newbcast:%5 row_mask:0xf bank_mask:0xf"
-        : "+v"(acc) : "v"(v), "v"(x[0]), "v"(x[1]), "n"(I), "n"(I + 1));
+#define A8_RB(op, acc, x, i) "v_" #op "_f32_dpp %" #acc ", %4, %" #x " row_newbcast:%" #i " row_mask:0xf bank_mask:0xf\n\t"
+template <int I> A8_DEV void row_dot4x2(float (&y)[4], float v, const float (&x)[4][2]) {       // y[f] of 4 frames of 2 states
+    asm("s_nop 1\n\t" A8_RB(mul, 0, 5, 13) A8_RB(mul, 1, 7, 15) A8_RB(mul, 2, 9, 17) A8_RB(mul, 3, 11, 19)
+        A8_RB(fmac, 0, 6, 14) A8_RB(fmac, 1, 8, 16) A8_RB(fmac, 2, 10, 18) A8_RB(fmac, 3, 12, 20)
+        : "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+        : "v"(v), "v"(x[0][0]), "v"(x[0][1]), "v"(x[1][0]), "v"(x[1][1]), "v"(x[2][0]), "v"(x[2][1]), "v"(x[3][0]), "v"(x[3][1]),
+          "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3), "n"(I + 4), "n"(I + 5), "n"(I + 6), "n"(I + 7));
 }
-template <int I> A8_DEV void row_dot(float& acc, float v, const float (&x)[4]) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n\t"
+#undef A8_RB
+template <int I> A8_DEV float row_dot(float v, const float (&x)[4]) {
+    float acc;
+    asm("s_nop 1\n\tv_mul_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n\t"
         "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
-        : "+v"(acc) : "v"(v), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3));
+        : "=&v"(acc) : "v"(v), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3));
+    return acc;
 }
 template <int I> A8_DEV void row_axpy(float (&x)[4], float v, float g) {
     asm("s_nop 1\n\tv_fmac_f32_dpp %0, %4, %5 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n\t"
@@ -161,18 +168,24 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
         float bv[NS], cv[NS];
         wave_bc<NS, BC>(bv, s_b, n0, lane);
         if constexpr (!ENDS) wave_bc<NS, BC>(cv, s_c, n0, lane);
-        unroll<TT>([&](auto tc) {
-            constexpr int t = decltype(tc)::value;
-            const float2 dx = s_dx[t][lane];
-            float y = 0.f;
-            if constexpr (ENDS) sum += dx.x;
-            unroll<NS>([&](auto nc) {
-                constexpr int n = decltype(nc)::value;
-                h[n] = fmaf(__builtin_amdgcn_exp2f(dx.x * A2[n]), h[n], dx.y * bc_at<NS, t, n>(bv));
+        unroll<TT / 4>([&](auto qc) {
+            constexpr int t4 = 4 * decltype(qc)::value;
+            float hq[4][NS], y[4];
+            unroll<4>([&](auto tc) {
+                constexpr int f = decltype(tc)::value, t = t4 + f;
+                const float2 dx = s_dx[t][lane];
+                if constexpr (ENDS) sum += dx.x;
+                unroll<NS>([&](auto nc) {
+                    constexpr int n = decltype(nc)::value;
+                    hq[f][n] = fmaf(__builtin_amdgcn_exp2f(dx.x * A2[n]), f ? hq[f ? f - 1 : 0][n] : h[n], dx.y * bc_at<NS, t, n>(bv));
+                });
             });
+#pragma unroll
+            for (int n = 0; n < NS; ++n) h[n] = hq[3][n];
             if constexpr (!ENDS) {
-                row_dot<(t % (16 / NS)) * NS>(y, cv[t / (16 / NS)], h);
-                s_y[wv][t][lane] = y;
+                row_dot4x2<(t4 % 8) * 2>(y, cv[t4 / 8], hq);
+#pragma unroll
+                for (int f = 0; f < 4; ++f) s_y[wv][t4 + f][lane] = y[f];
             }
         });
         lds_barrier();
@@ -206,8 +219,9 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
 
 // Sums over a wave's 64 lanes of 64 values that come 16 at a time (4 frames x 4 states), scattered: lane l gets the total of value l.  A step pairs
 // lanes that differ in one bit of the index, adds, and keeps the half of the values whose index has the lane's bit: one add per value left instead
-// of six per value.  Inside a row of 16 lanes through DPP (two selects and an add per value left: ~11 cycles), across the rows through the
-// half-wave and half-row register swaps (~15 cycles): the rows come last, when one value per 16 is left.
+// of six per value.  The bits that number a row's four banks of 4 lanes first (8 cycles per value left: the bank mask of the DPP add takes the place
+// of a select), then the two inside a bank (two selects and an add: 12), then, with one value per 16 left, the rows through the half-wave and
+// half-row register swaps (13).
 template <int CTRL, int M> A8_DEV void scatter_step(float* v, bool upper) {
 #pragma unroll
     for (int i = 0; i < M; ++i) {
@@ -215,9 +229,18 @@ template <int CTRL, int M> A8_DEV void scatter_step(float* v, bool upper) {
         v[i] = keep + dpp_f<CTRL>(send);
     }
 }
+#define A8_ROR8(a, b)                                                              \
+    "v_add_f32_dpp %" #a ", %" #a ", %" #a " row_ror:8 row_mask:0xf bank_mask:0x3\n\t" \
+    "v_add_f32_dpp %" #a ", %" #b ", %" #b " row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+#define A8_MIR8(a, b)                                                                      \
+    "v_add_f32_dpp %" #a ", %" #a ", %" #a " row_half_mirror row_mask:0xf bank_mask:0x5\n\t" \
+    "v_add_f32_dpp %" #a ", %" #b ", %" #b " row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
 A8_DEV float row_sum_scatter16(float (&v)[16], int lane) {      // lane l: the sum of v[l & 15] over its row
-    scatter_step<0x128, 8>(v, lane & 8);          // row_ror:8
-    scatter_step<0x141, 4>(v, lane & 4);          // row_half_mirror: flips the bits below too, on which nothing depends yet
+    // (the s_nops: two wait states between a VALU write and a DPP read of the register, on either side of what the compiler sees)
+    asm("s_nop 1\n\t" A8_ROR8(0, 8) A8_ROR8(4, 12) A8_ROR8(1, 9) A8_ROR8(5, 13) A8_ROR8(2, 10) A8_ROR8(6, 14) A8_ROR8(3, 11) A8_ROR8(7, 15)
+        A8_MIR8(0, 4) A8_MIR8(1, 5) A8_MIR8(2, 6) A8_MIR8(3, 7) "s_nop 1"
+        : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]),
+          "+v"(v[8]), "+v"(v[9]), "+v"(v[10]), "+v"(v[11]), "+v"(v[12]), "+v"(v[13]), "+v"(v[14]), "+v"(v[15]));
     scatter_step<0x4E, 2>(v, lane & 2);           // quad_perm xor 2
     scatter_step<0xB1, 1>(v, lane & 1);           // quad_perm xor 1
     return v[0];
@@ -238,7 +261,8 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
     __shared__ float2 s_dxs[2][TT][CH];                    // {D, D u}, by tile parity
     __shared__ float s_gs[2][TT][CH];                      // dout silu(z)
     __shared__ float s_b[TT * BC], s_c[TT * BC];
-    __shared__ float s_qb[ENDS ? 1 : NW][TT][CH], s_ak[ENDS ? 1 : NW][TT][CH], s_y[Z && !ENDS ? NW : 1][TT][CH];
+    __shared__ float2 s_q[ENDS ? 1 : NW][TT][CH];          // a wave's {sum q B, sum A k}
+    __shared__ float s_y[Z && !ENDS ? NW : 1][TT][CH];
     const a8_selective_scan_desc& d = p.d;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = wv * NS;
     const Where w = locate(p, lane, ENDS ? 1 : 0, ENDS ? p.chunks - 1 : p.chunks);
@@ -302,16 +326,12 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
             unroll<TT>([&](auto tc) {                      // the tile's states again, from the saved state before it
                 constexpr int t = decltype(tc)::value;
                 const float2 dx = s_dx[t][lane];
-                float y = 0.f;
                 unroll<NS>([&](auto nc) {
                     constexpr int n = decltype(nc)::value;
                     a[t][n] = __builtin_amdgcn_exp2f(dx.x * A2[n]);
                     h[t + 1][n] = fmaf(a[t][n], h[t][n], dx.y * bc_at<NS, t, n>(bv));
                 });
-                if constexpr (Z) {
-                    row_dot<(t % 4) * 4>(y, cv[t / 4], h[t + 1]);
-                    s_y[wv][t][lane] = y;
-                }
+                if constexpr (Z) s_y[wv][t][lane] = row_dot<(t % 4) * 4>(cv[t / 4], h[t + 1]);
                 if constexpr (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             });
         unroll<TT / 4>([&](auto qc) {                      // backwards, 4 frames at a time
@@ -327,8 +347,8 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
 #pragma unroll
                     for (int n = 0; n < NS; ++n) c[n] *= __builtin_amdgcn_exp2f(dx.x * A2[n]);
                 } else {
-                    float qb = 0.f, ak = 0.f;
-                    row_dot<(t % 4) * 4>(qb, bv[t / 4], c);
+                    const float qb = row_dot<(t % 4) * 4>(bv[t / 4], c);
+                    float ak = 0.f;
 #pragma unroll
                     for (int n = 0; n < NS; ++n) {
                         vb[(t - t4) * 4 + n] = c[n] * dx.y;
@@ -338,8 +358,7 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
                         ak = fmaf(A[n], k, ak);
                         dA[n] = fmaf(k, dx.x, dA[n]);
                     }
-                    s_qb[wv][t][lane] = qb;
-                    s_ak[wv][t][lane] = ak;
+                    s_q[wv][t][lane] = make_float2(qb, ak);
                 }
             });
             if constexpr (!ENDS) {
@@ -370,7 +389,7 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
                 const float u = to_f(cu.u[j]), g = s_g[t][lane];
                 float qb = 0.f, ak = 0.f, y = skip * u;
 #pragma unroll
-                for (int k = 0; k < NW; ++k) { qb += s_qb[k][t][lane]; ak += s_ak[k][t][lane]; }
+                for (int k = 0; k < NW; ++k) { const float2 q = s_q[k][t][lane]; qb += q.x; ak += q.y; }
                 float dd = fmaf(u, qb, ak);
                 if (sp) dd *= sigmoid_f(to_f(cu.dt[j]) + bias);
                 float dz = 0.f;
@@ -406,9 +425,8 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
                 ((T*)d.ddt)[at] = from_f<T>(0.f);
                 if constexpr (Z) ((T*)d.dz)[at] = from_f<T>(0.f);
             }
-        lds_barrier();                                     // (s_qb is read by the last tile's epilogue above)
-        s_qb[wv][0][lane] = dskip;
-        s_qb[wv][1][lane] = dbias;
+        lds_barrier();                                     // (s_q is read by the last tile's epilogue above)
+        s_q[wv][0][lane] = make_float2(dskip, dbias);
         lds_barrier();
         float* const part = p.part + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 2) * d.D + w.ch;
         if (w.live) {
@@ -421,7 +439,7 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
             if (wv == 0) {
                 float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                for (int k = 0; k < NW; ++k) { s0 += s_qb[k][0][lane]; s1 += s_qb[k][1][lane]; }
+                for (int k = 0; k < NW; ++k) { s0 += s_q[k][0][lane].x; s1 += s_q[k][0][lane].y; }
                 part[(int64_t)d.N * d.D] = s0;
                 part[(int64_t)(d.N + 1) * d.D] = s1;
             }
@@ -479,19 +497,31 @@ int scan_check(const a8_selective_scan_desc* d, const char* what) {
     A8_REQUIRE(d->A != nullptr, "%s: null A", what);
     return A8_OK;
 }
-// Frame chunks of a launch of `waves` waves: enough for about 2048 waves (two per SIMD), none shorter than 4 tiles.
-int scan_chunks(int64_t waves, int tiles) {
-    int n = waves >= 700 ? 1 : (int)((2048 + waves) / (waves > 0 ? waves : 1));
-    if (n > tiles / 4) n = tiles / 4;
-    return n < 1 ? 1 : n;
+// Frame chunks.  A launch of n chunks takes ceil-rounds of the blocks that the 256 CUs hold: `part[k - 1]` is the time of a round with k blocks on a
+// CU as a share of a full one, `extra` what the chunks' own ends cost more.  Measured, D = 1536 and 781 frames (us, 1 chunk / the count taken here):
+// forward B = 1 85 / 28 (12), B = 4 88 / 62 (8), B = 8 91 / 91 (1; 100 with 4); backward B = 1 256 / 55 (12), B = 4 275 / 119 (12), B = 8 279 / 199 (8);
+// 16 x 999 x 2048 (512 blocks) 180 and 503 with one chunk, 233 and 564 with two.  A chunk has at least 4 tiles: its first loads and its share of
+// the walk over the chunks before it stay small.
+int scan_chunks(float blocks, int tiles, const float* part, int resident, float extra) {
+    int best = 1;
+    float cost = 0.f;
+    for (int n = 1; n == 1 || (n <= 32 && n * 4 <= tiles); ++n) {
+        const int per_cu = (int)ceilf(blocks * n / 256.f);
+        const int full = per_cu / resident, rest = per_cu % resident;
+        const float c = (full + (rest ? part[rest - 1] : 0.f)) / n * (n > 1 ? 1.f + extra + 0.01f * n : 1.f);
+        if (n == 1 || c < cost) { best = n; cost = c; }
+    }
+    return best;
 }
-ScanArgs scan_args(const a8_selective_scan_desc* d, int ns) {
+const float FWD_PART[3] = {0.48f, 0.74f, 1.f}, BWD_PART[2] = {0.58f, 1.f};
+ScanArgs scan_args(const a8_selective_scan_desc* d, bool backward) {
     ScanArgs p = {};
     p.d = *d;
     p.cpg = d->D / d->G;
     p.tpg = cdiv(p.cpg, CH);
     p.tiles = cdiv(d->T, TT);
-    p.chunks = scan_chunks((int64_t)d->B * d->G * p.tpg * cdiv(d->N, ns), p.tiles);
+    const float blocks = (float)d->B * d->G * p.tpg;         // (in blocks of 16 states: fewer states, shorter blocks)
+    p.chunks = backward ? scan_chunks(blocks * cdiv(d->N, BNS) / 4.f, p.tiles, BWD_PART, 2, 0.13f) : scan_chunks(blocks * cdiv(d->N, FNS) / 8.f, p.tiles, FWD_PART, 3, 1.f);
     p.tpc = cdiv(p.tiles, p.chunks);
     p.chunks = p.tpc > 0 ? cdiv(p.tiles, p.tpc) : 1;         // (no empty chunks; T = 0: one without tiles)
     return p;
@@ -543,7 +573,7 @@ int launch_bwd(const ScanArgs& p, bool ends, hipStream_t st) {
 extern "C" int a8_selective_scan_workspace(const a8_selective_scan_desc* d, int backward, int64_t* ckpt_floats, int64_t* ws_floats) {
     if (int e = scan_check(d, "a8_selective_scan_workspace")) return e;
     A8_REQUIRE(ckpt_floats != nullptr && ws_floats != nullptr, "a8_selective_scan_workspace: null result");
-    const ScanArgs p = scan_args(d, backward ? BNS : FNS);
+    const ScanArgs p = scan_args(d, backward != 0);
     *ckpt_floats = (int64_t)d->B * p.tiles * d->N * d->D;
     *ws_floats = ends_floats(p);
     if (backward) *ws_floats += (int64_t)d->B * p.chunks * (d->N + 2) * d->D + 2 * (int64_t)p.tpg * d->B * d->T * d->G * d->N;
@@ -554,7 +584,7 @@ extern "C" int a8_selective_scan_fwd(const a8_selective_scan_desc* d, void* stre
     if (int e = scan_check(d, "a8_selective_scan_fwd")) return e;
     if (d->B == 0) return A8_OK;
     A8_REQUIRE(d->T == 0 || (d->u && d->dt && d->Bm && d->Cm && d->y), "a8_selective_scan_fwd: null u, dt, B, C or y");
-    ScanArgs p = scan_args(d, FNS);
+    ScanArgs p = scan_args(d, false);
     A8_REQUIRE(scan_blocks(p, p.chunks) < (1 << 21), "a8_selective_scan_fwd: B x D = %d x %d is too large", d->B, d->D);
     A8_REQUIRE(p.chunks == 1 || d->ws, "a8_selective_scan_fwd: null workspace");
     p.ends = d->ws;
@@ -565,7 +595,7 @@ extern "C" int a8_selective_scan_fwd(const a8_selective_scan_desc* d, void* stre
 
 extern "C" int a8_selective_scan_bwd(const a8_selective_scan_desc* d, void* stream) {
     if (int e = scan_check(d, "a8_selective_scan_bwd")) return e;
-    ScanArgs p = scan_args(d, BNS);
+    ScanArgs p = scan_args(d, true);
     A8_REQUIRE(d->B == 0 || d->ws, "a8_selective_scan_bwd: null workspace");
     A8_REQUIRE(d->B == 0 || d->T == 0 || (d->u && d->dt && d->Bm && d->Cm && d->dy && d->ckpt && d->du && d->ddt && d->dBm && d->dCm && (d->dz || !d->z)),
                "a8_selective_scan_bwd: null operand");
@@ -596,7 +626,7 @@ extern "C" int a8_selective_scan_step(const a8_selective_scan_desc* d, void* str
     A8_REQUIRE(d->B <= 65535, "a8_selective_scan_step: B = %d is too large", d->B);
     if (d->B == 0) return A8_OK;
     A8_REQUIRE(d->u && d->dt && d->Bm && d->Cm && d->y && d->h_out, "a8_selective_scan_step: null u, dt, B, C, y or state");
-    const ScanArgs p = scan_args(d, FNS);
+    const ScanArgs p = scan_args(d, false);
     const dim3 grid(cdiv(d->D, 64), d->B);
     if (d->dtype == A8_BF16) hipLaunchKernelGGL((scan_step_kernel<bf16>), grid, dim3(256), 0, (hipStream_t)stream, p);
     else hipLaunchKernelGGL((scan_step_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, p);
