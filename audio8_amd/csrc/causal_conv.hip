@@ -3,108 +3,215 @@
 //   e = (state[b, 0 .. K-2], x[b, 0 .. T-1]);   pre[t] = bias + sum_k w[k] e[t + k];   y = act(pre);   state' = e[len .. len + K - 2]
 //   g[t] = dy[t] act'(pre[t]);   de[j] = sum_k w[k] g[j - k] (+ dstate'[j - len]);   dw[k] = sum_{b,t} g[t] e[t + k];   dbias = sum g
 //
-// A lane owns a channel and walks frames with the last K inputs in registers, so an input is read once per span plus K - 1 frames of overlap.
+// Bound by HBM: x and y (backward: x, dy, dx) once.  A lane owns 4 channels (backward 2; 1 where width, strides or addresses do not allow it) and
+// walks a span of frames with the last K inputs in registers: an input is read once per span plus K - 1 frames of overlap, which come from L2.  A
+// wave is 64 such columns, the four waves of a block are consecutive spans of one utterance.  Short spans and narrow lanes win because they make
+// waves: bf16 8 x 781 x 1536, K = 4, forward 8 channels x 16 frames 16.7 us, 4 x 16 14.5, 4 x 8 12.0 (38 MB: 3.2 TB/s; 64 utterances 66 us, 4.6 TB/s);
+// backward 4 channels x 32 frames 27.2 us, 2 x 32 22.2, 2 x 16 19.6 but twice the partial sums (64 utterances 120 us against 111, 4.2 TB/s).
 #include "a8_seq.h"
 #include "a8hip_internal.h"
 
 namespace {
 
-constexpr int CONV_SPAN = 16;                 // frames per thread
+constexpr int FWD_SPAN = 8, BWD_SPAN = 32;    // frames per wave
 
-template <typename T> A8_DEV float conv_in(const a8_causal_conv_desc& d, int b, int j, int c, int len) {       // e[b, j, c]; 0 behind the end
-    if (j < d.K - 1) return d.state ? to_f(((const T*)d.state)[((int64_t)b * (d.K - 1) + j) * d.C + c]) : 0.f;
+// V consecutive channels, moved as one access
+template <typename T, int V> A8_DEV void ldv(float (&o)[V], const T* p) {
+    struct __attribute__((aligned(V * sizeof(T)))) W { T v[V]; };
+    const W w = *reinterpret_cast<const W*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = to_f(w.v[i]);
+}
+template <typename T, int V> A8_DEV void stv(T* p, const float (&o)[V]) {
+    struct __attribute__((aligned(V * sizeof(T)))) W { T v[V]; } w;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w.v[i] = from_f<T>(o[i]);
+    *reinterpret_cast<W*>(p) = w;
+}
+
+// block -> columns of V channels, utterance, first frame; the column of a lane past the width is the last one (its results are dropped)
+struct Place { int c, b, t0, len; bool on; int64_t row; };
+template <int V, int SPAN> A8_DEV Place place(const a8_causal_conv_desc& d, int cols, int quads) {
+    Place q;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cb = blockIdx.x % cols;
+    q.row = blockIdx.x / cols;
+    q.b = (int)(q.row / quads);
+    q.t0 = ((int)(q.row % quads) * 4 + wv) * SPAN;
+    const int c = (cb * 64 + lane) * V;
+    q.on = c < d.C;
+    q.c = q.on ? c : d.C - V;
+    q.len = seq_len(d.lengths, q.b, d.T);
+    return q;
+}
+// e[b, j]: history, input, or zero behind the end; j < K - 1 + len is loaded, anything else not
+template <typename T, int V> A8_DEV void conv_in(float (&o)[V], const a8_causal_conv_desc& d, const Place& q, int j) {
     const int t = j - (d.K - 1);
-    return t < len ? to_f(((const T*)d.x)[b * d.x_bs + t * d.x_ts + c]) : 0.f;
+    if (t >= 0 && t < q.len) ldv<T, V>(o, (const T*)d.x + (q.b * d.x_bs + t * d.x_ts + q.c));
+    else if (t < 0 && d.state) ldv<T, V>(o, (const T*)d.state + ((int64_t)q.b * (d.K - 1) + j) * d.C + q.c);
+    else
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = 0.f;
 }
 
-template <typename T, int K> __global__ __launch_bounds__(256) void conv_fwd_kernel(a8_causal_conv_desc d, int spans) {
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63);
-    const int64_t s = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (c >= d.C || s >= (int64_t)d.B * spans) return;
-    const int b = (int)(s / spans), t0 = (int)(s % spans) * CONV_SPAN, len = seq_len(d.lengths, b, d.T);
-    float w[K], e[K];
+template <typename T, int K, int V> __global__ __launch_bounds__(256) void conv_fwd_kernel(a8_causal_conv_desc d, int cols, int quads) {
+    const Place q = place<V, FWD_SPAN>(d, cols, quads);
+    if (q.t0 >= d.T && !(q.t0 == 0)) return;                   // (a whole wave)
+    float w[K][V], bias[V], e[K - 1][V];
 #pragma unroll
-    for (int k = 0; k < K; ++k) w[k] = d.w[(int64_t)c * K + k];
-    const float bias = d.bias ? d.bias[c] : 0.f;
+    for (int i = 0; i < V; ++i) {
+        bias[i] = d.bias ? d.bias[q.c + i] : 0.f;
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) e[k + 1] = conv_in<T>(d, b, t0 + k, c, len);
-    for (int t = t0; t < min(t0 + CONV_SPAN, d.T); ++t) {
-        float pre = bias;
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k) e[k] = e[k + 1];
-        e[K - 1] = conv_in<T>(d, b, t + K - 1, c, len);
-#pragma unroll
-        for (int k = 0; k < K; ++k) pre = fmaf(w[k], e[k], pre);
-        const float y = d.act == A8_CONV_ACT_SILU ? silu_f(pre) : pre;
-        ((T*)d.y)[((int64_t)b * d.T + t) * d.C + c] = from_f<T>(t < len ? y : 0.f);
+        for (int k = 0; k < K; ++k) w[k][i] = d.w[(int64_t)(q.c + i) * K + k];
     }
-    if (d.state_out && t0 == 0)
-        for (int j = 0; j < K - 1; ++j) ((T*)d.state_out)[((int64_t)b * (K - 1) + j) * d.C + c] = from_f<T>(conv_in<T>(d, b, len + j, c, len));
-}
-
-template <typename T, int K> __global__ __launch_bounds__(256) void conv_bwd_kernel(a8_causal_conv_desc d, int spans) {
-    __shared__ float red[4][K + 1][64];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane, quads = (spans + 3) / 4;
-    const int b = blockIdx.y / quads, span = (blockIdx.y % quads) * 4 + wv;
-    float dw[K] = {}, db = 0.f;
-    if (c < d.C && span < spans) {
-        const int t0 = span * CONV_SPAN, t1 = min(t0 + CONV_SPAN, d.T), len = seq_len(d.lengths, b, d.T);
-        float w[K], e[K], g[K];
 #pragma unroll
-        for (int k = 0; k < K; ++k) { w[k] = d.w[(int64_t)c * K + k]; g[k] = 0.f; }
-        const float bias = d.bias ? d.bias[c] : 0.f;
+    for (int k = 0; k < K - 1; ++k) conv_in<T, V>(e[k], d, q, q.t0 + k);
+    const bool silu = d.act == A8_CONV_ACT_SILU;
+    T* const y = (T*)d.y + ((int64_t)q.b * d.T + q.t0) * d.C + q.c;
+    auto frame = [&](int s, const float (&x)[V]) {             // frame t0 + s, whose input is x
+        float o[V];
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) e[k + 1] = conv_in<T>(d, b, t0 + k, c, len);
-        // g runs K - 1 frames past the span's end, de[j] of j = t0 .. t1 - 1 + K - 1 lags it; the first span also owns the history's gradient
-        for (int t = t0; t < t1 + K - 1; ++t) {
+        for (int i = 0; i < V; ++i) {
+            float pre = fmaf(w[K - 1][i], x[i], bias[i]);
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k) { e[k] = e[k + 1]; g[k] = g[k + 1]; }
-            e[K - 1] = conv_in<T>(d, b, t + K - 1, c, len);
-            float pre = bias;
+            for (int k = 0; k < K - 1; ++k) { pre = fmaf(w[k][i], e[k][i], pre); e[k][i] = k + 1 < K - 1 ? e[k + 1 < K - 1 ? k + 1 : 0][i] : x[i]; }
+            o[i] = silu ? silu_f(pre) : pre;
+        }
+        return stv<T, V>(y + (int64_t)s * d.C, o);
+    };
+    const T* const x = (const T*)d.x + (q.b * d.x_bs + q.t0 * d.x_ts + q.c);
+    if (q.t0 + FWD_SPAN <= q.len) {                            // a full span: 8 loads in flight at a time
 #pragma unroll
-            for (int k = 0; k < K; ++k) pre = fmaf(w[k], e[k], pre);
-            float gt = t < len ? to_f(((const T*)d.dy)[b * d.dy_bs + t * d.dy_ts + c]) : 0.f;
-            if (d.act == A8_CONV_ACT_SILU && t < len) gt *= silu_grad_f(pre);
-            g[K - 1] = gt;                                            // g[k] = g of frame t - (K - 1) + k
-            if (t < t1) {
-                db += gt;
+        for (int s8 = 0; s8 < FWD_SPAN; s8 += 8) {
+            float in[8][V];
 #pragma unroll
-                for (int k = 0; k < K; ++k) dw[k] = fmaf(gt, e[k], dw[k]);
-            }
-            const int j = t - t0 < K - 1 ? -1 : t;                    // e index whose gradient is complete: frame t - (K - 1)
-            if (j >= 0) {
-                float de = 0.f;
+            for (int s = 0; s < 8; ++s) ldv<T, V>(in[s], x + (s8 + s) * d.x_ts);
+            if (q.on)
 #pragma unroll
-                for (int k = 0; k < K; ++k) de = fmaf(w[K - 1 - k], g[k], de);
-                const int tx = j - (K - 1);
-                if (d.dstate_out && tx < len && tx >= len - (K - 1)) de += to_f(((const T*)d.dstate_out)[((int64_t)b * (K - 1) + tx + (K - 1) - len) * d.C + c]);
-                if (d.dx) ((T*)d.dx)[((int64_t)b * d.T + tx) * d.C + c] = from_f<T>(tx < len ? de : 0.f);
-            }
+                for (int s = 0; s < 8; ++s) frame(s8 + s, in[s]);
+        }
+    } else if (q.on) {
+        for (int s = 0; s < min(FWD_SPAN, d.T - q.t0); ++s) {
+            float in[V] = {};
+            if (q.t0 + s < q.len) { ldv<T, V>(in, x + s * d.x_ts); frame(s, in); }
+            else stv<T, V>(y + (int64_t)s * d.C, in);
         }
     }
-    if (span == 0 && c < d.C && d.dstate) {                           // de of the history: e indexes 0 .. K - 2
-        const int len = seq_len(d.lengths, b, d.T);
+    if (d.state_out && q.t0 == 0 && q.on)
         for (int j = 0; j < K - 1; ++j) {
-            float de = 0.f;
-            for (int t = 0; t <= min(j, len - 1); ++t) {              // frames t <= j read e[j] at tap j - t
-                float pre = d.bias ? d.bias[c] : 0.f;
-                for (int k = 0; k < K; ++k) pre = fmaf(d.w[(int64_t)c * K + k], conv_in<T>(d, b, t + k, c, len), pre);
-                float gt = to_f(((const T*)d.dy)[b * d.dy_bs + t * d.dy_ts + c]);
-                if (d.act == A8_CONV_ACT_SILU) gt *= silu_grad_f(pre);
-                de = fmaf(d.w[(int64_t)c * K + j - t], gt, de);
-            }
-            if (d.dstate_out && j >= len) de += to_f(((const T*)d.dstate_out)[((int64_t)b * (K - 1) + j - len) * d.C + c]);
-            ((T*)d.dstate)[((int64_t)b * (K - 1) + j) * d.C + c] = from_f<T>(de);
+            float o[V];
+            conv_in<T, V>(o, d, q, q.len + j);
+            stv<T, V>((T*)d.state_out + ((int64_t)q.b * (K - 1) + j) * d.C + q.c, o);
         }
-    }
+}
+
+template <typename T, int K, int V> __global__ __launch_bounds__(256) void conv_bwd_kernel(a8_causal_conv_desc d, int cols, int quads) {
+    __shared__ float red[4][K + 1][64 * V];
+    const Place q = place<V, BWD_SPAN>(d, cols, quads);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool silu = d.act == A8_CONV_ACT_SILU;
+    float dw[K][V] = {}, db[V] = {};
+    if (q.t0 < d.T) {
+        const int t1 = min(q.t0 + BWD_SPAN, d.T);
+        float w[K][V], bias[V], e[K][V], g[K][V] = {};         // e[k], g[k]: input and gradient before the activation of frame t - (K - 1) + k
 #pragma unroll
-    for (int k = 0; k < K; ++k) red[wv][k][lane] = dw[k];
-    red[wv][K][lane] = db;
+        for (int i = 0; i < V; ++i) {
+            bias[i] = d.bias ? d.bias[q.c + i] : 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k][i] = d.w[(int64_t)(q.c + i) * K + k];
+        }
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) conv_in<T, V>(e[k + 1], d, q, q.t0 + k);
+        const T* const xp = (const T*)d.x + (q.b * d.x_bs + q.c);
+        const T* const dp = (const T*)d.dy + (q.b * d.dy_bs + q.c);
+        T* const dx = (T*)d.dx + (int64_t)q.b * d.T * d.C + q.c;
+        auto frame = [&](int t, const float (&x)[V], const float (&dy)[V], bool own, bool valid) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) { e[k][i] = e[k + 1][i]; g[k][i] = g[k + 1][i]; }
+                e[K - 1][i] = x[i];
+                float pre = bias[i];
+#pragma unroll
+                for (int k = 0; k < K; ++k) pre = fmaf(w[k][i], e[k][i], pre);
+                const float gt = valid ? (silu ? dy[i] * silu_grad_f(pre) : dy[i]) : 0.f;
+                g[K - 1][i] = gt;
+                if (own) {
+                    db[i] += gt;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) dw[k][i] = fmaf(gt, e[k][i], dw[k][i]);
+                }
+            }
+        };
+        auto emit = [&](int tx) {                              // the input gradient of frame tx, whose last tap was just taken in
+            float de[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                de[i] = 0.f;
+#pragma unroll
+                for (int k = 0; k < K; ++k) de[i] = fmaf(w[K - 1 - k][i], g[k][i], de[i]);
+            }
+            if (d.dstate_out && tx < q.len && tx >= q.len - (K - 1)) {
+                float ds[V];
+                ldv<T, V>(ds, (const T*)d.dstate_out + ((int64_t)q.b * (K - 1) + tx + (K - 1) - q.len) * d.C + q.c);
+#pragma unroll
+                for (int i = 0; i < V; ++i) de[i] += ds[i];
+            }
+            if (tx >= q.len)
+#pragma unroll
+                for (int i = 0; i < V; ++i) de[i] = 0.f;
+            if (q.on && d.dx) stv<T, V>(dx + (int64_t)tx * d.C, de);
+        };
+        // g runs K - 1 frames past the span's end; the input gradient lags it by as many
+        auto slow = [&](int t) {
+            float x[V] = {}, dy[V] = {};
+            const bool valid = t < q.len;
+            if (valid) { ldv<T, V>(x, xp + t * d.x_ts); ldv<T, V>(dy, dp + t * d.dy_ts); }
+            frame(t, x, dy, t < t1, valid);
+            if (t - q.t0 >= K - 1) emit(t - (K - 1));
+        };
+        int t = q.t0;
+        for (; t < min(q.t0 + K - 1, t1 + K - 1); ++t) slow(t);
+        for (; t + 4 <= min(t1, q.len); t += 4) {              // four frames' loads in flight
+            float x[4][V], dy[4][V];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) { ldv<T, V>(x[s], xp + (t + s) * d.x_ts); ldv<T, V>(dy[s], dp + (t + s) * d.dy_ts); }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) { frame(t + s, x[s], dy[s], true, true); emit(t + s - (K - 1)); }
+        }
+        for (; t < t1 + K - 1; ++t) slow(t);
+    }
+    if (q.t0 == 0 && q.on && d.dstate)                         // the history's gradient: e indexes 0 .. K - 2, read by frames t <= j at tap j - t
+        for (int j = 0; j < K - 1; ++j)
+            for (int i = 0; i < V; ++i) {
+                const int c = q.c + i;
+                float de = 0.f;
+                for (int t = 0; t <= min(j, q.len - 1); ++t) {
+                    float pre = d.bias ? d.bias[c] : 0.f;
+                    for (int k = 0; k < K; ++k) {
+                        const int f = t + k - (K - 1);
+                        const float v = f >= 0 ? to_f(((const T*)d.x)[q.b * d.x_bs + f * d.x_ts + c])
+                                               : d.state ? to_f(((const T*)d.state)[((int64_t)q.b * (K - 1) + t + k) * d.C + c]) : 0.f;
+                        pre = fmaf(d.w[(int64_t)c * K + k], v, pre);
+                    }
+                    float gt = to_f(((const T*)d.dy)[q.b * d.dy_bs + t * d.dy_ts + c]);
+                    if (silu) gt *= silu_grad_f(pre);
+                    de = fmaf(d.w[(int64_t)c * K + j - t], gt, de);
+                }
+                if (d.dstate_out && j >= q.len) de += to_f(((const T*)d.dstate_out)[((int64_t)q.b * (K - 1) + j - q.len) * d.C + c]);
+                ((T*)d.dstate)[((int64_t)q.b * (K - 1) + j) * d.C + c] = from_f<T>(de);
+            }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) red[wv][k][lane * V + i] = dw[k][i];
+        red[wv][K][lane * V + i] = db[i];
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < (K + 1) * 64; i += 256) {
-        const int q = i >> 6, l = i & 63, cc = blockIdx.x * 64 + l;
-        if (cc < d.C) d.partials[((int64_t)blockIdx.y * (K + 1) + q) * d.C + cc] = (red[0][q][l] + red[1][q][l]) + (red[2][q][l] + red[3][q][l]);
+    const int c0 = (blockIdx.x % cols) * 64 * V;
+    for (int i = threadIdx.x; i < (K + 1) * 64 * V; i += 256) {
+        const int p = i / (64 * V), l = i % (64 * V);
+        if (c0 + l < d.C) d.partials[(q.row * (K + 1) + p) * d.C + c0 + l] = (red[0][p][l] + red[1][p][l]) + (red[2][p][l] + red[3][p][l]);
     }
 }
 
@@ -125,21 +232,28 @@ template <typename T, int K> __global__ __launch_bounds__(256) void conv_step_ke
     for (int k = 0; k < K - 1; ++k) st[(int64_t)k * d.C] = e[k + 1];
 }
 
-__global__ __launch_bounds__(256) void seq_reduce_kernel(A8SeqReduce r) {
-    __shared__ float red[4][64];
+// 16 columns of one plane per block; the 16 waves take four rows at a time (a quarter of the lanes each), four loads in flight, and meet in LDS.
+__global__ __launch_bounds__(1024) void seq_reduce_kernel(A8SeqReduce r) {
+    __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane, q = blockIdx.y;
-    float s = 0.f;
-    if (c < r.C)
-        for (int i = wv; i < r.rows; i += 4) s += r.in[((int64_t)i * r.planes + q) * r.C + c];
-    red[wv][lane] = s;
+    const int c = blockIdx.x * 16 + (lane & 15), q = blockIdx.y;
+    const float* const in = r.in + (int64_t)q * r.C + min(c, r.C - 1);
+    const int64_t pitch = (int64_t)r.planes * r.C;
+    float s[4] = {};
+    int i = wv * 4 + (lane >> 4);
+    for (; i + 192 < r.rows; i += 256)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] += in[(i + 64 * k) * pitch];
+    for (; i < r.rows; i += 64) s[0] += in[i * pitch];
+    red[wv][lane] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    if (wv == 0 && c < r.C) {
-        s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    if (threadIdx.x < 16 && c < r.C) {
+        float t = 0.f;
+        for (int k = 0; k < 64; ++k) t += red[k >> 2][(k & 3) * 16 + lane];
         float* out = q < r.np ? r.major + (int64_t)c * r.np + q : r.minor[q - r.np] + c;
         const bool have = q < r.np ? r.major != nullptr : r.minor[q - r.np] != nullptr;
         const int add = q < r.np ? r.add_major : r.add_minor[q - r.np];
-        if (have) *out = add ? *out + s : s;
+        if (have) *out = add ? *out + t : t;
     }
 }
 
@@ -152,25 +266,26 @@ int conv_check(const a8_causal_conv_desc* d, const char* what) {
     return A8_OK;
 }
 
-#define CONV_DISPATCH(KERNEL, GRID, STREAM, ...)                                                                                       \
-    do {                                                                                                                               \
-        if (d->dtype == A8_BF16) {                                                                                                     \
-            if (d->K == 2) hipLaunchKernelGGL((KERNEL<bf16, 2>), GRID, dim3(256), 0, STREAM, __VA_ARGS__);                              \
-            else if (d->K == 3) hipLaunchKernelGGL((KERNEL<bf16, 3>), GRID, dim3(256), 0, STREAM, __VA_ARGS__);                         \
-            else hipLaunchKernelGGL((KERNEL<bf16, 4>), GRID, dim3(256), 0, STREAM, __VA_ARGS__);                                        \
-        } else {                                                                                                                       \
-            if (d->K == 2) hipLaunchKernelGGL((KERNEL<float, 2>), GRID, dim3(256), 0, STREAM, __VA_ARGS__);                             \
-            else if (d->K == 3) hipLaunchKernelGGL((KERNEL<float, 3>), GRID, dim3(256), 0, STREAM, __VA_ARGS__);                        \
-            else hipLaunchKernelGGL((KERNEL<float, 4>), GRID, dim3(256), 0, STREAM, __VA_ARGS__);                                       \
-        }                                                                                                                              \
-    } while (0)
-
-int conv_rows(const a8_causal_conv_desc* d) { return d->B * cdiv(cdiv(d->T, CONV_SPAN), 4); }
+bool multiple(const void* p, int bytes) { return ((uintptr_t)p % bytes) == 0; }
+// whether V channels at a time are aligned everywhere: width, row and batch strides, base addresses
+bool conv_vec(const a8_causal_conv_desc* d, int V, bool backward) {
+    const int bytes = V * (d->dtype == A8_BF16 ? 2 : 4);
+    bool ok = d->C % V == 0 && d->x_bs % V == 0 && d->x_ts % V == 0;
+    for (const void* p : {d->x, d->state, (const void*)d->y, (const void*)d->state_out}) ok = ok && multiple(p, bytes);
+    if (backward) {
+        ok = ok && d->dy_bs % V == 0 && d->dy_ts % V == 0;
+        for (const void* p : {d->dy, d->dstate_out, (const void*)d->dx, (const void*)d->dstate}) ok = ok && multiple(p, bytes);
+    }
+    return ok;
+}
+#define CONV_TAPS(KERNEL, T, V) (d->K == 2 ? (KERNEL<T, 2, V>) : d->K == 3 ? (KERNEL<T, 3, V>) : (KERNEL<T, 4, V>))
+int conv_quads(const a8_causal_conv_desc* d, int span) { return cdiv(d->T > 0 ? d->T : 1, 4 * span); }        // blocks along an utterance (T = 0 still hands the history on)
+int conv_rows(const a8_causal_conv_desc* d) { return d->T > 0 ? d->B * conv_quads(d, BWD_SPAN) : 0; }
 
 }  // namespace
 
 int a8i_seq_reduce(const A8SeqReduce& r, void* stream) {
-    hipLaunchKernelGGL(seq_reduce_kernel, dim3(cdiv(r.C, 64), r.planes), dim3(256), 0, (hipStream_t)stream, r);
+    hipLaunchKernelGGL(seq_reduce_kernel, dim3(cdiv(r.C, 16), r.planes), dim3(1024), 0, (hipStream_t)stream, r);
     return a8_check_launch("a8i_seq_reduce");
 }
 
@@ -179,8 +294,13 @@ extern "C" int a8_causal_conv_fwd(const a8_causal_conv_desc* d, void* stream) {
     if (d->B == 0) return A8_OK;
     A8_REQUIRE((d->x && d->y) || d->T == 0, "a8_causal_conv_fwd: null x or y");
     A8_REQUIRE(d->state_out == nullptr || d->state_out != d->state, "a8_causal_conv_fwd: state_out may not be the state that is read");
-    const int spans = d->T > 0 ? cdiv(d->T, CONV_SPAN) : 1;              // T = 0 still hands the history on
-    CONV_DISPATCH(conv_fwd_kernel, dim3(cdiv(d->C, 64), cdiv((int64_t)d->B * spans, 4)), (hipStream_t)stream, *d, spans);
+    const bool bf = d->dtype == A8_BF16;
+    const int V = conv_vec(d, 4, false) ? 4 : 1;
+    const int cols = cdiv(d->C, 64 * V), quads = conv_quads(d, FWD_SPAN);
+    A8_REQUIRE((int64_t)cols * d->B * quads < (1 << 24), "a8_causal_conv_fwd: B x T x C = %d x %d x %d is too large", d->B, d->T, d->C);
+    auto kernel = bf ? (V == 4 ? CONV_TAPS(conv_fwd_kernel, bf16, 4) : CONV_TAPS(conv_fwd_kernel, bf16, 1))
+                     : (V == 4 ? CONV_TAPS(conv_fwd_kernel, float, 4) : CONV_TAPS(conv_fwd_kernel, float, 1));
+    hipLaunchKernelGGL(kernel, dim3(cols * d->B * quads), dim3(256), 0, (hipStream_t)stream, *d, cols, quads);
     return a8_check_launch("a8_causal_conv_fwd");
 }
 
@@ -193,12 +313,17 @@ extern "C" int a8_causal_conv_bwd_partial_floats(const a8_causal_conv_desc* d, i
 
 extern "C" int a8_causal_conv_bwd(const a8_causal_conv_desc* d, void* stream) {
     if (int e = conv_check(d, "a8_causal_conv_bwd")) return e;
-    const int spans = cdiv(d->T, CONV_SPAN), rows = conv_rows(d);
+    const int rows = conv_rows(d);
     A8_REQUIRE((d->x && d->dy && d->partials) || rows == 0, "a8_causal_conv_bwd: null x, dy or partials");
     A8_REQUIRE(d->T > 0 || d->B == 0 || d->dstate == nullptr, "a8_causal_conv_bwd: a history's gradient needs T >= 1");
-    A8_REQUIRE(rows <= 65535, "a8_causal_conv_bwd: B x T = %d x %d is too large", d->B, d->T);
     if (rows > 0) {
-        CONV_DISPATCH(conv_bwd_kernel, dim3(cdiv(d->C, 64), rows), (hipStream_t)stream, *d, spans);
+        const bool bf = d->dtype == A8_BF16;
+        const int V = conv_vec(d, 2, true) ? 2 : 1;
+        const int cols = cdiv(d->C, 64 * V), quads = conv_quads(d, BWD_SPAN);
+        A8_REQUIRE((int64_t)cols * rows < (1 << 24), "a8_causal_conv_bwd: B x T x C = %d x %d x %d is too large", d->B, d->T, d->C);
+        auto kernel = bf ? (V == 2 ? CONV_TAPS(conv_bwd_kernel, bf16, 2) : CONV_TAPS(conv_bwd_kernel, bf16, 1))
+                         : (V == 2 ? CONV_TAPS(conv_bwd_kernel, float, 2) : CONV_TAPS(conv_bwd_kernel, float, 1));
+        hipLaunchKernelGGL(kernel, dim3(cols * rows), dim3(256), 0, (hipStream_t)stream, *d, cols, quads);
         if (int e = a8_check_launch("a8_causal_conv_bwd")) return e;
     }
     A8SeqReduce r = {d->partials, rows, d->K + 1, d->C, d->K, d->dw, {d->dbias}, d->add_dw, {d->add_dbias}};
@@ -210,6 +335,8 @@ extern "C" int a8_causal_conv_step(const a8_causal_conv_desc* d, void* stream) {
     A8_REQUIRE(d->T == 1, "a8_causal_conv_step: one frame at a time (T = %d)", d->T);
     if (d->B == 0) return A8_OK;
     A8_REQUIRE(d->x && d->y && d->state_out, "a8_causal_conv_step: null x, y or state");
-    CONV_DISPATCH(conv_step_kernel, dim3(cdiv((int64_t)d->B * d->C, 256)), (hipStream_t)stream, *d);
+    auto kernel = d->dtype == A8_BF16 ? (d->K == 2 ? conv_step_kernel<bf16, 2> : d->K == 3 ? conv_step_kernel<bf16, 3> : conv_step_kernel<bf16, 4>)
+                                      : (d->K == 2 ? conv_step_kernel<float, 2> : d->K == 3 ? conv_step_kernel<float, 3> : conv_step_kernel<float, 4>);
+    hipLaunchKernelGGL(kernel, dim3(cdiv((int64_t)d->B * d->C, 256)), dim3(256), 0, (hipStream_t)stream, *d);
     return a8_check_launch("a8_causal_conv_step");
 }

@@ -2,17 +2,19 @@
 //
 //   p = N(o; pw, pb) (or o);  r = x + scale gate p;  n = N(r; w, b)      N: LayerNorm or RMS norm over the C channels of a row
 // Gradient, from x, o, gate and the four row statistics (r is formed again in f32 instead of being read back rounded):
-//   dR = dr + N'(dn w);  dx = dR;  dgate = dR scale p;  dscale = sum dR gate p;  dp = dR scale gate;  do = N'(dp pw)
-//   dw = sum dn rhat, db = sum dn, dpw = sum dp ohat, dpb = sum dp;   N'(v) = rstd (v - mean(v) - hat mean(v hat)), RMS without mean(v)
+//   dR = dr + N'(dn w);  dx = dR;  dgate = dR scale p;  do = N'(dR scale gate pw);   N'(v) = rstd (v - mean(v) - hat mean(v hat)), RMS without mean(v)
+//   dw = sum dn rhat, db = sum dn;  with E1 = sum dR gate ohat, E0 = sum dR gate:  dpw = scale E1, dpb = scale E0, dscale = pw E1 + pb E0
+// (four column sums instead of five: p and dp are columns times ohat and dR gate).
 //
-// A row is held in registers by one wave (C <= 1024) or by a block (wider rows), 8 consecutive channels per lane and round: every tensor is
-// read and written once, statistics are exact two-pass in f32, and the backward keeps its column sums in registers over all rows of its block.
+// Bound by HBM.  A row is held in registers by one wave (C <= 1024) or by a block (wider rows), 8 consecutive channels per lane and round: every
+// tensor is read and written once, statistics are exact two-pass in f32.  The backward walks many rows per wave, the next row's loads in flight, the
+// parameters in LDS, the column sums in registers.
 #include "a8_seq.h"
 #include "a8hip_internal.h"
 
 namespace {
 
-enum { PLANE_W = 0, PLANE_B, PLANE_PW, PLANE_PB, PLANE_SCALE, PLANES };
+enum { PLANE_W = 0, PLANE_B, PLANE_E1, PLANE_E0, PLANES };
 
 struct NormArgs { a8_residual_norm_desc d; int chunks, rows_per_chunk, vec; };
 
@@ -176,159 +178,213 @@ template <typename T, int RW, int NCH> __global__ __launch_bounds__(RW == 1 ? 25
     }
 }
 
-// v -> rstd (v - mean(v) - h mean(v h)), RMS without mean(v)
-template <int RW, int NCH, typename R> A8_DEV void norm_back(const R& row, float (&v)[NCH][8], const float (&h)[NCH][8], bool layer, float rstd, float* red) {
-    float s = 0.f, q = 0.f;
+// 8 elements as loaded
+template <typename T> struct Raw {
+    T v[8];
+    A8_DEV void load(const T* p, bool vec, int left) {
+        if (vec) {
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
+            for (int k = 0; k < (int)(8 * sizeof(T) / 16); ++k) reinterpret_cast<u32x4*>(v)[k] = reinterpret_cast<const u32x4*>(p)[k];
+        } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) { s += v[j][k]; q = fmaf(v[j][k], h[j][k], q); }
-    const float inv = 1.0f / (float)row.C;
-    s = layer ? row_sum<RW>(s, red) * inv : 0.f;
-    q = row_sum<RW>(q, red) * inv;
+            for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : from_f<T>(0.f);
+        }
+    }
+};
+
+// two row sums at once
+template <int RW> A8_DEV void row_sum2(float& a, float& b, float2* red) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (RW > 1) {
+        const int w = threadIdx.x >> 6;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[w] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.f;
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[j][k] = rstd * (v[j][k] - s - h[j][k] * q);
+        for (int i = 0; i < RW; ++i) { a += red[i].x; b += red[i].y; }
+    }
 }
 
-template <typename T, int RW, int NCH> __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void rnorm_bwd_kernel(NormArgs p) {
+template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void rnorm_bwd_kernel(NormArgs p) {
     typedef Row<T, RW, NCH> R;
-    __shared__ float red[R::WAVES];
-    __shared__ float comb[RW == 1 ? 4 * NCH * 512 : 1];
+    constexpr int W = R::NT * NCH * 8;                         // columns a row's threads cover
+    __shared__ float2 red[R::WAVES];
+    __shared__ __align__(16) float par[4][W];                  // scale, pw, pb, w (1, 1, 0, 1 where there is none); then the waves' column sums
     const a8_residual_norm_desc& d = p.d;
     R row;
-    row.init(d.C, p.vec);
+    row.init(d.C, VEC);
     const int rows = d.B * d.T, b = blockIdx.x / p.chunks, ck = blockIdx.x % p.chunks;
     const int ta = ck * p.rows_per_chunk, tb = min(ta + p.rows_per_chunk, d.T);
-    const int wv = RW == 1 ? threadIdx.x >> 6 : 0, step = RW == 1 ? 4 : 1;
+    const int wv = RW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, step = RW == 1 ? 4 : 1;
     const bool layer = d.kind == A8_NORM_LAYER, gate_rows = d.gate && d.gate_rows;
-    float acc[PLANES][NCH][8] = {}, accg[NCH][8] = {};
+    for (int c = threadIdx.x; c < W; c += R::WAVES * 64) {
+        const bool in = c < d.C;
+        par[0][c] = in && d.scale ? d.scale[c] : 1.f;
+        par[1][c] = in && d.post ? d.post_w[c] : 1.f;
+        par[2][c] = in && d.post && d.post_b ? d.post_b[c] : 0.f;
+        par[3][c] = in && d.w ? d.w[c] : 1.f;
+    }
+    __syncthreads();
+    float acc[PLANES][NCH][8] = {}, ug[NCH][8];                // ug: the utterance's gate, 1 without one; gates per frame are loaded with the rows
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ug[j][k] = 1.f;
+    if (d.gate && !gate_rows) row.load(ug, (const T*)d.gate + (int64_t)b * d.g_bs);
+    Raw<T> ro[NCH], rx[NCH], rdr[NCH], rdn[NCH], rg[NCH];
+    float st[4];
+    auto load = [&](int t) {
+        const int64_t r = (int64_t)b * d.T + t;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+            if (row.on[j]) {
+                const int c = row.col[j], left = d.C - c;
+                ro[j].load((const T*)d.o + r * d.o_ld + c, VEC, left);
+                if (d.dn) {
+                    rx[j].load((const T*)d.x + r * d.x_ld + c, VEC, left);
+                    rdn[j].load((const T*)d.dn + r * d.C + c, VEC, left);
+                }
+                if (d.dr) rdr[j].load((const T*)d.dr + r * d.C + c, VEC, left);
+                if (gate_rows) rg[j].load((const T*)d.gate + (int64_t)b * d.g_bs + (int64_t)t * d.g_ts + c, VEC, left);
+            }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) st[k] = (k < 2 ? d.post != 0 : d.dn != nullptr) ? d.stats[k * (int64_t)rows + r] : k & 1;
+    };
+    if (ta + wv < tb) load(ta + wv);
     for (int t = ta + wv; t < tb; t += step) {
         const int64_t r = (int64_t)b * d.T + t;
-        float oh[NCH][8], s[NCH][8], v[NCH][8], h[NCH][8], dr[NCH][8];     // ohat (or o); scale x gate; scratch; rhat; dR
-        row.load(oh, (const T*)d.o + r * d.o_ld);
-        float rstd_o = 0.f;
-        if (d.post) {
-            const float mean = d.stats[r];
-            rstd_o = d.stats[(int64_t)rows + r];
+        float oh[NCH][8], g[NCH][8], h[NCH][8], v[NCH][8], dR[NCH][8];     // ohat (or o), gate, rhat, scratch, dr then dR
+        const float mo = st[0], so = st[1], mr = st[2], sr = st[3];
 #pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) oh[j][k] = row.has(j, k) ? (oh[j][k] - mean) * rstd_o : 0.f;
-        }
-        float pp[NCH][8];                                                   // p
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) pp[j][k] = oh[j][k];
-        if (d.post) {
-            row.load(v, d.post_w);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) pp[j][k] *= v[j][k];
-            if (d.post_b) {
-                row.load(v, d.post_b);
-#pragma unroll
-                for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) pp[j][k] += v[j][k];
-            }
-        }
-        float gt[NCH][8];
-        if (d.gate) row.load(gt, (const T*)d.gate + (int64_t)b * d.g_bs + (gate_rows ? (int64_t)t * d.g_ts : 0));
-        else
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) gt[j][k] = 1.f;
-        if (d.scale) row.load(s, d.scale);
-        else
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) s[j][k] = 1.f;
-        if (d.dr) row.load(dr, (const T*)d.dr + r * d.C);
-        else
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) dr[j][k] = 0.f;
-        if (d.dn) {
-            const float mean = d.stats[2 * (int64_t)rows + r], rstd = d.stats[3 * (int64_t)rows + r];
-            row.load(h, (const T*)d.x + r * d.x_ld);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) h[j][k] = row.has(j, k) ? (h[j][k] + s[j][k] * gt[j][k] * pp[j][k] - mean) * rstd : 0.f;
-            float dn[NCH][8];
-            row.load(dn, (const T*)d.dn + r * d.C);
-            row.load(v, d.w);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    acc[PLANE_W][j][k] = fmaf(dn[j][k], h[j][k], acc[PLANE_W][j][k]);
-                    acc[PLANE_B][j][k] += dn[j][k];
-                    dn[j][k] *= v[j][k];
-                }
-            norm_back<RW, NCH>(row, dn, h, layer, rstd, red);
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) dr[j][k] += row.has(j, k) ? dn[j][k] : 0.f;
-        }
-        row.store((T*)d.dx + r * d.C, dr);
-        if (d.gate) {
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) { v[j][k] = dr[j][k] * s[j][k] * pp[j][k]; accg[j][k] += v[j][k]; }
-            if (gate_rows) row.store((T*)d.dgate + r * d.C, v);
-        }
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
+        for (int j = 0; j < NCH; ++j) {
+            const float* const pc = &par[0][row.col[j]];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                acc[PLANE_SCALE][j][k] = fmaf(dr[j][k] * gt[j][k], pp[j][k], acc[PLANE_SCALE][j][k]);
-                dr[j][k] *= s[j][k] * gt[j][k];                             // dp
-                acc[PLANE_PW][j][k] = fmaf(dr[j][k], oh[j][k], acc[PLANE_PW][j][k]);
-                acc[PLANE_PB][j][k] += dr[j][k];
+                const bool in = row.has(j, k);
+                const float xh = d.dn ? to_f(rx[j].v[k]) : 0.f;
+                oh[j][k] = in ? (to_f(ro[j].v[k]) - mo) * so : 0.f;         // (mo = 0, so = 1 without a norm)
+                g[j][k] = in ? (gate_rows ? to_f(rg[j].v[k]) : ug[j][k]) : 0.f;
+                dR[j][k] = in && d.dr ? to_f(rdr[j].v[k]) : 0.f;
+                const float pp = fmaf(oh[j][k], pc[W + k], pc[2 * W + k]);
+                h[j][k] = in && d.dn ? (fmaf(pc[k] * g[j][k], pp, xh) - mr) * sr : 0.f;
+                const float dn = in && d.dn ? to_f(rdn[j].v[k]) : 0.f;
+                acc[PLANE_W][j][k] = fmaf(dn, h[j][k], acc[PLANE_W][j][k]);
+                acc[PLANE_B][j][k] += dn;
+                v[j][k] = dn * pc[3 * W + k];
             }
-        if (d.post) {
-            row.load(v, d.post_w);
+        }
+        if (t + step < tb) load(t + step);
+        float s1 = 0.f, s2 = 0.f;
+        const float inv = 1.0f / (float)d.C;
+        if (d.dn) {
 #pragma unroll
             for (int j = 0; j < NCH; ++j)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) dr[j][k] *= v[j][k];
-            norm_back<RW, NCH>(row, dr, oh, layer, rstd_o, red);
+                for (int k = 0; k < 8; ++k) { s1 += v[j][k]; s2 = fmaf(v[j][k], h[j][k], s2); }
+            row_sum2<RW>(s1, s2, red);
+            s1 = layer ? s1 * inv : 0.f;
+            s2 *= inv;
+#pragma unroll
+            for (int j = 0; j < NCH; ++j)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) dR[j][k] += row.has(j, k) ? sr * (v[j][k] - s1 - h[j][k] * s2) : 0.f;
         }
-        row.store((T*)d.d_o + r * d.C, dr);
+        row.store((T*)d.dx + r * d.C, dR);
+        s1 = s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            const float* const pc = &par[0][row.col[j]];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float pp = fmaf(oh[j][k], pc[W + k], pc[2 * W + k]), ds = dR[j][k] * pc[k];
+                v[j][k] = ds * pp;                                          // the gate's gradient
+                const float dg = gate_rows ? dR[j][k] * g[j][k] : dR[j][k];        // (a gate per utterance comes in at the end)
+                acc[PLANE_E1][j][k] = fmaf(dg, oh[j][k], acc[PLANE_E1][j][k]);
+                acc[PLANE_E0][j][k] += dg;
+                h[j][k] = ds * g[j][k] * pc[W + k];                         // dp pw
+                s1 += h[j][k];
+                s2 = fmaf(h[j][k], oh[j][k], s2);
+            }
+        }
+        if (gate_rows) row.store((T*)d.dgate + r * d.C, v);
+        if (d.post) {
+            row_sum2<RW>(s1, s2, red);
+            s1 = layer ? s1 * inv : 0.f;
+            s2 *= inv;
+#pragma unroll
+            for (int j = 0; j < NCH; ++j)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) h[j][k] = so * (h[j][k] - s1 - oh[j][k] * s2);
+        }
+        row.store((T*)d.d_o + r * d.C, h);
     }
-    // block totals: the four waves' rows are joined through LDS when a row is one wave
+    // block totals [4 planes][C], and the utterance gate's gradient behind all blocks' planes.  Its terms per frame are dR scale (pw ohat + pb).
+    float* const part = d.ws + (int64_t)blockIdx.x * PLANES * d.C;
+    float* const partg = d.ws + (int64_t)gridDim.x * PLANES * d.C + (int64_t)blockIdx.x * d.C;
+    const bool utt = d.gate && !gate_rows;
+    float gd[NCH][8];
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        const float* const pc = &par[0][row.col[j]];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            gd[j][k] = pc[k] * fmaf(pc[W + k], acc[PLANE_E1][j][k], pc[2 * W + k] * acc[PLANE_E0][j][k]);
+            if (utt) { acc[PLANE_E1][j][k] *= ug[j][k]; acc[PLANE_E0][j][k] *= ug[j][k]; }
+        }
+    }
     auto emit = [&](float* out, float (&v)[NCH][8]) {
         if constexpr (RW == 1) {
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < NCH; ++j)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) comb[wv * NCH * 512 + row.col[j] + k] = v[j][k];
+                for (int k = 0; k < 8; ++k) par[wv][row.col[j] + k] = v[j][k];
             __syncthreads();
-            for (int c = threadIdx.x; c < d.C; c += 256)
-                out[c] = (comb[c] + comb[NCH * 512 + c]) + (comb[2 * NCH * 512 + c] + comb[3 * NCH * 512 + c]);
+            for (int c = threadIdx.x; c < d.C; c += 256) out[c] = (par[0][c] + par[1][c]) + (par[2][c] + par[3][c]);
         } else {
-#pragma unroll
-            for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (row.col[j] + k < d.C) out[row.col[j] + k] = v[j][k];
+            row.store(out, v);
         }
     };
-    float* const part = d.ws + (int64_t)blockIdx.x * PLANES * d.C;
 #pragma unroll
     for (int q = 0; q < PLANES; ++q) emit(part + (int64_t)q * d.C, acc[q]);
-    if (d.gate && !gate_rows) emit(d.ws + (int64_t)gridDim.x * PLANES * d.C + (int64_t)blockIdx.x * d.C, accg);
+    if (utt) emit(partg, gd);
+}
+
+// the blocks' column sums -> the five parameter gradients.  16 columns per block; wave = plane x quarter of the rows, four rows at a time.
+__global__ __launch_bounds__(1024) void rnorm_reduce_kernel(a8_residual_norm_desc d, int blocks) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q = wv & 3;
+    const int c = blockIdx.x * 16 + (lane & 15), cc = min(c, d.C - 1);
+    const int64_t pitch = (int64_t)PLANES * d.C;
+    const float* const in = d.ws + (int64_t)q * d.C + cc;
+    float s[4] = {};
+    int i = (wv >> 2) * 4 + (lane >> 4);
+    for (; i + 48 < blocks; i += 64)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] += in[(i + 16 * k) * pitch];
+    for (; i < blocks; i += 16) s[0] += in[i * pitch];
+    red[wv][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (threadIdx.x < 16 && c < d.C) {
+        float t[PLANES];
+#pragma unroll
+        for (int k = 0; k < PLANES; ++k) {
+            t[k] = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) t[k] += red[w * 4 + k][g * 16 + lane];
+        }
+        const float sc = d.scale ? d.scale[c] : 1.f, pw = d.post ? d.post_w[c] : 1.f, pb = d.post && d.post_b ? d.post_b[c] : 0.f;
+        auto put = [&](float* out, int add, float v) { if (out) out[c] = add ? out[c] + v : v; };
+        put(d.dw, d.add_dw, t[PLANE_W]);
+        put(d.db, d.add_db, t[PLANE_B]);
+        put(d.dpost_w, d.add_dpost_w, sc * t[PLANE_E1]);
+        put(d.dpost_b, d.add_dpost_b, sc * t[PLANE_E0]);
+        put(d.dscale, d.add_dscale, fmaf(pw, t[PLANE_E1], pb * t[PLANE_E0]));
+    }
 }
 
 // dgate of a gate per utterance: the sum of the utterance's chunks
@@ -365,24 +421,11 @@ NormArgs norm_args(const a8_residual_norm_desc* d) {
     return p;
 }
 
-#define NORM_DISPATCH(KERNEL, BLOCKS1, BLOCKSN)                                                                                     \
-    do {                                                                                                                            \
-        const hipStream_t st = (hipStream_t)stream;                                                                                 \
-        const dim3 g1((unsigned)(BLOCKS1)), gn((unsigned)(BLOCKSN));                                                                \
-        if (d->dtype == A8_BF16) {                                                                                                  \
-            if (d->C <= 512) hipLaunchKernelGGL((KERNEL<bf16, 1, 1>), g1, dim3(256), 0, st, p);                                      \
-            else if (d->C <= 1024) hipLaunchKernelGGL((KERNEL<bf16, 1, 2>), g1, dim3(256), 0, st, p);                                \
-            else if (d->C <= 2048) hipLaunchKernelGGL((KERNEL<bf16, 4, 1>), gn, dim3(256), 0, st, p);                                \
-            else if (d->C <= 4096) hipLaunchKernelGGL((KERNEL<bf16, 8, 1>), gn, dim3(512), 0, st, p);                                \
-            else hipLaunchKernelGGL((KERNEL<bf16, 16, 1>), gn, dim3(1024), 0, st, p);                                                \
-        } else {                                                                                                                    \
-            if (d->C <= 512) hipLaunchKernelGGL((KERNEL<float, 1, 1>), g1, dim3(256), 0, st, p);                                     \
-            else if (d->C <= 1024) hipLaunchKernelGGL((KERNEL<float, 1, 2>), g1, dim3(256), 0, st, p);                               \
-            else if (d->C <= 2048) hipLaunchKernelGGL((KERNEL<float, 4, 1>), gn, dim3(256), 0, st, p);                               \
-            else if (d->C <= 4096) hipLaunchKernelGGL((KERNEL<float, 8, 1>), gn, dim3(512), 0, st, p);                               \
-            else hipLaunchKernelGGL((KERNEL<float, 16, 1>), gn, dim3(1024), 0, st, p);                                               \
-        }                                                                                                                           \
-    } while (0)
+// C <= 1024: a wave per row, four rows side by side; wider: a block per row
+#define NORM_WIDTH(KERNEL, T, ...)                                                                                                \
+    (d->C <= 512 ? (KERNEL<T, 1, 1, ##__VA_ARGS__>) : d->C <= 1024 ? (KERNEL<T, 1, 2, ##__VA_ARGS__>) : d->C <= 2048 ? (KERNEL<T, 4, 1, ##__VA_ARGS__>) \
+     : d->C <= 4096 ? (KERNEL<T, 8, 1, ##__VA_ARGS__>) : (KERNEL<T, 16, 1, ##__VA_ARGS__>))
+int norm_threads(const a8_residual_norm_desc* d) { return d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024; }
 
 }  // namespace
 
@@ -392,7 +435,8 @@ extern "C" int a8_residual_norm_fwd(const a8_residual_norm_desc* d, void* stream
     A8_REQUIRE(d->x && d->o && d->r && (d->w || !d->n), "a8_residual_norm_fwd: null x, o, r or weight");
     const NormArgs p = norm_args(d);
     const int rows = d->B * d->T;
-    NORM_DISPATCH(rnorm_fwd_kernel, cdiv(rows, 4), rows);
+    auto kernel = d->dtype == A8_BF16 ? NORM_WIDTH(rnorm_fwd_kernel, bf16) : NORM_WIDTH(rnorm_fwd_kernel, float);
+    hipLaunchKernelGGL(kernel, dim3(d->C <= 1024 ? cdiv(rows, 4) : rows), dim3(norm_threads(d)), 0, (hipStream_t)stream, p);
     return a8_check_launch("a8_residual_norm_fwd");
 }
 
@@ -410,7 +454,9 @@ extern "C" int a8_residual_norm_bwd(const a8_residual_norm_desc* d, void* stream
     if (blocks > 0) {
         A8_REQUIRE(d->x && d->o && d->dx && d->d_o && d->ws && (d->dgate || !d->gate) && (d->stats || !(d->post || d->dn)) && (d->w || !d->dn),
                    "a8_residual_norm_bwd: null operand");
-        NORM_DISPATCH(rnorm_bwd_kernel, blocks, blocks);
+        auto kernel = d->dtype == A8_BF16 ? (p.vec ? NORM_WIDTH(rnorm_bwd_kernel, bf16, true) : NORM_WIDTH(rnorm_bwd_kernel, bf16, false))
+                                          : (p.vec ? NORM_WIDTH(rnorm_bwd_kernel, float, true) : NORM_WIDTH(rnorm_bwd_kernel, float, false));
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(norm_threads(d)), 0, (hipStream_t)stream, p);
         if (int e = a8_check_launch("a8_residual_norm_bwd")) return e;
     }
     if (d->gate && !d->gate_rows && d->B > 0) {
@@ -420,6 +466,6 @@ extern "C" int a8_residual_norm_bwd(const a8_residual_norm_desc* d, void* stream
         else hipLaunchKernelGGL((rnorm_gate_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, p, part);
         if (int e = a8_check_launch("a8_residual_norm_bwd")) return e;
     }
-    A8SeqReduce r = {d->ws, blocks, PLANES, d->C, 0, nullptr, {d->dw, d->db, d->dpost_w, d->dpost_b, d->dscale}, 0, {d->add_dw, d->add_db, d->add_dpost_w, d->add_dpost_b, d->add_dscale}};
-    return a8i_seq_reduce(r, stream);
+    hipLaunchKernelGGL(rnorm_reduce_kernel, dim3(cdiv(d->C, 16)), dim3(1024), 0, (hipStream_t)stream, *d, blocks);
+    return a8_check_launch("a8_residual_norm_bwd");
 }
