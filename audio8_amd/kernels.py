@@ -388,36 +388,42 @@ def gelu_bwd_bias(dy, z, dbias):
 
 
 # ----------------------------------------------------------------------------- causal sequence operators
+# Each operator's arguments are checked where its descriptor is built; the forward's descriptor comes back for the backward (`desc`), which then
+# only adds its own operands where the saved tensors are still the ones it points to (a saved-tensor hook may have replaced them, and the
+# replacement may even lie at the old address): these calls are short, and the host's share of them counts.
 def _seq_stream(*ts):
     """The current stream of the current device, on which every tensor of the call has to live."""
-    L.require_cuda(*ts)
-    dev = torch.cuda.current_device()
+    dev = torch.cuda.current_device() if torch.cuda.is_initialized() else None
     for t in ts:
         if t is not None and t.get_device() != dev:
-            raise RuntimeError(f"a8hip: a tensor lives on cuda:{t.get_device()}, the current device is cuda:{dev}")
+            L.require_cuda(t)
+            dev = torch.cuda.current_device()
+            if t.get_device() != dev:
+                raise RuntimeError(f"a8hip: a tensor lives on cuda:{t.get_device()}, the current device is cuda:{dev}")
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _act(name, t, shape, dtype):
     """An activation with channels contiguous and any other strides."""
-    if t is None:
+    if t is None or (t.dtype is dtype and t.shape == shape and (t.stride(-1) == 1 or shape[-1] <= 1)):
         return
     if t.dtype != dtype:
         raise TypeError(f"a8hip: {name} is {t.dtype}, expected {dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"a8hip: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise RuntimeError(f"a8hip: {name} needs contiguous channels")
+    raise RuntimeError(f"a8hip: {name} needs contiguous channels")
 
 
 def _dense(name, t, shape, dtype=torch.float32):
+    if t is None or (t.dtype is dtype and t.shape == shape and t.is_contiguous()):
+        return
     _act(name, t, shape, dtype)
-    if t is not None and not t.is_contiguous():
-        raise RuntimeError(f"a8hip: {name} has to be contiguous")
+    raise RuntimeError(f"a8hip: {name} has to be contiguous")
 
 
 CONV_ACTS = {None: 0, "silu": 1}
 NORM_KINDS = {"layer": 0, "rms": 1}
+_DT = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 
 
 def _conv_desc(x, w, bias, act, state, lengths, what):
@@ -426,53 +432,72 @@ def _conv_desc(x, w, bias, act, state, lengths, what):
     if x.dim() != 3:
         raise ValueError(f"a8hip {what}: x has {x.dim()} axes, expected [batch, frames, channels]")
     B, T, Cn = x.shape
-    if w.dim() not in (2, 3) or w.shape[0] != Cn or (w.dim() == 3 and w.shape[1] != 1) or not 2 <= w.shape[-1] <= 4:
-        raise ValueError(f"a8hip {what}: weight has shape {tuple(w.shape)}, expected ({Cn}, taps) or ({Cn}, 1, taps) with 2 to 4 taps")
-    Kn = w.shape[-1]
-    code = L.dt(x)
-    _act("x", x, x.shape, x.dtype)
-    _dense("weight", w, w.shape)
+    ws = w.shape
+    if len(ws) not in (2, 3) or ws[0] != Cn or (len(ws) == 3 and ws[1] != 1) or not 2 <= ws[-1] <= 4:
+        raise ValueError(f"a8hip {what}: weight has shape {tuple(ws)}, expected ({Cn}, taps) or ({Cn}, 1, taps) with 2 to 4 taps")
+    Kn = ws[-1]
+    dtype = x.dtype
+    code = _DT.get(dtype)
+    if code is None:
+        code = L.dt(x)
+    bs, ts, cs = x.stride()
+    if cs != 1 and Cn > 1:
+        raise RuntimeError("a8hip: x needs contiguous channels")
+    _dense("weight", w, ws)
     _dense("bias", bias, (Cn,))
-    _dense("state", state, (B, Kn - 1, Cn), x.dtype)
+    _dense("state", state, (B, Kn - 1, Cn), dtype)
     _dense("lengths", lengths, (B,), torch.int32)
-    d = L.CausalConvDesc(L.CONV_DESC_SIZE, code, B, T, Cn, Kn, CONV_ACTS[act], x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), L.ptr(bias),
-                         L.ptr(state), L.ptr(lengths))
-    return d
+    return L.CausalConvDesc(L.CONV_DESC_SIZE, code, B, T, Cn, Kn, CONV_ACTS[act], x.data_ptr(), bs, ts, w.data_ptr(), L.ptr(bias), L.ptr(state), L.ptr(lengths))
 
 
 def causal_conv_fwd(x, w, bias=None, act="silu", state=None, lengths=None, want_state=False):
-    """x [B,T,C] (channels contiguous, any other strides), w f32 [C,K] or [C,1,K] -> (y [B,T,C], final history [B,K-1,C] or None)."""
+    """x [B,T,C] (channels contiguous, any other strides), w f32 [C,K] or [C,1,K] -> (y [B,T,C], final history [B,K-1,C] or None, descriptor)."""
     d = _conv_desc(x, w, bias, act, state, lengths, "causal_conv_fwd")
     stream = _seq_stream(x, w, bias, state, lengths)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    out = torch.empty((d.B, d.K - 1, d.C), device=x.device, dtype=x.dtype) if want_state else None
-    d.y, d.state_out = y.data_ptr(), L.ptr(out)
+    y = x.new_empty(x.shape)
+    d.y = y.data_ptr()
+    out = None
+    if want_state:
+        out = x.new_empty((d.B, d.K - 1, d.C))
+        d.state_out = out.data_ptr()
     L.check(L.lib().a8_causal_conv_fwd(C.byref(d), stream), "a8_causal_conv_fwd")
-    return y, out
+    return y, out, d
+
+
+_size = C.c_int64
+
+
+def _conv_partials(d):
+    n = _size()
+    L.check(L.lib().a8_causal_conv_bwd_partial_floats(C.byref(d), C.byref(n)), "a8_causal_conv_bwd_partial_floats")
+    return n.value
 
 
 def causal_conv_bwd(dy, x, w, bias=None, act="silu", state=None, lengths=None, dstate_out=None, want_dstate=False, dw=None, dbias=None,
-                    add=(False, False)):
+                    add=(False, False), desc=None):
     """-> (dx, dstate or None); dw f32 (shape of w) and dbias f32 [C] are written (add: accumulated into) when given."""
-    d = _conv_desc(x, w, bias, act, state, lengths, "causal_conv_bwd")
-    _act("dy", dy, x.shape, x.dtype)
-    _dense("dstate_out", dstate_out, (d.B, d.K - 1, d.C), x.dtype)
+    if desc is not None and (desc.x, desc.x_bs, desc.x_ts, 1, desc.w, desc.bias, desc.state, desc.lengths) == \
+            (x.data_ptr(), *x.stride(), w.data_ptr(), L.ptr(bias), L.ptr(state), L.ptr(lengths)):
+        d = L.CausalConvDesc.from_buffer_copy(desc)
+    else:
+        d = _conv_desc(x, w, bias, act, state, lengths, "causal_conv_bwd")
+    dtype = x.dtype
+    _act("dy", dy, x.shape, dtype)
+    _dense("dstate_out", dstate_out, (d.B, d.K - 1, d.C), dtype)
     _dense("dw", dw, w.shape)
     _dense("dbias", dbias, (d.C,))
     stream = _seq_stream(dy, x, w, bias, state, lengths, dstate_out, dw, dbias)
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    dstate = None
+    dx = x.new_empty(x.shape)
+    d.y = d.state_out = dstate = None
     if want_dstate and d.T == 0:             # no frame: the history is handed on
-        dstate = dstate_out.clone() if dstate_out is not None else torch.zeros((d.B, d.K - 1, d.C), device=x.device, dtype=x.dtype)
+        dstate = dstate_out.clone() if dstate_out is not None else torch.zeros((d.B, d.K - 1, d.C), device=x.device, dtype=dtype)
     elif want_dstate:
-        dstate = torch.empty((d.B, d.K - 1, d.C), device=x.device, dtype=x.dtype)
+        dstate = x.new_empty((d.B, d.K - 1, d.C))
         d.dstate = dstate.data_ptr()
-    n = C.c_int64()
-    L.check(L.lib().a8_causal_conv_bwd_partial_floats(C.byref(d), C.addressof(n)), "a8_causal_conv_bwd_partial_floats")
-    part = torch.empty((n.value,), device=x.device, dtype=torch.float32)
-    d.dy, d.dy_bs, d.dy_ts = dy.data_ptr(), dy.stride(0), dy.stride(1)
+    part = torch.empty(_conv_partials(d), device=x.device)
+    d.dy, (d.dy_bs, d.dy_ts, _) = dy.data_ptr(), dy.stride()
     d.dstate_out, d.dx, d.dw, d.dbias = L.ptr(dstate_out), dx.data_ptr(), L.ptr(dw), L.ptr(dbias)
-    d.add_dw, d.add_dbias = (1 if a else 0 for a in add)
+    d.add_dw, d.add_dbias = add
     d.partials = part.data_ptr()
     L.check(L.lib().a8_causal_conv_bwd(C.byref(d), stream), "a8_causal_conv_bwd")
     return dx, dstate
@@ -482,9 +507,11 @@ def causal_conv_step(x, state, w, bias=None, act="silu"):
     """One frame: x [B,C], state [B,K-1,C] (read and updated in place) -> y [B,C]."""
     if x.dim() != 2:
         raise ValueError(f"a8hip causal_conv_step: x has {x.dim()} axes, expected [batch, channels]")
+    if state is None:
+        raise ValueError("a8hip causal_conv_step: a step needs its state")
     d = _conv_desc(x.unsqueeze(1), w, bias, act, state, None, "causal_conv_step")
     stream = _seq_stream(x, w, bias, state)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = x.new_empty(x.shape)
     d.y, d.state, d.state_out = y.data_ptr(), None, state.data_ptr()
     L.check(L.lib().a8_causal_conv_step(C.byref(d), stream), "a8_causal_conv_step")
     return y
@@ -493,56 +520,81 @@ def causal_conv_step(x, state, w, bias=None, act="silu"):
 def _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, what):
     if u.dim() != 3:
         raise ValueError(f"a8hip {what}: u has {u.dim()} axes, expected [batch, frames, channels]")
-    Bn, T, Dn = u.shape
+    us = u.shape
+    Bn, T, Dn = us
     if A.dim() != 2 or A.shape[0] != Dn or not 1 <= A.shape[1] <= 32:
         raise ValueError(f"a8hip {what}: A has shape {tuple(A.shape)}, expected ({Dn}, states) with 1 to 32 states")
     N = A.shape[1]
-    if B.dim() != 4 or B.shape[2] < 1 or Dn % B.shape[2]:
-        raise ValueError(f"a8hip {what}: B has shape {tuple(B.shape)}, expected [batch, frames, groups, states] with groups dividing {Dn} channels")
-    G = B.shape[2]
-    code = L.dt(u)
-    _act("u", u, u.shape, u.dtype)
-    _act("dt", dt, u.shape, u.dtype)
-    _act("z", z, u.shape, u.dtype)
-    _act("B", B, (Bn, T, G, N), u.dtype)
-    _act("C", Cm, (Bn, T, G, N), u.dtype)
+    bs = B.shape
+    if len(bs) != 4 or bs[2] < 1 or Dn % bs[2]:
+        raise ValueError(f"a8hip {what}: B has shape {tuple(bs)}, expected [batch, frames, groups, states] with groups dividing {Dn} channels")
+    G = bs[2]
+    dtype = u.dtype
+    code = _DT.get(dtype)
+    if code is None:
+        code = L.dt(u)
+    want = (Bn, T, G, N)
+    _act("u", u, us, dtype)
+    _act("dt", dt, us, dtype)
+    _act("z", z, us, dtype)
+    _act("B", B, want, dtype)
+    _act("C", Cm, want, dtype)
     _dense("A", A, (Dn, N))
     _dense("D", D, (Dn,))
     _dense("dt_bias", dt_bias, (Dn,))
     _dense("state", state, (Bn, Dn, N))
     _dense("lengths", lengths, (Bn,), torch.int32)
-    zs = (0, 0) if z is None else (z.stride(0), z.stride(1))
-    return L.SelectiveScanDesc(L.SCAN_DESC_SIZE, code, Bn, T, Dn, N, G, 1 if softplus else 0, u.data_ptr(), u.stride(0), u.stride(1),
-                               dt.data_ptr(), dt.stride(0), dt.stride(1), L.ptr(z), zs[0], zs[1], B.data_ptr(), B.stride(0), B.stride(1), B.stride(2),
-                               Cm.data_ptr(), Cm.stride(0), Cm.stride(1), Cm.stride(2), A.data_ptr(), L.ptr(D), L.ptr(dt_bias), L.ptr(state), L.ptr(lengths))
+    u0, u1, _ = u.stride()
+    t0, t1, _ = dt.stride()
+    z0, z1 = (0, 0) if z is None else z.stride()[:2]
+    b0, b1, b2, _ = B.stride()
+    c0, c1, c2, _ = Cm.stride()
+    return L.SelectiveScanDesc(L.SCAN_DESC_SIZE, code, Bn, T, Dn, N, G, 1 if softplus else 0, u.data_ptr(), u0, u1, dt.data_ptr(), t0, t1, L.ptr(z), z0, z1,
+                               B.data_ptr(), b0, b1, b2, Cm.data_ptr(), c0, c1, c2, A.data_ptr(), L.ptr(D), L.ptr(dt_bias), L.ptr(state), L.ptr(lengths))
 
 
 def _scan_sizes(d, backward):
-    ck, ws = C.c_int64(), C.c_int64()
-    L.check(L.lib().a8_selective_scan_workspace(C.byref(d), backward, C.addressof(ck), C.addressof(ws)), "a8_selective_scan_workspace")
+    ck, ws = _size(), _size()
+    L.check(L.lib().a8_selective_scan_workspace(C.byref(d), backward, C.byref(ck), C.byref(ws)), "a8_selective_scan_workspace")
     return ck.value, ws.value
 
 
 def selective_scan_fwd(u, dt, A, B, Cm, D=None, z=None, dt_bias=None, softplus=True, state=None, lengths=None, want_state=False, want_ckpt=False):
     """u, dt, z [B,T,D]; A f32 [D,N]; B, Cm [B,T,G,N] (last axis contiguous, any other strides); state f32 [B,D,N]
-    -> (y [B,T,D], final state f32 [B,D,N] or None, states saved for selective_scan_bwd or None)."""
+    -> (y [B,T,D], final state f32 [B,D,N] or None, states saved for selective_scan_bwd or None, descriptor)."""
     d = _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, "selective_scan_fwd")
     stream = _seq_stream(u, dt, A, B, Cm, D, z, dt_bias, state, lengths)
     nck, nws = _scan_sizes(d, 0)
-    y = torch.empty(u.shape, device=u.device, dtype=u.dtype)
-    out = torch.empty((d.B, d.D, d.N), device=u.device, dtype=torch.float32) if want_state else None
-    ckpt = torch.empty((nck,), device=u.device, dtype=torch.float32) if want_ckpt else None
-    ws = torch.empty((nws,), device=u.device, dtype=torch.float32) if nws else None
-    d.y, d.h_out, d.ckpt, d.ws = y.data_ptr(), L.ptr(out), L.ptr(ckpt), L.ptr(ws)
+    dev = u.device
+    y = u.new_empty(u.shape)
+    d.y = y.data_ptr()
+    out = ckpt = None
+    if want_state:
+        out = torch.empty((d.B, d.D, d.N), device=dev)
+        d.h_out = out.data_ptr()
+    if want_ckpt:
+        ckpt = torch.empty(nck, device=dev)
+        d.ckpt = ckpt.data_ptr()
+    if nws:
+        ws = torch.empty(nws, device=dev)
+        d.ws = ws.data_ptr()
     L.check(L.lib().a8_selective_scan_fwd(C.byref(d), stream), "a8_selective_scan_fwd")
-    return y, out, ckpt
+    return y, out, ckpt, d
 
 
 def selective_scan_bwd(dy, ckpt, u, dt, A, B, Cm, D=None, z=None, dt_bias=None, softplus=True, state=None, lengths=None, dstate_out=None,
-                       want_dstate=False, dA=None, dD=None, ddt_bias=None, add=(False, False, False)):
+                       want_dstate=False, dA=None, dD=None, ddt_bias=None, add=(False, False, False), desc=None):
     """-> (du, ddt, dz or None, dB, dC, dstate or None); dA, dD, ddt_bias (f32) are written (add: accumulated into) when given."""
-    d = _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, "selective_scan_bwd")
-    _act("dy", dy, u.shape, u.dtype)
+    P = L.ptr
+    if desc is not None and (desc.u, desc.u_bs, desc.u_ts, 1, desc.dt, desc.dt_bs, desc.dt_ts, 1, desc.Bm, desc.b_bs, desc.b_ts, desc.b_gs, 1,
+                             desc.Cm, desc.c_bs, desc.c_ts, desc.c_gs, 1, desc.A, desc.Dskip, desc.z, desc.dt_bias, desc.h0, desc.lengths) == \
+            (u.data_ptr(), *u.stride(), dt.data_ptr(), *dt.stride(), B.data_ptr(), *B.stride(), Cm.data_ptr(), *Cm.stride(),
+             A.data_ptr(), P(D), P(z), P(dt_bias), P(state), P(lengths)) and (z is None or (desc.z_bs, desc.z_ts, 1) == z.stride()):
+        d = L.SelectiveScanDesc.from_buffer_copy(desc)
+    else:
+        d = _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, "selective_scan_bwd")
+    us, dtype = u.shape, u.dtype
+    _act("dy", dy, us, dtype)
     _dense("dstate_out", dstate_out, (d.B, d.D, d.N))
     _dense("dA", dA, A.shape)
     _dense("dD", dD, (d.D,))
@@ -551,16 +603,19 @@ def selective_scan_bwd(dy, ckpt, u, dt, A, B, Cm, D=None, z=None, dt_bias=None, 
     nck, nws = _scan_sizes(d, 1)
     _dense("ckpt", ckpt, (nck,))
     dev = u.device
-    du, ddt = torch.empty(u.shape, device=dev, dtype=u.dtype), torch.empty(u.shape, device=dev, dtype=u.dtype)
-    dz = torch.empty(u.shape, device=dev, dtype=u.dtype) if z is not None else None
-    dB, dC = torch.empty(B.shape, device=dev, dtype=u.dtype), torch.empty(B.shape, device=dev, dtype=u.dtype)
-    dstate = torch.empty((d.B, d.D, d.N), device=dev, dtype=torch.float32) if want_dstate else None
-    ws = torch.empty((nws,), device=dev, dtype=torch.float32)
+    if z is not None:
+        du, ddt, dz = u.new_empty((3, *us)).unbind(0)
+    else:
+        (du, ddt), dz = u.new_empty((2, *us)).unbind(0), None
+    dB, dC = u.new_empty((2, *B.shape)).unbind(0)
+    dstate = torch.empty((d.B, d.D, d.N), device=dev) if want_dstate else None
+    ws = torch.empty(nws, device=dev)
+    d.y = d.h_out = None
     d.ckpt, d.ws = ckpt.data_ptr(), ws.data_ptr()
-    d.dy, d.dy_bs, d.dy_ts, d.dh_out = dy.data_ptr(), dy.stride(0), dy.stride(1), L.ptr(dstate_out)
-    d.du, d.ddt, d.dz, d.dBm, d.dCm = du.data_ptr(), ddt.data_ptr(), L.ptr(dz), dB.data_ptr(), dC.data_ptr()
-    d.dA, d.dD, d.ddt_bias, d.dh0 = L.ptr(dA), L.ptr(dD), L.ptr(ddt_bias), L.ptr(dstate)
-    d.add_dA, d.add_dD, d.add_ddt_bias = (1 if a else 0 for a in add)
+    d.dy, (d.dy_bs, d.dy_ts, _), d.dh_out = dy.data_ptr(), dy.stride(), P(dstate_out)
+    d.du, d.ddt, d.dz, d.dBm, d.dCm = du.data_ptr(), ddt.data_ptr(), P(dz), dB.data_ptr(), dC.data_ptr()
+    d.dA, d.dD, d.ddt_bias, d.dh0 = P(dA), P(dD), P(ddt_bias), P(dstate)
+    d.add_dA, d.add_dD, d.add_ddt_bias = add
     L.check(L.lib().a8_selective_scan_bwd(C.byref(d), stream), "a8_selective_scan_bwd")
     return du, ddt, dz, dB, dC, dstate
 
@@ -569,10 +624,12 @@ def selective_scan_step(u, dt, A, B, Cm, state, D=None, z=None, dt_bias=None, so
     """One frame: u, dt, z [B,D]; B, Cm [B,G,N]; state f32 [B,D,N] (read and updated in place) -> y [B,D]."""
     if u.dim() != 2 or B.dim() != 3 or Cm.dim() != 3 or dt.dim() != 2 or (z is not None and z.dim() != 2):
         raise ValueError("a8hip selective_scan_step: u, dt and z are [batch, channels], B and C [batch, groups, states]")
+    if state is None:
+        raise ValueError("a8hip selective_scan_step: a step needs its state")
     d = _scan_desc(u.unsqueeze(1), dt.unsqueeze(1), A, B.unsqueeze(1), Cm.unsqueeze(1), D, z.unsqueeze(1) if z is not None else None, dt_bias,
                    softplus, state, None, "selective_scan_step")
     stream = _seq_stream(u, dt, A, B, Cm, D, z, dt_bias, state)
-    y = torch.empty(u.shape, device=u.device, dtype=u.dtype)
+    y = u.new_empty(u.shape)
     d.y, d.h0, d.h_out = y.data_ptr(), None, state.data_ptr()
     L.check(L.lib().a8_selective_scan_step(C.byref(d), stream), "a8_selective_scan_step")
     return y
@@ -581,11 +638,14 @@ def selective_scan_step(u, dt, A, B, Cm, state, D=None, z=None, dt_bias=None, so
 def _rows_ld(name, t):
     """Leading dimension of [B,T,C] as B * T equally spaced rows."""
     B, T, Cn = t.shape
-    if t.stride(-1) != 1 and Cn > 1:
+    bs, ts, cs = t.stride()
+    if cs != 1 and Cn > 1:
         raise RuntimeError(f"a8hip: {name} needs contiguous channels")
-    if B > 1 and T > 1 and t.stride(0) != T * t.stride(1):
-        raise RuntimeError(f"a8hip: {name} needs equally spaced rows")
-    return t.stride(1) if T > 1 else t.stride(0) if B > 1 else Cn
+    if T > 1:
+        if B > 1 and bs != T * ts:
+            raise RuntimeError(f"a8hip: {name} needs equally spaced rows")
+        return ts
+    return bs if B > 1 else Cn
 
 
 def _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, what):
@@ -598,53 +658,76 @@ def _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, what):
         raise ValueError(f"a8hip {what}: {Cn} channels, expected 1 to 8192")
     if (b is not None and w is None) or (post_b is not None and post_w is None):
         raise ValueError(f"a8hip {what}: a bias without its weight")
-    code = L.dt(x)
-    _act("o", o, x.shape, x.dtype)
-    for name, t in (("weight", w), ("bias", b), ("post_weight", post_w), ("post_bias", post_b), ("scale", scale)):
-        _dense(name, t, (Cn,))
-    g_rows, gs = 0, (0, 0)
+    dtype, col = x.dtype, (Cn,)
+    code = _DT.get(dtype)
+    if code is None:
+        code = L.dt(x)
+    _act("o", o, x.shape, dtype)
+    _dense("weight", w, col)
+    _dense("bias", b, col)
+    _dense("post_weight", post_w, col)
+    _dense("post_bias", post_b, col)
+    _dense("scale", scale, col)
+    rows, g0, g1 = 0, 0, 0
     if gate is not None:
-        g_rows = 1 if gate.dim() == 3 and gate.shape[1] == T else 0
-        _act("gate", gate, (B, T if g_rows else 1, Cn), x.dtype)
-        gs = gate.stride(0), gate.stride(1)
-    return L.ResidualNormDesc(L.RNORM_DESC_SIZE, code, B, T, Cn, NORM_KINDS[kind], 1 if post_w is not None else 0, g_rows, eps,
-                              x.data_ptr(), _rows_ld("x", x), o.data_ptr(), _rows_ld("o", o), L.ptr(gate), gs[0], gs[1], L.ptr(scale), L.ptr(w), L.ptr(b),
-                              L.ptr(post_w), L.ptr(post_b))
+        rows = 1 if gate.dim() == 3 and gate.shape[1] == T else 0
+        _act("gate", gate, (B, T if rows else 1, Cn), dtype)
+        g0, g1, _ = gate.stride()
+    P = L.ptr
+    return L.ResidualNormDesc(L.RNORM_DESC_SIZE, code, B, T, Cn, NORM_KINDS[kind], 1 if post_w is not None else 0, rows, eps,
+                              x.data_ptr(), _rows_ld("x", x), o.data_ptr(), _rows_ld("o", o), P(gate), g0, g1, P(scale), P(w), P(b), P(post_w), P(post_b))
 
 
 def residual_norm_fwd(x, o, w=None, b=None, post_w=None, post_b=None, gate=None, scale=None, eps=1e-6, kind="layer", want_stats=False):
-    """x, o [B,T,C]; gate [B,T,C] or [B,1,C]; norm parameters and scale f32 [C] -> (r, n or None when w is None, stats f32 [4, B*T] or None)."""
+    """x, o [B,T,C]; gate [B,T,C] or [B,1,C]; norm parameters and scale f32 [C]
+    -> (r, n or None when w is None, stats f32 [4, B*T] or None, descriptor)."""
     d = _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, "residual_norm_fwd")
     stream = _seq_stream(x, o, w, b, post_w, post_b, gate, scale)
-    r = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    n = torch.empty(x.shape, device=x.device, dtype=x.dtype) if w is not None else None
-    stats = torch.empty((4, d.B * d.T), device=x.device, dtype=torch.float32) if want_stats else None
-    d.r, d.n, d.stats = r.data_ptr(), L.ptr(n), L.ptr(stats)
+    n = stats = None
+    if w is not None:
+        n = x.new_empty(x.shape)
+        d.n = n.data_ptr()
+    r = x.new_empty(x.shape)
+    d.r = r.data_ptr()
+    if want_stats:
+        stats = torch.empty((4, d.B * d.T), device=x.device)
+        d.stats = stats.data_ptr()
     L.check(L.lib().a8_residual_norm_fwd(C.byref(d), stream), "a8_residual_norm_fwd")
-    return r, n, stats
+    return r, n, stats, d
 
 
 def residual_norm_bwd(dr, dn, stats, x, o, w=None, b=None, post_w=None, post_b=None, gate=None, scale=None, eps=1e-6, kind="layer", dw=None, db=None,
-                      dpost_w=None, dpost_b=None, dscale=None, add=(False,) * 5):
+                      dpost_w=None, dpost_b=None, dscale=None, add=(False,) * 5, desc=None):
     """-> (dx, do, dgate or None); the parameter gradients (f32 [C], in the order of `add`) are written (add: accumulated into) when given."""
-    d = _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, "residual_norm_bwd")
-    _dense("dr", dr, x.shape, x.dtype)
-    _dense("dn", dn, x.shape, x.dtype)
+    P = L.ptr
+    if desc is not None and (desc.x, desc.x_ld, desc.o, desc.o_ld, desc.w, desc.b, desc.post_w, desc.post_b, desc.gate, desc.scale) == \
+            (x.data_ptr(), _rows_ld("x", x), o.data_ptr(), _rows_ld("o", o), P(w), P(b), P(post_w), P(post_b), P(gate), P(scale)) and \
+            (gate is None or (desc.g_bs, desc.g_ts, 1) == gate.stride()):
+        d = L.ResidualNormDesc.from_buffer_copy(desc)
+    else:
+        d = _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, "residual_norm_bwd")
+    xs, dtype, col = x.shape, x.dtype, (d.C,)
+    _dense("dr", dr, xs, dtype)
+    _dense("dn", dn, xs, dtype)
     _dense("stats", stats, (4, d.B * d.T))
-    for name, t in (("dw", dw), ("db", db), ("dpost_w", dpost_w), ("dpost_b", dpost_b), ("dscale", dscale)):
-        _dense(name, t, (d.C,))
+    _dense("dw", dw, col)
+    _dense("db", db, col)
+    _dense("dpost_w", dpost_w, col)
+    _dense("dpost_b", dpost_b, col)
+    _dense("dscale", dscale, col)
     if dn is not None and w is None:
         raise ValueError("a8hip residual_norm_bwd: dn without the second norm's weight")
     stream = _seq_stream(dr, dn, stats, x, o, w, b, post_w, post_b, gate, scale, dw, db, dpost_w, dpost_b, dscale)
-    dx, do = torch.empty(x.shape, device=x.device, dtype=x.dtype), torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    dgate = torch.empty(gate.shape, device=x.device, dtype=x.dtype) if gate is not None else None
-    ptrs = (dr, dn, dx, do, dgate, dw, db, dpost_w, dpost_b, dscale)
-    d.dr, d.dn, d.dx, d.d_o, d.dgate, d.dw, d.db, d.dpost_w, d.dpost_b, d.dscale = (L.ptr(t) for t in ptrs)
+    dx, do = x.new_empty((2, *xs)).unbind(0)
+    dgate = x.new_empty(gate.shape) if gate is not None else None
+    d.r = d.n = None
+    d.dr, d.dn, d.dx, d.d_o, d.dgate, d.dw, d.db, d.dpost_w, d.dpost_b, d.dscale = \
+        P(dr), P(dn), dx.data_ptr(), do.data_ptr(), P(dgate), P(dw), P(db), P(dpost_w), P(dpost_b), P(dscale)
     d.stats = stats.data_ptr()
-    d.add_dw, d.add_db, d.add_dpost_w, d.add_dpost_b, d.add_dscale = (1 if a else 0 for a in add)
-    n = C.c_int64()
-    L.check(L.lib().a8_residual_norm_bwd_workspace(C.byref(d), C.addressof(n)), "a8_residual_norm_bwd_workspace")
-    ws = torch.empty((n.value,), device=x.device, dtype=torch.float32)
+    d.add_dw, d.add_db, d.add_dpost_w, d.add_dpost_b, d.add_dscale = add
+    n = _size()
+    L.check(L.lib().a8_residual_norm_bwd_workspace(C.byref(d), C.byref(n)), "a8_residual_norm_bwd_workspace")
+    ws = torch.empty(n.value, device=x.device)
     d.ws = ws.data_ptr()
     L.check(L.lib().a8_residual_norm_bwd(C.byref(d), stream), "a8_residual_norm_bwd")
     return dx, do, dgate

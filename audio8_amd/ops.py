@@ -495,24 +495,26 @@ def _param_grads(ctx, params):
     """Targets of the parameter gradients, per parameter (position in the forward's arguments, tensor): p.grad when gradients go there
     directly, a fresh tensor otherwise, None when not needed.  -> (targets, add flags, gradients to return)."""
     tgts, add, ret = [], [], []
+    needs = ctx.needs_input_grad
     for at, p in params:
         t = g = None
-        if p is not None and ctx.needs_input_grad[at]:
-            t = _target(p) if p.is_leaf else None
-            add.append(t is not None)
+        direct = False
+        if p is not None and needs[at]:
+            if DIRECT_GRADS and p.is_leaf:
+                t = _target(p)
             if t is None:
-                t = g = torch.empty(p.shape, device=p.device, dtype=torch.float32)
-        else:
-            add.append(False)
+                t = g = torch.empty_like(p)
+            else:
+                direct = True
         tgts.append(t)
+        add.append(direct)
         ret.append(g)
     return tgts, add, ret
 
 
 def _ready_direct(params, add):
-    for (_, p), a in zip(params, add):
-        if a:
-            _ready(p)
+    if True in add:
+        _ready(*(p for (_, p), a in zip(params, add) if a))
 
 
 def _rows(t):
@@ -528,7 +530,7 @@ def _step_only(what, *ts):
 class CausalConvFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, lengths, act, want_state):
-        y, out = K.causal_conv_fwd(x.detach(), weight.detach(), bias.detach() if bias is not None else None, act, state, lengths, want_state)
+        y, out, ctx.desc = K.causal_conv_fwd(x, weight, bias, act, state, lengths, want_state)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, state, lengths, weight, bias)
         ctx.act, ctx.params = act, ((1, weight), (2, bias))
@@ -541,7 +543,7 @@ class CausalConvFn(torch.autograd.Function):
         dy = torch.zeros(x.shape, device=x.device, dtype=x.dtype) if dy is None else _rows(dy)
         dout = dout.contiguous() if dout is not None else None
         (dw, db), add, ret = _param_grads(ctx, ctx.params)
-        dx, dstate = K.causal_conv_bwd(dy, x, weight, bias, ctx.act, state, lengths, dout, ctx.needs_input_grad[3], dw, db, add)
+        dx, dstate = K.causal_conv_bwd(dy, x, weight, bias, ctx.act, state, lengths, dout, ctx.needs_input_grad[3], dw, db, add, ctx.desc)
         _ready_direct(ctx.params, add)
         return dx, ret[0], ret[1], dstate, None, None, None
 
@@ -560,7 +562,7 @@ def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=
 def causal_conv_step(x, state, weight, bias=None, *, activation="silu"):
     """One frame of causal_conv for each utterance: x [B, C], state [B, K - 1, C] updated in place -> y [B, C].  No gradient."""
     _step_only("causal_conv_step", x, state)
-    y = K.causal_conv_step(_rows(x), state, weight.detach(), bias.detach() if bias is not None else None, activation)
+    y = K.causal_conv_step(_rows(x), state, weight, bias, activation)
     torch.autograd.graph.increment_version(state)
     return y
 
@@ -569,12 +571,11 @@ class SelectiveScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state):
         grad = any(ctx.needs_input_grad)
-        y, out, ckpt = K.selective_scan_fwd(u.detach(), dt, A.detach(), B, C, D.detach() if D is not None else None, z,
-                                            dt_bias.detach() if dt_bias is not None else None, softplus, state, lengths, want_state, grad)
-        ctx.set_materialize_grads(False)
+        y, out, ckpt, desc = K.selective_scan_fwd(u, dt, A, B, C, D, z, dt_bias, softplus, state, lengths, want_state, grad)
         if grad:
+            ctx.set_materialize_grads(False)
             ctx.save_for_backward(u, dt, A, B, C, D, z, dt_bias, state, lengths, ckpt)
-            ctx.softplus, ctx.params = softplus, ((2, A), (5, D), (7, dt_bias))
+            ctx.desc, ctx.softplus, ctx.params = desc, softplus, ((2, A), (5, D), (7, dt_bias))
         return y, out
 
     @staticmethod
@@ -585,7 +586,7 @@ class SelectiveScanFn(torch.autograd.Function):
         dout = dout.contiguous() if dout is not None else None
         (dA, dD, db), add, ret = _param_grads(ctx, ctx.params)
         du, ddt, dz, dB, dC, dstate = K.selective_scan_bwd(dy, ckpt, u, dt, A, B, C, D, z, dt_bias, ctx.softplus, state, lengths, dout,
-                                                           ctx.needs_input_grad[8], dA, dD, db, add)
+                                                           ctx.needs_input_grad[8], dA, dD, db, add, ctx.desc)
         _ready_direct(ctx.params, add)
         return du, ddt, ret[0], dB, dC, ret[1], dz, ret[2], dstate, None, None, None
 
@@ -610,8 +611,7 @@ def selective_scan_step(u, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, 
     _step_only("selective_scan_step", u, dt, B, C, z, state)
     if B.dim() == 2 and C.dim() == 2:
         B, C = B.unsqueeze(1), C.unsqueeze(1)
-    y = K.selective_scan_step(_rows(u), _rows(dt), A.detach(), _rows(B), _rows(C), state, D.detach() if D is not None else None, _rows(z),
-                              dt_bias.detach() if dt_bias is not None else None, softplus)
+    y = K.selective_scan_step(_rows(u), _rows(dt), A, _rows(B), _rows(C), state, D, _rows(z), dt_bias, softplus)
     torch.autograd.graph.increment_version(state)
     return y
 
@@ -620,12 +620,11 @@ class GatedResidualNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, o, weight, bias, post_weight, post_bias, gate, scale, eps, kind):
         grad = any(ctx.needs_input_grad)
-        r, n, stats = K.residual_norm_fwd(x, o, *(p.detach() if p is not None else None for p in (weight, bias, post_weight, post_bias)), gate,
-                                          scale.detach() if scale is not None else None, eps, kind, grad)
-        ctx.set_materialize_grads(False)
+        r, n, stats, desc = K.residual_norm_fwd(x, o, weight, bias, post_weight, post_bias, gate, scale, eps, kind, grad)
         if grad:
+            ctx.set_materialize_grads(False)
             ctx.save_for_backward(x, o, weight, bias, post_weight, post_bias, gate, scale, stats)
-            ctx.eps, ctx.kind = eps, kind
+            ctx.desc, ctx.eps, ctx.kind = desc, eps, kind
             ctx.params = ((2, weight), (3, bias), (4, post_weight), (5, post_bias), (7, scale))
         return r, n
 
@@ -635,7 +634,7 @@ class GatedResidualNormFn(torch.autograd.Function):
         x, o, w, b, pw, pb, gate, scale, stats = ctx.saved_tensors
         tgts, add, ret = _param_grads(ctx, ctx.params)
         dx, do, dgate = K.residual_norm_bwd(dr.contiguous() if dr is not None else None, dn.contiguous() if dn is not None else None, stats, x, o,
-                                            w, b, pw, pb, gate, scale, ctx.eps, ctx.kind, *tgts, add=add)
+                                            w, b, pw, pb, gate, scale, ctx.eps, ctx.kind, *tgts, add, ctx.desc)
         _ready_direct(ctx.params, add)
         return dx, do, ret[0], ret[1], ret[2], ret[3], dgate, ret[4], None, None
 

@@ -546,3 +546,33 @@ def test_a_step_marks_its_state_as_changed():
         ops.causal_conv_step(x[:, 0], st, w)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_saved_tensor_hooks_that_replace_what_was_saved():
+    """A hook that keeps copies elsewhere hands other tensors (dense ones, perhaps at a freed tensor's address) to the backward."""
+    from audio8_amd import ops
+    v = _train_inputs(4)
+    want = _train(ops, v)
+    wide_x = torch.cat([v["x"].detach(), v["x"].detach()], -1)
+
+    def pack(t):
+        return t.detach().cpu()
+
+    def unpack(t):
+        return t.cuda()
+    v["x"] = wide_x[..., :136].requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        got = _train(ops, v)
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+
+
+def test_a_graph_walked_twice_gives_the_same_gradients():
+    from audio8_amd import ops
+    x, w = cu(rnd(2, 30, 64, seed=1), True), cu(rnd(64, 4, seed=2), True)
+    A, bc = cu(-rnd(64, 16, seed=3).exp(), True), cu(rnd(2, 30, 16, seed=4), True)
+    y = ops.selective_scan(ops.causal_conv(x, w), x, A, bc, bc)
+    r, n = ops.gated_residual_norm(x, y, cu(rnd(64, seed=5)))
+    first, second = (torch.autograd.grad([r, n], [x, w, A, bc], [r.detach(), n.detach()], retain_graph=True) for _ in range(2))
+    for p, q in zip(first, second):
+        assert torch.equal(p, q)
