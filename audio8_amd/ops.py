@@ -494,21 +494,18 @@ class ZeroFn(torch.autograd.Function):
 def _param_grads(ctx, params):
     """Targets of the parameter gradients, per parameter (position in the forward's arguments, tensor): p.grad when gradients go there
     directly, a fresh tensor otherwise, None when not needed.  -> (targets, add flags, gradients to return)."""
-    tgts, add, ret = [], [], []
     needs = ctx.needs_input_grad
-    for at, p in params:
-        t = g = None
-        direct = False
-        if p is not None and needs[at]:
-            if DIRECT_GRADS and p.is_leaf:
-                t = _target(p)
-            if t is None:
-                t = g = torch.empty_like(p)
-            else:
-                direct = True
-        tgts.append(t)
-        add.append(direct)
-        ret.append(g)
+    tgts = [_target(p) if DIRECT_GRADS and p is not None and p.is_leaf and needs[at] else None for at, p in params]
+    fresh = [i for i, (at, p) in enumerate(params) if p is not None and needs[at] and tgts[i] is None]
+    add = [t is not None for t in tgts]
+    ret = [None] * len(params)
+    like = params[fresh[0]][1] if fresh else None
+    if len(fresh) > 2 and all(params[i][1].shape == like.shape for i in fresh):
+        slab = torch.empty((len(fresh), *like.shape), device=like.device).unbind(0)          # one allocation for a norm's handful of columns
+    else:
+        slab = [torch.empty_like(params[i][1]) for i in fresh]
+    for i, g in zip(fresh, slab):
+        tgts[i] = ret[i] = g
     return tgts, add, ret
 
 
