@@ -14,18 +14,15 @@ A8_DEV float silu_grad_f(float x) {
     const float s = x >= 0.f ? big : small, c = x >= 0.f ? small : big;
     return s * fmaf(x, c, 1.0f);
 }
-// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1].  log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, by its odd series up to
-// s^15 (the first term left out is < 2 (1/3)^17 / 17 = 9e-10): no 1 + e is rounded, so small step lengths keep their relative precision.
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1].  log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, with 2 atanh(s) / s as a polynomial of
+// degree 4 in s^2 (Chebyshev fit on [0, 1/9]: 4e-9 off, 7e-8 evaluated in f32): no 1 + e is rounded, so small step lengths keep their relative precision.
 A8_DEV float softplus_f(float x) {
     const float e = exp_fast(-fabsf(x));
     const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
-    float r = 2.0f / 15.0f;
-    r = fmaf(r, q, 2.0f / 13.0f);
-    r = fmaf(r, q, 2.0f / 11.0f);
-    r = fmaf(r, q, 2.0f / 9.0f);
-    r = fmaf(r, q, 2.0f / 7.0f);
-    r = fmaf(r, q, 2.0f / 5.0f);
-    r = fmaf(r, q, 2.0f / 3.0f);
+    float r = 0.2817465662956238f;
+    r = fmaf(r, q, 0.2796141803264618f);
+    r = fmaf(r, q, 0.40024852752685547f);
+    r = fmaf(r, q, 0.6666631698608398f);
     r = fmaf(r, q, 2.0f);
     return fmaf(s, r, fmaxf(x, 0.f));
 }

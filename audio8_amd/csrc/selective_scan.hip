@@ -51,6 +51,15 @@ A8_DEV Where locate(const ScanArgs& p, int lane, int first_chunk, int nchunks) {
 // row (b, t) of a strided input: a wave-uniform address, so that a load is one scalar base and one 32-bit lane offset
 template <typename T> A8_DEV const T* row_of(const void* p, int64_t bs, int64_t ts, int b, int t) { return (const T*)p + (b * bs + t * ts); }
 
+// The lane's byte offset in such a row, kept apart from the row's address: folded into it once, every access would need a 64-bit add of its own.
+template <typename T> A8_DEV uint32_t lane_bytes(int ch) {
+    uint32_t o = (uint32_t)ch * sizeof(T);
+    asm volatile("" : "+v"(o));
+    return o;
+}
+template <typename T> A8_DEV T ld_at(const T* row, uint32_t bytes) { return *(const T*)((const char*)row + bytes); }
+template <typename T> A8_DEV void st_at(T* row, uint32_t bytes, T v) { *(T*)((char*)row + bytes) = v; }
+
 // value I of the 16 that every row of 16 lanes holds in v, as a DPP operand
 template <int I> A8_DEV float row_value(float v) { return dpp_f<0x150 + I>(v); }
 template <int... I, typename F> A8_DEV void unroll_impl(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>()), ...); }
@@ -62,13 +71,14 @@ template <typename T, int NW, int NS, bool Z, bool DY> struct TileRegs {
     static constexpr int EP = TT / NW, BC = NS * NW;       // (frame, channel) elements per thread: frames wv, wv + NW, ...; states of the block
     T u[EP], dt[EP], z[Z ? EP : 1], dy[DY ? EP : 1], b, c;
     A8_DEV void load(const a8_selective_scan_desc& d, const Where& w, int wv, int t0) {
+        const uint32_t at = lane_bytes<T>(w.ch);
 #pragma unroll
         for (int j = 0; j < EP; ++j) {
             const int t = min(t0 + wv + NW * j, w.len - 1);
-            u[j] = row_of<T>(d.u, d.u_bs, d.u_ts, w.b, t)[(uint32_t)w.ch];
-            dt[j] = row_of<T>(d.dt, d.dt_bs, d.dt_ts, w.b, t)[(uint32_t)w.ch];
-            if constexpr (Z) z[j] = row_of<T>(d.z, d.z_bs, d.z_ts, w.b, t)[(uint32_t)w.ch];
-            if constexpr (DY) dy[j] = row_of<T>(d.dy, d.dy_bs, d.dy_ts, w.b, t)[(uint32_t)w.ch];
+            u[j] = ld_at(row_of<T>(d.u, d.u_bs, d.u_ts, w.b, t), at);
+            dt[j] = ld_at(row_of<T>(d.dt, d.dt_bs, d.dt_ts, w.b, t), at);
+            if constexpr (Z) z[j] = ld_at(row_of<T>(d.z, d.z_bs, d.z_ts, w.b, t), at);
+            if constexpr (DY) dy[j] = ld_at(row_of<T>(d.dy, d.dy_bs, d.dy_ts, w.b, t), at);
         }
         // B and C: one value per thread (at most: TT BC <= 64 NW), frame tid / BC, state tid % BC
         const int n = min((int)threadIdx.x % BC, d.N - 1), t = min(t0 + (int)threadIdx.x / BC, w.len - 1);
@@ -101,6 +111,13 @@ template <int I> A8_DEV void row_dot4x2(float (&y)[4], float v, const float (&x)
           "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3), "n"(I + 4), "n"(I + 5), "n"(I + 6), "n"(I + 7));
 }
 #undef A8_RB
+#define A8_RM(o, x, i) "v_mul_f32_dpp %" #o ", %8, %" #x " row_newbcast:%" #i " row_mask:0xf bank_mask:0xf\n\t"
+template <int I> A8_DEV void row_outer4x2(float (&o)[4][2], float v, float x0, float x1, float x2, float x3) {       // o[f][n] = row value (I + 2 f + n) of v * x_f
+    asm("s_nop 1\n\t" A8_RM(0, 9, 13) A8_RM(1, 9, 14) A8_RM(2, 10, 15) A8_RM(3, 10, 16) A8_RM(4, 11, 17) A8_RM(5, 11, 18) A8_RM(6, 12, 19) A8_RM(7, 12, 20)
+        : "=&v"(o[0][0]), "=&v"(o[0][1]), "=&v"(o[1][0]), "=&v"(o[1][1]), "=&v"(o[2][0]), "=&v"(o[2][1]), "=&v"(o[3][0]), "=&v"(o[3][1])
+        : "v"(v), "v"(x0), "v"(x1), "v"(x2), "v"(x3), "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3), "n"(I + 4), "n"(I + 5), "n"(I + 6), "n"(I + 7));
+}
+#undef A8_RM
 template <int I> A8_DEV float row_dot(float v, const float (&x)[4]) {
     float acc;
     asm("s_nop 1\n\tv_mul_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n\t"
@@ -150,6 +167,7 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
             const float raw = to_f(nx.dt[j]) + bias, s = sp ? softplus_f(raw) : raw, u = to_f(nx.u[j]);
             const bool in = t0 + t < w.len;
             s_dx[t][lane] = make_float2(in ? s : 0.f, in ? s * u : 0.f);
+            if constexpr (ENDS) sum += in ? s : 0.f;
         }
         nx.stage_bc(d, w, t0, s_b, s_c);
     };
@@ -171,15 +189,14 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
         unroll<TT / 4>([&](auto qc) {
             constexpr int t4 = 4 * decltype(qc)::value;
             float hq[4][NS], y[4];
-            unroll<4>([&](auto tc) {
-                constexpr int f = decltype(tc)::value, t = t4 + f;
-                const float2 dx = s_dx[t][lane];
-                if constexpr (ENDS) sum += dx.x;
-                unroll<NS>([&](auto nc) {
-                    constexpr int n = decltype(nc)::value;
-                    hq[f][n] = fmaf(__builtin_amdgcn_exp2f(dx.x * A2[n]), f ? hq[f ? f - 1 : 0][n] : h[n], dx.y * bc_at<NS, t, n>(bv));
-                });
-            });
+            float2 dx[4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) dx[f] = s_dx[t4 + f][lane];
+            row_outer4x2<(t4 % 8) * 2>(hq, bv[t4 / 8], dx[0].y, dx[1].y, dx[2].y, dx[3].y);      // D u B, then the state in its place
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int n = 0; n < NS; ++n) hq[f][n] = fmaf(__builtin_amdgcn_exp2f(dx[f].x * A2[n]), f ? hq[f ? f - 1 : 0][n] : h[n], hq[f][n]);
 #pragma unroll
             for (int n = 0; n < NS; ++n) h[n] = hq[3][n];
             if constexpr (!ENDS) {
@@ -190,7 +207,8 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
         });
         lds_barrier();
         if (i + 1 < w.i1) stage(t0 + TT);                  // (the loads are a tile old; the stores below are not waited for)
-        if constexpr (!ENDS)
+        if constexpr (!ENDS) {
+            const uint32_t at = lane_bytes<T>(w.ch);
 #pragma unroll
             for (int j = 0; j < EP; ++j) {
                 const int t = wv + NW * j;
@@ -198,8 +216,16 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
 #pragma unroll
                 for (int v = 0; v < NW; ++v) y += s_y[v][t][lane];
                 if constexpr (Z) y *= silu_f(to_f(cu.z[j]));
-                if (t0 + t < w.len && w.live) ((T*)d.y + ((int64_t)w.b * d.T + t0 + t) * d.D)[(uint32_t)w.ch] = from_f<T>(y);
+                if (t0 + t < w.len && w.live) st_at((T*)d.y + ((int64_t)w.b * d.T + t0 + t) * d.D, at, from_f<T>(y));
             }
+        }
+    }
+    if constexpr (ENDS) {                                  // the block's sum of steps: each thread's own frames, then the waves
+        s_y[0][wv][lane] = sum;
+        lds_barrier();
+        sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < NW; ++v) sum += s_y[0][v][lane];
     }
     if (!w.live) return;
     if constexpr (ENDS) {
@@ -383,6 +409,7 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
                     p.part_c[at] = sc;
                 }
             }
+            const uint32_t at = lane_bytes<T>(w.ch);
 #pragma unroll
             for (int j = 0; j < EP; ++j) {
                 const int t = wv + NW * j;
@@ -399,12 +426,12 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
                     dz = to_f(cu.dy[j]) * y * silu_grad_f(to_f(cu.z[j]));
                 }
                 if (t0 + t < w.len && w.live) {
-                    const int64_t at = ((int64_t)w.b * d.T + t0 + t) * d.D;
+                    const int64_t row = ((int64_t)w.b * d.T + t0 + t) * d.D;
                     dskip = fmaf(g, u, dskip);
                     dbias += dd;
-                    ((T*)d.du + at)[(uint32_t)w.ch] = from_f<T>(fmaf(s_dx[t][lane].x, qb, skip * g));
-                    ((T*)d.ddt + at)[(uint32_t)w.ch] = from_f<T>(dd);
-                    if constexpr (Z) ((T*)d.dz + at)[(uint32_t)w.ch] = from_f<T>(dz);
+                    st_at((T*)d.du + row, at, from_f<T>(fmaf(s_dx[t][lane].x, qb, skip * g)));
+                    st_at((T*)d.ddt + row, at, from_f<T>(dd));
+                    if constexpr (Z) st_at((T*)d.dz + row, at, from_f<T>(dz));
                 }
             }
         }
