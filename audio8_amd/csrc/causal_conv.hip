@@ -232,20 +232,20 @@ template <typename T, int K> __global__ __launch_bounds__(256) void conv_step_ke
     for (int k = 0; k < K - 1; ++k) st[(int64_t)k * d.C] = e[k + 1];
 }
 
-// 16 columns of one plane per block; the 16 waves take four rows at a time (a quarter of the lanes each), four loads in flight, and meet in LDS.
+// 16 columns of one plane per block; the 16 waves take four rows at a time (a quarter of the lanes each), eight loads in flight, and meet in LDS.
 __global__ __launch_bounds__(1024) void seq_reduce_kernel(A8SeqReduce r) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int c = blockIdx.x * 16 + (lane & 15), q = blockIdx.y;
     const float* const in = r.in + (int64_t)q * r.C + min(c, r.C - 1);
     const int64_t pitch = (int64_t)r.planes * r.C;
-    float s[4] = {};
+    float s[8] = {};
     int i = wv * 4 + (lane >> 4);
-    for (; i + 192 < r.rows; i += 256)
+    for (; i + 448 < r.rows; i += 512)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] += in[(i + 64 * k) * pitch];
+        for (int k = 0; k < 8; ++k) s[k] += in[(i + 64 * k) * pitch];
     for (; i < r.rows; i += 64) s[0] += in[i * pitch];
-    red[wv][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    red[wv][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (threadIdx.x < 16 && c < r.C) {
         float t = 0.f;

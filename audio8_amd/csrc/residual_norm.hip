@@ -14,7 +14,7 @@
 
 namespace {
 
-enum { PLANE_W = 0, PLANE_B, PLANE_E1, PLANE_E0, PLANES };
+enum { PLANE_W = 0, PLANE_B, PLANE_E1, PLANE_E0, PLANES };      // (rnorm_reduce_kernel takes them in pairs)
 
 struct NormArgs { a8_residual_norm_desc d; int chunks, rows_per_chunk, vec; };
 
@@ -207,7 +207,9 @@ template <int RW> A8_DEV void row_sum2(float& a, float& b, float2* red) {
     }
 }
 
-template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void rnorm_bwd_kernel(NormArgs p) {
+enum { GATE_NONE = 0, GATE_ROWS, GATE_UTT };
+// (the kind of gate is a template parameter for its registers: with all three in one kernel a row of 1024 took 314 and one wave per SIMD)
+template <typename T, int RW, int NCH, bool VEC, int GATE> __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void rnorm_bwd_kernel(NormArgs p) {
     typedef Row<T, RW, NCH> R;
     constexpr int W = R::NT * NCH * 8;                         // columns a row's threads cover
     __shared__ float2 red[R::WAVES];
@@ -218,7 +220,8 @@ template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW
     const int rows = d.B * d.T, b = blockIdx.x / p.chunks, ck = blockIdx.x % p.chunks;
     const int ta = ck * p.rows_per_chunk, tb = min(ta + p.rows_per_chunk, d.T);
     const int wv = RW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, step = RW == 1 ? 4 : 1;
-    const bool layer = d.kind == A8_NORM_LAYER, gate_rows = d.gate && d.gate_rows;
+    constexpr bool gate_rows = GATE == GATE_ROWS;
+    const bool layer = d.kind == A8_NORM_LAYER;
     for (int c = threadIdx.x; c < W; c += R::WAVES * 64) {
         const bool in = c < d.C;
         par[0][c] = in && d.scale ? d.scale[c] : 1.f;
@@ -227,13 +230,14 @@ template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW
         par[3][c] = in && d.w ? d.w[c] : 1.f;
     }
     __syncthreads();
-    float acc[PLANES][NCH][8] = {}, ug[NCH][8];                // ug: the utterance's gate, 1 without one; gates per frame are loaded with the rows
+    float acc[PLANES][NCH][8] = {};
+    Raw<T> ug[GATE == GATE_UTT ? NCH : 1], rg[GATE == GATE_ROWS ? NCH : 1];       // the utterance's gate; the row's
+    if constexpr (GATE == GATE_UTT)
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ug[j][k] = 1.f;
-    if (d.gate && !gate_rows) row.load(ug, (const T*)d.gate + (int64_t)b * d.g_bs);
-    Raw<T> ro[NCH], rx[NCH], rdr[NCH], rdn[NCH], rg[NCH];
+        for (int j = 0; j < NCH; ++j)
+            if (row.on[j]) ug[j].load((const T*)d.gate + (int64_t)b * d.g_bs + row.col[j], VEC, d.C - row.col[j]);
+    auto gate_of = [&](int j, int k) { return GATE == GATE_ROWS ? to_f(rg[GATE == GATE_ROWS ? j : 0].v[k]) : GATE == GATE_UTT ? to_f(ug[GATE == GATE_UTT ? j : 0].v[k]) : 1.f; };
+    Raw<T> ro[NCH], rx[NCH], rdr[NCH], rdn[NCH];
     float st[4];
     auto load = [&](int t) {
         const int64_t r = (int64_t)b * d.T + t;
@@ -247,7 +251,7 @@ template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW
                     rdn[j].load((const T*)d.dn + r * d.C + c, VEC, left);
                 }
                 if (d.dr) rdr[j].load((const T*)d.dr + r * d.C + c, VEC, left);
-                if (gate_rows) rg[j].load((const T*)d.gate + (int64_t)b * d.g_bs + (int64_t)t * d.g_ts + c, VEC, left);
+                if constexpr (gate_rows) rg[j].load((const T*)d.gate + (int64_t)b * d.g_bs + (int64_t)t * d.g_ts + c, VEC, left);
             }
 #pragma unroll
         for (int k = 0; k < 4; ++k) st[k] = (k < 2 ? d.post != 0 : d.dn != nullptr) ? d.stats[k * (int64_t)rows + r] : k & 1;
@@ -255,7 +259,7 @@ template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW
     if (ta + wv < tb) load(ta + wv);
     for (int t = ta + wv; t < tb; t += step) {
         const int64_t r = (int64_t)b * d.T + t;
-        float oh[NCH][8], g[NCH][8], h[NCH][8], v[NCH][8], dR[NCH][8];     // ohat (or o), gate, rhat, scratch, dr then dR
+        float oh[NCH][8], g[gate_rows ? NCH : 1][8], h[NCH][8], v[NCH][8], dR[NCH][8];     // ohat (or o), the row's gate, rhat, scratch, dr then dR
         const float mo = st[0], so = st[1], mr = st[2], sr = st[3];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
@@ -265,10 +269,11 @@ template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW
                 const bool in = row.has(j, k);
                 const float xh = d.dn ? to_f(rx[j].v[k]) : 0.f;
                 oh[j][k] = in ? (to_f(ro[j].v[k]) - mo) * so : 0.f;         // (mo = 0, so = 1 without a norm)
-                g[j][k] = in ? (gate_rows ? to_f(rg[j].v[k]) : ug[j][k]) : 0.f;
+                const float gt = in ? gate_of(j, k) : 0.f;
+                if constexpr (gate_rows) g[j][k] = gt;
                 dR[j][k] = in && d.dr ? to_f(rdr[j].v[k]) : 0.f;
                 const float pp = fmaf(oh[j][k], pc[W + k], pc[2 * W + k]);
-                h[j][k] = in && d.dn ? (fmaf(pc[k] * g[j][k], pp, xh) - mr) * sr : 0.f;
+                h[j][k] = in && d.dn ? (fmaf(pc[k] * gt, pp, xh) - mr) * sr : 0.f;
                 const float dn = in && d.dn ? to_f(rdn[j].v[k]) : 0.f;
                 acc[PLANE_W][j][k] = fmaf(dn, h[j][k], acc[PLANE_W][j][k]);
                 acc[PLANE_B][j][k] += dn;
@@ -300,15 +305,16 @@ template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW
             for (int k = 0; k < 8; ++k) {
                 const float pp = fmaf(oh[j][k], pc[W + k], pc[2 * W + k]), ds = dR[j][k] * pc[k];
                 v[j][k] = ds * pp;                                          // the gate's gradient
-                const float dg = gate_rows ? dR[j][k] * g[j][k] : dR[j][k];        // (a gate per utterance comes in at the end)
+                const float gt = gate_rows ? g[gate_rows ? j : 0][k] : row.has(j, k) ? gate_of(j, k) : 0.f;
+                const float dg = gate_rows ? dR[j][k] * gt : dR[j][k];             // (a gate per utterance comes in at the end)
                 acc[PLANE_E1][j][k] = fmaf(dg, oh[j][k], acc[PLANE_E1][j][k]);
                 acc[PLANE_E0][j][k] += dg;
-                h[j][k] = ds * g[j][k] * pc[W + k];                         // dp pw
+                h[j][k] = ds * gt * pc[W + k];                              // dp pw
                 s1 += h[j][k];
                 s2 = fmaf(h[j][k], oh[j][k], s2);
             }
         }
-        if (gate_rows) row.store((T*)d.dgate + r * d.C, v);
+        if constexpr (gate_rows) row.store((T*)d.dgate + r * d.C, v);
         if (d.post) {
             row_sum2<RW>(s1, s2, red);
             s1 = layer ? s1 * inv : 0.f;
@@ -323,17 +329,20 @@ template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW
     // block totals [4 planes][C], and the utterance gate's gradient behind all blocks' planes.  Its terms per frame are dR scale (pw ohat + pb).
     float* const part = d.ws + (int64_t)blockIdx.x * PLANES * d.C;
     float* const partg = d.ws + (int64_t)gridDim.x * PLANES * d.C + (int64_t)blockIdx.x * d.C;
-    const bool utt = d.gate && !gate_rows;
-    float gd[NCH][8];
+    constexpr bool utt = GATE == GATE_UTT;
+    float gd[utt ? NCH : 1][8];
+    if constexpr (utt)
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-        const float* const pc = &par[0][row.col[j]];
+        for (int j = 0; j < NCH; ++j) {
+            const float* const pc = &par[0][row.col[j]];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            gd[j][k] = pc[k] * fmaf(pc[W + k], acc[PLANE_E1][j][k], pc[2 * W + k] * acc[PLANE_E0][j][k]);
-            if (utt) { acc[PLANE_E1][j][k] *= ug[j][k]; acc[PLANE_E0][j][k] *= ug[j][k]; }
+            for (int k = 0; k < 8; ++k) {
+                const float gt = row.has(j, k) ? gate_of(j, k) : 0.f;
+                gd[j][k] = pc[k] * fmaf(pc[W + k], acc[PLANE_E1][j][k], pc[2 * W + k] * acc[PLANE_E0][j][k]);
+                acc[PLANE_E1][j][k] *= gt;
+                acc[PLANE_E0][j][k] *= gt;
+            }
         }
-    }
     auto emit = [&](float* out, float (&v)[NCH][8]) {
         if constexpr (RW == 1) {
             __syncthreads();
@@ -349,52 +358,57 @@ template <typename T, int RW, int NCH, bool VEC> __global__ __launch_bounds__(RW
     };
 #pragma unroll
     for (int q = 0; q < PLANES; ++q) emit(part + (int64_t)q * d.C, acc[q]);
-    if (utt) emit(partg, gd);
+    if constexpr (utt) emit(partg, gd);
 }
 
-// the blocks' column sums -> the five parameter gradients.  16 columns per block; wave = plane x quarter of the rows, four rows at a time.
-__global__ __launch_bounds__(1024) void rnorm_reduce_kernel(a8_residual_norm_desc d, int blocks) {
+// The blocks' column sums -> the five parameter gradients: the first 2 cdiv(C, 16) blocks, 16 columns and the two planes of one norm each; wave = plane x
+// eighth of the rows, four rows and eight loads at a time.  The blocks behind them add up a gate per utterance's chunks: 1024 elements of dgate [B][C] each.
+template <typename T> __global__ __launch_bounds__(1024) void rnorm_reduce_kernel(a8_residual_norm_desc d, int blocks, int chunks) {
     __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, q = wv & 3;
-    const int c = blockIdx.x * 16 + (lane & 15), cc = min(c, d.C - 1);
-    const int64_t pitch = (int64_t)PLANES * d.C;
-    const float* const in = d.ws + (int64_t)q * d.C + cc;
-    float s[4] = {};
-    int i = (wv >> 2) * 4 + (lane >> 4);
-    for (; i + 48 < blocks; i += 64)
+    const int colblocks = (d.C + 15) / 16 * 2;
+    if ((int)blockIdx.x >= colblocks) {
+        const int64_t i = (int64_t)(blockIdx.x - colblocks) * 1024 + threadIdx.x;
+        if (i >= (int64_t)d.B * d.C) return;
+        const int64_t b = i / d.C, c = i % d.C;
+        const float* const g = d.ws + (int64_t)blocks * PLANES * d.C + b * chunks * d.C + c;
+        float s[8] = {};
+        int k = 0;
+        for (; k + 8 <= chunks; k += 8)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] += in[(i + 16 * k) * pitch];
-    for (; i < blocks; i += 16) s[0] += in[i * pitch];
-    red[wv][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+            for (int j = 0; j < 8; ++j) s[j] += g[(int64_t)(k + j) * d.C];
+        for (; k < chunks; ++k) s[0] += g[(int64_t)k * d.C];
+        ((T*)d.dgate)[i] = from_f<T>(((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])));
+        return;
+    }
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, post = blockIdx.x & 1;
+    const int c = (int)(blockIdx.x >> 1) * 16 + (lane & 15), cc = min(c, d.C - 1);
+    const int64_t pitch = (int64_t)PLANES * d.C;
+    const float* const in = d.ws + (int64_t)(2 * post + (wv & 1)) * d.C + cc;
+    float s[8] = {};
+    int i = (wv >> 1) * 4 + (lane >> 4);
+    for (; i + 224 < blocks; i += 256)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] += in[(i + 32 * k) * pitch];
+    for (; i < blocks; i += 32) s[0] += in[i * pitch];
+    red[wv][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (threadIdx.x < 16 && c < d.C) {
-        float t[PLANES];
+        float t[2] = {};
 #pragma unroll
-        for (int k = 0; k < PLANES; ++k) {
-            t[k] = 0.f;
+        for (int w = 0; w < 16; ++w)
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) t[k] += red[w * 4 + k][g * 16 + lane];
-        }
-        const float sc = d.scale ? d.scale[c] : 1.f, pw = d.post ? d.post_w[c] : 1.f, pb = d.post && d.post_b ? d.post_b[c] : 0.f;
+            for (int g = 0; g < 4; ++g) t[w & 1] += red[w][g * 16 + lane];
         auto put = [&](float* out, int add, float v) { if (out) out[c] = add ? out[c] + v : v; };
-        put(d.dw, d.add_dw, t[PLANE_W]);
-        put(d.db, d.add_db, t[PLANE_B]);
-        put(d.dpost_w, d.add_dpost_w, sc * t[PLANE_E1]);
-        put(d.dpost_b, d.add_dpost_b, sc * t[PLANE_E0]);
-        put(d.dscale, d.add_dscale, fmaf(pw, t[PLANE_E1], pb * t[PLANE_E0]));
+        if (post == 0) {
+            put(d.dw, d.add_dw, t[0]);
+            put(d.db, d.add_db, t[1]);
+        } else {
+            const float sc = d.scale ? d.scale[c] : 1.f, pw = d.post ? d.post_w[c] : 1.f, pb = d.post && d.post_b ? d.post_b[c] : 0.f;
+            put(d.dpost_w, d.add_dpost_w, sc * t[0]);
+            put(d.dpost_b, d.add_dpost_b, sc * t[1]);
+            put(d.dscale, d.add_dscale, fmaf(pw, t[0], pb * t[1]));
+        }
     }
-}
-
-// dgate of a gate per utterance: the sum of the utterance's chunks
-template <typename T> __global__ __launch_bounds__(256) void rnorm_gate_kernel(NormArgs p, const float* part) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)p.d.B * p.d.C) return;
-    const int64_t b = i / p.d.C, c = i % p.d.C;
-    float s = 0.f;
-    for (int k = 0; k < p.chunks; ++k) s += part[(b * p.chunks + k) * p.d.C + c];
-    ((T*)p.d.dgate)[i] = from_f<T>(s);
 }
 
 int norm_check(const a8_residual_norm_desc* d, const char* what) {
@@ -414,18 +428,22 @@ NormArgs norm_args(const a8_residual_norm_desc* d) {
     const void* ptrs[] = {d->x, d->o, d->gate, d->r, d->n, d->post_w, d->post_b, d->w, d->b, d->scale, d->dr, d->dn, d->dx, d->d_o, d->dgate};
     p.vec = d->C % 8 == 0 && d->x_ld % 8 == 0 && d->o_ld % 8 == 0 && (!d->gate || (d->g_bs % 8 == 0 && (!d->gate_rows || d->g_ts % 8 == 0)));
     for (const void* q : ptrs) p.vec = p.vec && aligned16(q);
-    const int per_b = d->B > 0 ? cdiv(512, d->B) : 1;        // about 512 blocks in all, at least 4 rows each
+    const int per_b = d->B > 0 ? cdiv(d->C <= 512 ? 512 : 1024, d->B) : 1;       // about two waves per SIMD in all, at least 4 rows per block
     p.rows_per_chunk = d->T > 0 ? cdiv(d->T, per_b) : 1;
     if (p.rows_per_chunk < 4) p.rows_per_chunk = 4;
     p.chunks = d->T > 0 ? cdiv(d->T, p.rows_per_chunk) : 0;
     return p;
 }
 
-// C <= 1024: a wave per row, four rows side by side; wider: a block per row
-#define NORM_WIDTH(KERNEL, T, ...)                                                                                                \
-    (d->C <= 512 ? (KERNEL<T, 1, 1, ##__VA_ARGS__>) : d->C <= 1024 ? (KERNEL<T, 1, 2, ##__VA_ARGS__>) : d->C <= 2048 ? (KERNEL<T, 4, 1, ##__VA_ARGS__>) \
-     : d->C <= 4096 ? (KERNEL<T, 8, 1, ##__VA_ARGS__>) : (KERNEL<T, 16, 1, ##__VA_ARGS__>))
-int norm_threads(const a8_residual_norm_desc* d) { return d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024; }
+// Forward: a wave per row up to 1024 channels (four rows side by side), a block per row beyond.  Backward: two waves per row from 513 on (a lane with 16
+// channels takes over 250 registers: 32 x 1499 x 1024 with a block count that fits each, 166 us, two waves 153 .. 169, and 8 x 781 x 768 39 us against 29).
+#define NORM_WIDE(KERNEL, T, ...)                                                                                                 \
+    (d->C <= 2048 ? (KERNEL<T, 4, 1, ##__VA_ARGS__>) : d->C <= 4096 ? (KERNEL<T, 8, 1, ##__VA_ARGS__>) : (KERNEL<T, 16, 1, ##__VA_ARGS__>))
+#define NORM_FWD(T) (d->C <= 512 ? (rnorm_fwd_kernel<T, 1, 1>) : d->C <= 1024 ? (rnorm_fwd_kernel<T, 1, 2>) : NORM_WIDE(rnorm_fwd_kernel, T))
+#define NORM_BWD(T, VEC, GATE)                                                                                                    \
+    (d->C <= 512 ? (rnorm_bwd_kernel<T, 1, 1, VEC, GATE>) : d->C <= 1024 ? (rnorm_bwd_kernel<T, 2, 1, VEC, GATE>) : NORM_WIDE(rnorm_bwd_kernel, T, VEC, GATE))
+#define NORM_GATE(T, VEC) (!d->gate ? NORM_BWD(T, VEC, GATE_NONE) : d->gate_rows ? NORM_BWD(T, VEC, GATE_ROWS) : NORM_BWD(T, VEC, GATE_UTT))
+int wide_threads(const a8_residual_norm_desc* d) { return d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024; }
 
 }  // namespace
 
@@ -435,8 +453,8 @@ extern "C" int a8_residual_norm_fwd(const a8_residual_norm_desc* d, void* stream
     A8_REQUIRE(d->x && d->o && d->r && (d->w || !d->n), "a8_residual_norm_fwd: null x, o, r or weight");
     const NormArgs p = norm_args(d);
     const int rows = d->B * d->T;
-    auto kernel = d->dtype == A8_BF16 ? NORM_WIDTH(rnorm_fwd_kernel, bf16) : NORM_WIDTH(rnorm_fwd_kernel, float);
-    hipLaunchKernelGGL(kernel, dim3(d->C <= 1024 ? cdiv(rows, 4) : rows), dim3(norm_threads(d)), 0, (hipStream_t)stream, p);
+    auto kernel = d->dtype == A8_BF16 ? NORM_FWD(bf16) : NORM_FWD(float);
+    hipLaunchKernelGGL(kernel, dim3(d->C <= 1024 ? cdiv(rows, 4) : rows), dim3(wide_threads(d)), 0, (hipStream_t)stream, p);
     return a8_check_launch("a8_residual_norm_fwd");
 }
 
@@ -454,18 +472,13 @@ extern "C" int a8_residual_norm_bwd(const a8_residual_norm_desc* d, void* stream
     if (blocks > 0) {
         A8_REQUIRE(d->x && d->o && d->dx && d->d_o && d->ws && (d->dgate || !d->gate) && (d->stats || !(d->post || d->dn)) && (d->w || !d->dn),
                    "a8_residual_norm_bwd: null operand");
-        auto kernel = d->dtype == A8_BF16 ? (p.vec ? NORM_WIDTH(rnorm_bwd_kernel, bf16, true) : NORM_WIDTH(rnorm_bwd_kernel, bf16, false))
-                                          : (p.vec ? NORM_WIDTH(rnorm_bwd_kernel, float, true) : NORM_WIDTH(rnorm_bwd_kernel, float, false));
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(norm_threads(d)), 0, (hipStream_t)stream, p);
+        auto kernel = d->dtype == A8_BF16 ? (p.vec ? NORM_GATE(bf16, true) : NORM_GATE(bf16, false)) : (p.vec ? NORM_GATE(float, true) : NORM_GATE(float, false));
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(d->C <= 512 ? 256 : d->C <= 1024 ? 128 : wide_threads(d)), 0, (hipStream_t)stream, p);
         if (int e = a8_check_launch("a8_residual_norm_bwd")) return e;
     }
-    if (d->gate && !d->gate_rows && d->B > 0) {
-        const dim3 grid((unsigned)(((int64_t)d->B * d->C + 255) / 256));
-        const float* part = d->ws + (int64_t)blocks * PLANES * d->C;
-        if (d->dtype == A8_BF16) hipLaunchKernelGGL((rnorm_gate_kernel<bf16>), grid, dim3(256), 0, (hipStream_t)stream, p, part);
-        else hipLaunchKernelGGL((rnorm_gate_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, p, part);
-        if (int e = a8_check_launch("a8_residual_norm_bwd")) return e;
-    }
-    hipLaunchKernelGGL(rnorm_reduce_kernel, dim3(cdiv(d->C, 16)), dim3(1024), 0, (hipStream_t)stream, *d, blocks);
+    const int gate_blocks = d->gate && !d->gate_rows ? cdiv((int64_t)d->B * d->C, 1024) : 0;
+    const dim3 grid(2 * cdiv(d->C, 16) + gate_blocks);
+    if (d->dtype == A8_BF16) hipLaunchKernelGGL(rnorm_reduce_kernel<bf16>, grid, dim3(1024), 0, (hipStream_t)stream, *d, blocks, p.chunks);
+    else hipLaunchKernelGGL(rnorm_reduce_kernel<float>, grid, dim3(1024), 0, (hipStream_t)stream, *d, blocks, p.chunks);
     return a8_check_launch("a8_residual_norm_bwd");
 }

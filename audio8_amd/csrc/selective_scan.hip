@@ -488,30 +488,57 @@ template <typename T> __global__ __launch_bounds__(256) void scan_bc_kernel(Scan
     ((T*)d.dCm)[i] = from_f<T>(sc);
 }
 
-// One frame: 4 lanes per channel, 4 consecutive states per lane and round; the state is read and written once.
+// One frame: 4 lanes per channel, 4 consecutive states per lane and round; the state is read and written once.  What a launch of one frame costs is
+// latency, so every load is issued before the first use.  VEC: N % 4 = 0 and 16-byte aligned A and state.
 template <typename T> A8_DEV float ldf(const void* p, int64_t i) { return to_f(((const T*)p)[i]); }
-template <typename T> __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p) {
+template <typename T, bool VEC> __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p) {
     const a8_selective_scan_desc& d = p.d;
     const int b = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x >> 2), s4 = threadIdx.x & 3;
     const int ch = min(c, d.D - 1), g = ch / p.cpg;
-    const float raw = ldf<T>(d.dt, b * d.dt_bs + ch) + (d.dt_bias ? d.dt_bias[ch] : 0.f);
-    const float u = ldf<T>(d.u, b * d.u_bs + ch), D = d.softplus ? softplus_f(raw) : raw, x = D * u;
     float* const st = d.h_out + ((int64_t)b * d.D + ch) * d.N;
     const float* const A = d.A + (int64_t)ch * d.N;
-    float y = 0.f;
-    for (int n = s4 * 4; n < d.N; n += 16)
+    const T* const Bp = (const T*)d.Bm + (b * d.b_bs + g * d.b_gs);
+    const T* const Cp = (const T*)d.Cm + (b * d.c_bs + g * d.c_gs);
+    const T rdt = ((const T*)d.dt)[b * d.dt_bs + ch], ru = ((const T*)d.u)[b * d.u_bs + ch];
+    const T rz = d.z ? ((const T*)d.z)[b * d.z_bs + ch] : from_f<T>(0.f);
+    const float bias = d.dt_bias ? d.dt_bias[ch] : 0.f, skip = d.Dskip ? d.Dskip[ch] : 0.f;
+    float y = 0.f, D = 0.f, x = 0.f;
+    for (int n = s4 * 4; n < d.N; n += 16) {
+        float h[4], a[4], Bv[4], Cv[4];
+        if constexpr (VEC) {
+            const f32x4 hv = *reinterpret_cast<const f32x4*>(st + n), av = *reinterpret_cast<const f32x4*>(A + n);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (n + k < d.N) {
-                const float h = fmaf(exp_fast(D * A[n + k]), st[n + k], x * ldf<T>(d.Bm, b * d.b_bs + g * d.b_gs + n + k));
-                y = fmaf(ldf<T>(d.Cm, b * d.c_bs + g * d.c_gs + n + k), h, y);
-                if (c < d.D) st[n + k] = h;
+            for (int k = 0; k < 4; ++k) { h[k] = hv[k]; a[k] = av[k]; Bv[k] = to_f(Bp[n + k]); Cv[k] = to_f(Cp[n + k]); }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int m = min(n + k, d.N - 1);
+                h[k] = st[m]; a[k] = A[m]; Bv[k] = to_f(Bp[m]); Cv[k] = n + k < d.N ? to_f(Cp[m]) : 0.f;
             }
+        }
+        if (n < 16) {                                      // (the first round; behind the loads)
+            const float raw = to_f(rdt) + bias;
+            D = d.softplus ? softplus_f(raw) : raw;
+            x = D * to_f(ru);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            h[k] = fmaf(exp_fast(D * a[k]), h[k], x * Bv[k]);
+            y = fmaf(Cv[k], VEC || n + k < d.N ? h[k] : 0.f, y);
+        }
+        if (c < d.D) {
+            if constexpr (VEC) *reinterpret_cast<f32x4*>(st + n) = (f32x4){h[0], h[1], h[2], h[3]};
+            else
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (n + k < d.N) st[n + k] = h[k];
+        }
+    }
     y += dpp_f<0xB1>(y);
     y += dpp_f<0x4E>(y);
     if (s4 == 0 && c < d.D) {
-        if (d.Dskip) y = fmaf(d.Dskip[ch], u, y);
-        if (d.z) y *= silu_f(ldf<T>(d.z, b * d.z_bs + ch));
+        y = fmaf(skip, to_f(ru), y);
+        if (d.z) y *= silu_f(to_f(rz));
         ((T*)d.y)[(int64_t)b * d.D + ch] = from_f<T>(y);
     }
 }
@@ -655,7 +682,9 @@ extern "C" int a8_selective_scan_step(const a8_selective_scan_desc* d, void* str
     A8_REQUIRE(d->u && d->dt && d->Bm && d->Cm && d->y && d->h_out, "a8_selective_scan_step: null u, dt, B, C, y or state");
     const ScanArgs p = scan_args(d, false);
     const dim3 grid(cdiv(d->D, 64), d->B);
-    if (d->dtype == A8_BF16) hipLaunchKernelGGL((scan_step_kernel<bf16>), grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL((scan_step_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, p);
+    const bool vec = d->N % 4 == 0 && ((uintptr_t)d->A | (uintptr_t)d->h_out) % 16 == 0;
+    auto kernel = d->dtype == A8_BF16 ? (vec ? scan_step_kernel<bf16, true> : scan_step_kernel<bf16, false>)
+                                      : (vec ? scan_step_kernel<float, true> : scan_step_kernel<float, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, p);
     return a8_check_launch("a8_selective_scan_step");
 }
