@@ -334,6 +334,7 @@ extern "C" int a8_causal_conv_step(const a8_causal_conv_desc* d, void* stream) {
     if (int e = conv_check(d, "a8_causal_conv_step")) return e;
     A8_REQUIRE(d->T == 1, "a8_causal_conv_step: one frame at a time (T = %d)", d->T);
     if (d->B == 0) return A8_OK;
+    A8_REQUIRE((int64_t)d->B * d->C < (1 << 30), "a8_causal_conv_step: B x C = %d x %d is too large", d->B, d->C);
     A8_REQUIRE(d->x && d->y && d->state_out, "a8_causal_conv_step: null x, y or state");
     auto kernel = d->dtype == A8_BF16 ? (d->K == 2 ? conv_step_kernel<bf16, 2> : d->K == 3 ? conv_step_kernel<bf16, 3> : conv_step_kernel<bf16, 4>)
                                       : (d->K == 2 ? conv_step_kernel<float, 2> : d->K == 3 ? conv_step_kernel<float, 3> : conv_step_kernel<float, 4>);

@@ -415,7 +415,8 @@ int norm_check(const a8_residual_norm_desc* d, const char* what) {
     A8_REQUIRE(d != nullptr && d->size == (int)sizeof(a8_residual_norm_desc), "%s: descriptor size %d, expected %d", what, d ? d->size : 0, (int)sizeof(a8_residual_norm_desc));
     A8_REQUIRE(d->dtype == A8_F32 || d->dtype == A8_BF16, "%s: bad dtype %d", what, d->dtype);
     A8_REQUIRE(d->B >= 0 && d->T >= 0 && d->C >= 1 && d->C <= 8192, "%s: bad sizes B=%d T=%d C=%d (1 to 8192 channels)", what, d->B, d->T, d->C);
-    A8_REQUIRE((int64_t)d->B * d->T < (1 << 30), "%s: B x T = %d x %d is too large", what, d->B, d->T);
+    const int row_threads = d->C <= 1024 ? 64 : d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024;       // (forward; a grid holds less than 2^32 threads)
+    A8_REQUIRE(((int64_t)d->B * d->T + 4) * row_threads < (1ll << 32) && (int64_t)d->B * d->T < (1 << 30), "%s: B x T = %d x %d is too large", what, d->B, d->T);
     A8_REQUIRE(d->kind == A8_NORM_LAYER || d->kind == A8_NORM_RMS, "%s: unknown kind %d", what, d->kind);
     A8_REQUIRE(!d->post || d->post_w, "%s: null post weight", what);
     return A8_OK;
@@ -425,7 +426,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 NormArgs norm_args(const a8_residual_norm_desc* d) {
     NormArgs p = {};
     p.d = *d;
-    const void* ptrs[] = {d->x, d->o, d->gate, d->r, d->n, d->post_w, d->post_b, d->w, d->b, d->scale, d->dr, d->dn, d->dx, d->d_o, d->dgate};
+    const void* ptrs[] = {d->x, d->o, d->gate, d->r, d->n, d->post_w, d->post_b, d->w, d->b, d->scale, d->dr, d->dn, d->dx, d->d_o, d->dgate, d->ws};
     p.vec = d->C % 8 == 0 && d->x_ld % 8 == 0 && d->o_ld % 8 == 0 && (!d->gate || (d->g_bs % 8 == 0 && (!d->gate_rows || d->g_ts % 8 == 0)));
     for (const void* q : ptrs) p.vec = p.vec && aligned16(q);
     const int per_b = d->B > 0 ? cdiv(d->C <= 512 ? 512 : 1024, d->B) : 1;       // about two waves per SIMD in all, at least 4 rows per block
@@ -476,6 +477,7 @@ extern "C" int a8_residual_norm_bwd(const a8_residual_norm_desc* d, void* stream
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(d->C <= 512 ? 256 : d->C <= 1024 ? 128 : wide_threads(d)), 0, (hipStream_t)stream, p);
         if (int e = a8_check_launch("a8_residual_norm_bwd")) return e;
     }
+    A8_REQUIRE((int64_t)d->B * d->C < (1 << 30), "a8_residual_norm_bwd: B x C = %d x %d is too large", d->B, d->C);
     const int gate_blocks = d->gate && !d->gate_rows ? cdiv((int64_t)d->B * d->C, 1024) : 0;
     const dim3 grid(2 * cdiv(d->C, 16) + gate_blocks);
     if (d->dtype == A8_BF16) hipLaunchKernelGGL(rnorm_reduce_kernel<bf16>, grid, dim3(1024), 0, (hipStream_t)stream, *d, blocks, p.chunks);

@@ -654,6 +654,8 @@ extern "C" int a8_selective_scan_bwd(const a8_selective_scan_desc* d, void* stre
     A8_REQUIRE(d->B == 0 || d->T == 0 || (d->u && d->dt && d->Bm && d->Cm && d->dy && d->ckpt && d->du && d->ddt && d->dBm && d->dCm && (d->dz || !d->z)),
                "a8_selective_scan_bwd: null operand");
     A8_REQUIRE(scan_blocks(p, p.chunks) < (1 << 21), "a8_selective_scan_bwd: B x D = %d x %d is too large", d->B, d->D);
+    const int64_t total = (int64_t)d->B * d->T * d->G * d->N;
+    A8_REQUIRE(total < (1ll << 32) - 256, "a8_selective_scan_bwd: B x T x G x N = %d x %d x %d x %d is too large", d->B, d->T, d->G, d->N);
     p.ends = d->ws;
     p.part = p.ends + ends_floats(p);
     p.part_b = p.part + (int64_t)d->B * p.chunks * (d->N + 2) * d->D;
@@ -662,7 +664,6 @@ extern "C" int a8_selective_scan_bwd(const a8_selective_scan_desc* d, void* stre
         if (p.chunks > 1)
             if (int e = launch_bwd(p, true, (hipStream_t)stream)) return e;
         if (int e = launch_bwd(p, false, (hipStream_t)stream)) return e;
-        const int64_t total = (int64_t)d->B * d->T * d->G * d->N;
         if (total > 0) {
             const dim3 grid((unsigned)((total + 255) / 256));
             if (d->dtype == A8_BF16) hipLaunchKernelGGL((scan_bc_kernel<bf16>), grid, dim3(256), 0, (hipStream_t)stream, p);

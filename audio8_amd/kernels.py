@@ -4,6 +4,7 @@ Tensors are torch CUDA tensors used only as device-memory handles; every wrapper
 torch's current HIP stream.  All arithmetic happens inside liba8hip.so.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -464,11 +465,11 @@ def causal_conv_fwd(x, w, bias=None, act="silu", state=None, lengths=None, want_
     return y, out, d
 
 
-_size = C.c_int64
-
-
-def _conv_partials(d):
-    n = _size()
+# Workspace sizes are functions of a call's sizes alone.
+@functools.lru_cache(maxsize=1024)
+def _conv_partials(B, T, Cn, Kn):
+    d, n = L.CausalConvDesc(L.CONV_DESC_SIZE, L.F32, B, T, Cn, Kn, 0), C.c_int64()
+    d.w = 1                                  # (a size needs no data; the entry point checks that there is some)
     L.check(L.lib().a8_causal_conv_bwd_partial_floats(C.byref(d), C.byref(n)), "a8_causal_conv_bwd_partial_floats")
     return n.value
 
@@ -481,12 +482,13 @@ def causal_conv_bwd(dy, x, w, bias=None, act="silu", state=None, lengths=None, d
         d = L.CausalConvDesc.from_buffer_copy(desc)
     else:
         d = _conv_desc(x, w, bias, act, state, lengths, "causal_conv_bwd")
+        _seq_stream(w, bias, state, lengths)
     dtype = x.dtype
     _act("dy", dy, x.shape, dtype)
     _dense("dstate_out", dstate_out, (d.B, d.K - 1, d.C), dtype)
     _dense("dw", dw, w.shape)
     _dense("dbias", dbias, (d.C,))
-    stream = _seq_stream(dy, x, w, bias, state, lengths, dstate_out, dw, dbias)
+    stream = _seq_stream(dy, x, dstate_out, dw, dbias)
     dx = x.new_empty(x.shape)
     d.y = d.state_out = dstate = None
     if want_dstate and d.T == 0:             # no frame: the history is handed on
@@ -494,7 +496,7 @@ def causal_conv_bwd(dy, x, w, bias=None, act="silu", state=None, lengths=None, d
     elif want_dstate:
         dstate = x.new_empty((d.B, d.K - 1, d.C))
         d.dstate = dstate.data_ptr()
-    part = torch.empty(_conv_partials(d), device=x.device)
+    part = torch.empty(_conv_partials(d.B, d.T, d.C, d.K), device=x.device, dtype=torch.float32)
     d.dy, (d.dy_bs, d.dy_ts, _) = dy.data_ptr(), dy.stride()
     d.dstate_out, d.dx, d.dw, d.dbias = L.ptr(dstate_out), dx.data_ptr(), L.ptr(dw), L.ptr(dbias)
     d.add_dw, d.add_dbias = add
@@ -553,8 +555,10 @@ def _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, what):
                                B.data_ptr(), b0, b1, b2, Cm.data_ptr(), c0, c1, c2, A.data_ptr(), L.ptr(D), L.ptr(dt_bias), L.ptr(state), L.ptr(lengths))
 
 
-def _scan_sizes(d, backward):
-    ck, ws = _size(), _size()
+@functools.lru_cache(maxsize=1024)
+def _scan_sizes(B, T, Dn, N, G, backward):
+    d, ck, ws = L.SelectiveScanDesc(L.SCAN_DESC_SIZE, L.F32, B, T, Dn, N, G, 1), C.c_int64(), C.c_int64()
+    d.A = 1
     L.check(L.lib().a8_selective_scan_workspace(C.byref(d), backward, C.byref(ck), C.byref(ws)), "a8_selective_scan_workspace")
     return ck.value, ws.value
 
@@ -564,19 +568,19 @@ def selective_scan_fwd(u, dt, A, B, Cm, D=None, z=None, dt_bias=None, softplus=T
     -> (y [B,T,D], final state f32 [B,D,N] or None, states saved for selective_scan_bwd or None, descriptor)."""
     d = _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, "selective_scan_fwd")
     stream = _seq_stream(u, dt, A, B, Cm, D, z, dt_bias, state, lengths)
-    nck, nws = _scan_sizes(d, 0)
+    nck, nws = _scan_sizes(d.B, d.T, d.D, d.N, d.G, 0)
     dev = u.device
     y = u.new_empty(u.shape)
     d.y = y.data_ptr()
     out = ckpt = None
     if want_state:
-        out = torch.empty((d.B, d.D, d.N), device=dev)
+        out = torch.empty((d.B, d.D, d.N), device=dev, dtype=torch.float32)
         d.h_out = out.data_ptr()
     if want_ckpt:
-        ckpt = torch.empty(nck, device=dev)
+        ckpt = torch.empty(nck, device=dev, dtype=torch.float32)
         d.ckpt = ckpt.data_ptr()
     if nws:
-        ws = torch.empty(nws, device=dev)
+        ws = torch.empty(nws, device=dev, dtype=torch.float32)
         d.ws = ws.data_ptr()
     L.check(L.lib().a8_selective_scan_fwd(C.byref(d), stream), "a8_selective_scan_fwd")
     return y, out, ckpt, d
@@ -593,14 +597,15 @@ def selective_scan_bwd(dy, ckpt, u, dt, A, B, Cm, D=None, z=None, dt_bias=None, 
         d = L.SelectiveScanDesc.from_buffer_copy(desc)
     else:
         d = _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, "selective_scan_bwd")
+        _seq_stream(dt, A, B, Cm, D, z, dt_bias, state, lengths)
     us, dtype = u.shape, u.dtype
     _act("dy", dy, us, dtype)
     _dense("dstate_out", dstate_out, (d.B, d.D, d.N))
     _dense("dA", dA, A.shape)
     _dense("dD", dD, (d.D,))
     _dense("ddt_bias", ddt_bias, (d.D,))
-    stream = _seq_stream(dy, ckpt, u, dt, A, B, Cm, D, z, dt_bias, state, lengths, dstate_out, dA, dD, ddt_bias)
-    nck, nws = _scan_sizes(d, 1)
+    stream = _seq_stream(dy, ckpt, u, dstate_out, dA, dD, ddt_bias)
+    nck, nws = _scan_sizes(d.B, d.T, d.D, d.N, d.G, 1)
     _dense("ckpt", ckpt, (nck,))
     dev = u.device
     if z is not None:
@@ -608,8 +613,8 @@ def selective_scan_bwd(dy, ckpt, u, dt, A, B, Cm, D=None, z=None, dt_bias=None, 
     else:
         (du, ddt), dz = u.new_empty((2, *us)).unbind(0), None
     dB, dC = u.new_empty((2, *B.shape)).unbind(0)
-    dstate = torch.empty((d.B, d.D, d.N), device=dev) if want_dstate else None
-    ws = torch.empty(nws, device=dev)
+    dstate = torch.empty((d.B, d.D, d.N), device=dev, dtype=torch.float32) if want_dstate else None
+    ws = torch.empty(nws, device=dev, dtype=torch.float32)
     d.y = d.h_out = None
     d.ckpt, d.ws = ckpt.data_ptr(), ws.data_ptr()
     d.dy, (d.dy_bs, d.dy_ts, _), d.dh_out = dy.data_ptr(), dy.stride(), P(dstate_out)
@@ -678,6 +683,13 @@ def _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, what):
                               x.data_ptr(), _rows_ld("x", x), o.data_ptr(), _rows_ld("o", o), P(gate), g0, g1, P(scale), P(w), P(b), P(post_w), P(post_b))
 
 
+@functools.lru_cache(maxsize=1024)
+def _rnorm_floats(B, T, Cn):
+    d, n = L.ResidualNormDesc(L.RNORM_DESC_SIZE, L.F32, B, T, Cn), C.c_int64()
+    L.check(L.lib().a8_residual_norm_bwd_workspace(C.byref(d), C.byref(n)), "a8_residual_norm_bwd_workspace")
+    return n.value
+
+
 def residual_norm_fwd(x, o, w=None, b=None, post_w=None, post_b=None, gate=None, scale=None, eps=1e-6, kind="layer", want_stats=False):
     """x, o [B,T,C]; gate [B,T,C] or [B,1,C]; norm parameters and scale f32 [C]
     -> (r, n or None when w is None, stats f32 [4, B*T] or None, descriptor)."""
@@ -690,7 +702,7 @@ def residual_norm_fwd(x, o, w=None, b=None, post_w=None, post_b=None, gate=None,
     r = x.new_empty(x.shape)
     d.r = r.data_ptr()
     if want_stats:
-        stats = torch.empty((4, d.B * d.T), device=x.device)
+        stats = torch.empty((4, d.B * d.T), device=x.device, dtype=torch.float32)
         d.stats = stats.data_ptr()
     L.check(L.lib().a8_residual_norm_fwd(C.byref(d), stream), "a8_residual_norm_fwd")
     return r, n, stats, d
@@ -706,6 +718,7 @@ def residual_norm_bwd(dr, dn, stats, x, o, w=None, b=None, post_w=None, post_b=N
         d = L.ResidualNormDesc.from_buffer_copy(desc)
     else:
         d = _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, "residual_norm_bwd")
+        _seq_stream(o, w, b, post_w, post_b, gate, scale)
     xs, dtype, col = x.shape, x.dtype, (d.C,)
     _dense("dr", dr, xs, dtype)
     _dense("dn", dn, xs, dtype)
@@ -717,7 +730,7 @@ def residual_norm_bwd(dr, dn, stats, x, o, w=None, b=None, post_w=None, post_b=N
     _dense("dscale", dscale, col)
     if dn is not None and w is None:
         raise ValueError("a8hip residual_norm_bwd: dn without the second norm's weight")
-    stream = _seq_stream(dr, dn, stats, x, o, w, b, post_w, post_b, gate, scale, dw, db, dpost_w, dpost_b, dscale)
+    stream = _seq_stream(dr, dn, stats, x, dw, db, dpost_w, dpost_b, dscale)
     dx, do = x.new_empty((2, *xs)).unbind(0)
     dgate = x.new_empty(gate.shape) if gate is not None else None
     d.r = d.n = None
@@ -725,9 +738,7 @@ def residual_norm_bwd(dr, dn, stats, x, o, w=None, b=None, post_w=None, post_b=N
         P(dr), P(dn), dx.data_ptr(), do.data_ptr(), P(dgate), P(dw), P(db), P(dpost_w), P(dpost_b), P(dscale)
     d.stats = stats.data_ptr()
     d.add_dw, d.add_db, d.add_dpost_w, d.add_dpost_b, d.add_dscale = add
-    n = _size()
-    L.check(L.lib().a8_residual_norm_bwd_workspace(C.byref(d), C.byref(n)), "a8_residual_norm_bwd_workspace")
-    ws = torch.empty(n.value, device=x.device)
+    ws = torch.empty(_rnorm_floats(d.B, d.T, d.C), device=x.device, dtype=torch.float32)
     d.ws = ws.data_ptr()
     L.check(L.lib().a8_residual_norm_bwd(C.byref(d), stream), "a8_residual_norm_bwd")
     return dx, do, dgate

@@ -495,13 +495,16 @@ def _param_grads(ctx, params):
     """Targets of the parameter gradients, per parameter (position in the forward's arguments, tensor): p.grad when gradients go there
     directly, a fresh tensor otherwise, None when not needed.  -> (targets, add flags, gradients to return)."""
     needs = ctx.needs_input_grad
-    tgts = [_target(p) if DIRECT_GRADS and p is not None and p.is_leaf and needs[at] else None for at, p in params]
+    tgts = [None] * len(params)
+    if DIRECT_GRADS:
+        once = [sum(p is q for _, q in params) == 1 for _, p in params]        # (one tensor in two places: two blocks would add to the same target)
+        tgts = [_target(p) if p is not None and p.is_leaf and needs[at] and o else None for (at, p), o in zip(params, once)]
     fresh = [i for i, (at, p) in enumerate(params) if p is not None and needs[at] and tgts[i] is None]
     add = [t is not None for t in tgts]
     ret = [None] * len(params)
     like = params[fresh[0]][1] if fresh else None
     if len(fresh) > 2 and all(params[i][1].shape == like.shape for i in fresh):
-        slab = torch.empty((len(fresh), *like.shape), device=like.device).unbind(0)          # one allocation for a norm's handful of columns
+        slab = torch.empty((len(fresh), *like.shape), device=like.device, dtype=torch.float32).unbind(0)          # one allocation for a norm's handful of columns
     else:
         slab = [torch.empty_like(params[i][1]) for i in fresh]
     for i, g in zip(fresh, slab):

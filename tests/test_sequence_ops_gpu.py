@@ -576,3 +576,72 @@ def test_a_graph_walked_twice_gives_the_same_gradients():
     first, second = (torch.autograd.grad([r, n], [x, w, A, bc], [r.detach(), n.detach()], retain_graph=True) for _ in range(2))
     for p, q in zip(first, second):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+def test_workspaces_do_not_follow_the_default_dtype(default):
+    from audio8_amd import ops
+    v = _train_inputs(5)
+    want = _train(ops, v)
+    was = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        got = _train(ops, v)
+        h = ops.selective_scan(v["x"], v["dt"], v["A"], v["B"], v["C"], return_state=True)[1]
+    finally:
+        torch.set_default_dtype(was)
+    assert h.dtype == torch.float32
+    for p, q in zip(got, want):
+        assert p.dtype == q.dtype and torch.equal(p, q)
+
+
+def test_one_parameter_in_two_places_of_a_call():
+    """Direct gradients would have two blocks add to one target: such a parameter's gradients come back through the tape instead."""
+    import audio8_amd.ops as ops
+    x, o, up = rnd(2, 20, 64, seed=1).cuda(), cu(rnd(2, 20, 64, seed=2), True), rnd(2, 20, 64, seed=3).cuda()
+    w = torch.nn.Parameter(rnd(64, seed=4).cuda())
+
+    def loss():
+        r, n = ops.gated_residual_norm(x, o, w, post_weight=w, scale=w)
+        return (r * up).sum() + (n * up).sum()
+    (want,) = torch.autograd.grad(loss(), [w])
+    w.grad = torch.zeros_like(w)
+    was = ops.DIRECT_GRADS
+    ops.DIRECT_GRADS = True
+    try:
+        loss().backward()
+    finally:
+        ops.DIRECT_GRADS = was
+    assert torch.allclose(w.grad, want, rtol=2.0 ** -21, atol=2.0 ** -21 * float(want.abs().max()))
+
+
+def test_steps_in_inference_mode():
+    from audio8_amd import ops
+    with torch.inference_mode():
+        x, w = rnd(2, 8, seed=1).cuda(), rnd(8, 4, seed=2).cuda()
+        c, h = torch.zeros(2, 3, 8, device="cuda"), torch.zeros(2, 8, 4, device="cuda")
+        bc = rnd(2, 4, seed=3).cuda()
+        y = ops.selective_scan_step(ops.causal_conv_step(x, c, w), x, -torch.ones(8, 4, device="cuda"), bc, bc, h)
+    assert torch.isfinite(y).all() and c.any() and h.any()
+
+
+def test_offsets_past_32_bits():
+    """One recording of 1.1 million frames x 2048 channels: 2.25e9 elements.  Its last frames come out as those frames do on their own."""
+    from audio8_amd import ops
+    T, C, K, tail = 1_100_000, 2048, 4, 80
+    x = torch.zeros(1, T, C, device="cuda", dtype=torch.bfloat16)
+    x[:, -tail:] = rnd(1, tail, C, seed=1, dtype=torch.bfloat16).cuda()
+    x.requires_grad_()
+    short = x.detach()[:, -tail:].clone().requires_grad_()
+    w, A, g = rnd(C, K, seed=2).cuda(), -rnd(C, 4, seed=3).exp().cuda(), rnd(C, seed=4).cuda()
+    bc, bs = torch.zeros(1, T, 4, device="cuda", dtype=torch.bfloat16), rnd(1, tail, 4, seed=5, dtype=torch.bfloat16).cuda()
+    bc[:, -tail:] = bs
+    for f in (lambda v, b: ops.causal_conv(v, w), lambda v, b: ops.selective_scan(v, v, A, b, b), lambda v, b: ops.gated_residual_norm(v, v, g, post_weight=g, gate=v)[1]):
+        y, ys = f(x, bc), f(short, bs)
+        assert torch.equal(y[:, -tail:], ys)
+        up = torch.zeros_like(y)
+        up[:, -tail:] = 1
+        (dx,), (ds,) = torch.autograd.grad(y, [x], [up]), torch.autograd.grad(ys, [short], [torch.ones_like(ys)])
+        # frames before the tail see the tail's gradient through the recurrence and the taps, not the other way round; the scan's frame chunks differ
+        assert torch.allclose(dx[:, -tail:].float(), ds.float(), rtol=2.0 ** -7, atol=2.0 ** -14 * float(ds.abs().max()))
+        del y, up, dx
