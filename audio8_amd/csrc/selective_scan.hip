@@ -85,12 +85,12 @@ template <typename T, int NW, int NS, bool Z, bool DY> struct TileRegs {
         b = ((const T*)d.Bm)[w.b * d.b_bs + t * d.b_ts + w.g * d.b_gs + n];
         c = ((const T*)d.Cm)[w.b * d.c_bs + t * d.c_ts + w.g * d.c_gs + n];
     }
-    A8_DEV void stage_bc(const a8_selective_scan_desc& d, const Where& w, int t0, float* s_b, float* s_c) const {       // -> LDS [TT][BC]
+    template <bool B = true, bool C = true> A8_DEV void stage_bc(const a8_selective_scan_desc& d, const Where& w, int t0, float* s_b, float* s_c) const {       // -> LDS [TT][BC]
         const int tid = threadIdx.x;
         if (TT * BC == 64 * NW || tid < TT * BC) {
             const bool in = tid % BC < d.N && t0 + tid / BC < w.len;
-            s_b[tid] = in ? to_f(b) : 0.f;
-            s_c[tid] = in ? to_f(c) : 0.f;
+            if constexpr (B) s_b[tid] = in ? to_f(b) : 0.f;
+            if constexpr (C) s_c[tid] = in ? to_f(c) : 0.f;
         }
     }
 };
@@ -133,32 +133,30 @@ template <int I> A8_DEV void row_axpy(float (&x)[4], float v, float g) {
 // element (t, n) of wave_bc's values
 template <int NS, int T_, int N_> A8_DEV float bc_at(const float (&v)[NS]) { return row_value<(T_ % (16 / NS)) * NS + N_>(v[T_ / (16 / NS)]); }
 
-// ENDS: only each chunk's own end state (from zero) and the sum of its steps; else the chunk itself, from the state that the chunks before it leave.
-template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs p) {
+template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs p) {
     constexpr int NS = FNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dx[TT][CH];                        // {D, D u}
     __shared__ float s_b[TT * BC], s_c[TT * BC];
-    __shared__ float s_y[ENDS ? 1 : NW][TT][CH];
+    __shared__ float s_y[NW][TT][CH];
     const a8_selective_scan_desc& d = p.d;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = wv * NS;
-    const Where w = locate(p, lane, 0, ENDS ? p.chunks - 1 : p.chunks);
+    const Where w = locate(p, lane, 0, p.chunks);
     const float bias = d.dt_bias ? d.dt_bias[w.ch] : 0.f, skip = d.Dskip ? d.Dskip[w.ch] : 0.f;
     const bool sp = d.softplus != 0;
-    float A2[NS], h[NS], sum = 0.f;
+    float A2[NS], h[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const bool has = n0 + n < d.N;
         A2[n] = has ? d.A[(int64_t)w.ch * d.N + n0 + n] * SEQ_LOG2E : 0.f;
-        h[n] = !ENDS && has && d.h0 ? d.h0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
+        h[n] = has && d.h0 ? d.h0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
     }
-    if constexpr (!ENDS)
-        for (int k = 0; k < w.ck; ++k) {                   // the states that the chunks before leave: at most a few dozen, each two loads away
-            const float* const e = p.ends + ((int64_t)w.b * p.chunks + k) * (d.N + 1) * d.D + w.ch;
-            const float s = e[(int64_t)d.N * d.D];
+    for (int k = 0; k < w.ck; ++k) {                       // the states that the chunks before leave: at most a few dozen, each two loads away
+        const float* const e = p.ends + ((int64_t)w.b * p.chunks + k) * (d.N + 1) * d.D + w.ch;
+        const float s = e[(int64_t)d.N * d.D];
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-                if (n0 + n < d.N) h[n] = fmaf(__builtin_amdgcn_exp2f(A2[n] * s), h[n], e[(int64_t)(n0 + n) * d.D]);
-        }
+        for (int n = 0; n < NS; ++n)
+            if (n0 + n < d.N) h[n] = fmaf(__builtin_amdgcn_exp2f(A2[n] * s), h[n], e[(int64_t)(n0 + n) * d.D]);
+    }
     TileRegs<T, NW, NS, Z, false> nx, cu;                  // the next tile's inputs, this tile's u and z
     auto stage = [&](int t0) {                             // nx -> LDS
 #pragma unroll
@@ -167,7 +165,6 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
             const float raw = to_f(nx.dt[j]) + bias, s = sp ? softplus_f(raw) : raw, u = to_f(nx.u[j]);
             const bool in = t0 + t < w.len;
             s_dx[t][lane] = make_float2(in ? s : 0.f, in ? s * u : 0.f);
-            if constexpr (ENDS) sum += in ? s : 0.f;
         }
         nx.stage_bc(d, w, t0, s_b, s_c);
     };
@@ -175,7 +172,7 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
     for (int i = w.i0; i < w.i1; ++i) {
         const int t0 = i * TT;
         cu = nx;
-        if (!ENDS && d.ckpt && w.live) {
+        if (d.ckpt && w.live) {
             float* const ck = d.ckpt + (((int64_t)w.b * p.tiles + i) * d.N + n0) * d.D;
 #pragma unroll
             for (int n = 0; n < NS; ++n)
@@ -185,7 +182,7 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
         if (i + 1 < w.i1) nx.load(d, w, wv, t0 + TT);
         float bv[NS], cv[NS];
         wave_bc<NS, BC>(bv, s_b, n0, lane);
-        if constexpr (!ENDS) wave_bc<NS, BC>(cv, s_c, n0, lane);
+        wave_bc<NS, BC>(cv, s_c, n0, lane);
         unroll<TT / 4>([&](auto qc) {
             constexpr int t4 = 4 * decltype(qc)::value;
             float hq[4][NS], y[4];
@@ -199,47 +196,97 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
                 for (int n = 0; n < NS; ++n) hq[f][n] = fmaf(__builtin_amdgcn_exp2f(dx[f].x * A2[n]), f ? hq[f ? f - 1 : 0][n] : h[n], hq[f][n]);
 #pragma unroll
             for (int n = 0; n < NS; ++n) h[n] = hq[3][n];
-            if constexpr (!ENDS) {
-                row_dot4x2<(t4 % 8) * 2>(y, cv[t4 / 8], hq);
+            row_dot4x2<(t4 % 8) * 2>(y, cv[t4 / 8], hq);
 #pragma unroll
-                for (int f = 0; f < 4; ++f) s_y[wv][t4 + f][lane] = y[f];
-            }
+            for (int f = 0; f < 4; ++f) s_y[wv][t4 + f][lane] = y[f];
         });
         lds_barrier();
         if (i + 1 < w.i1) stage(t0 + TT);                  // (the loads are a tile old; the stores below are not waited for)
-        if constexpr (!ENDS) {
-            const uint32_t at = lane_bytes<T>(w.ch);
+        const uint32_t at = lane_bytes<T>(w.ch);
 #pragma unroll
-            for (int j = 0; j < EP; ++j) {
-                const int t = wv + NW * j;
-                float y = skip * to_f(cu.u[j]);
+        for (int j = 0; j < EP; ++j) {
+            const int t = wv + NW * j;
+            float y = skip * to_f(cu.u[j]);
 #pragma unroll
-                for (int v = 0; v < NW; ++v) y += s_y[v][t][lane];
-                if constexpr (Z) y *= silu_f(to_f(cu.z[j]));
-                if (t0 + t < w.len && w.live) st_at((T*)d.y + ((int64_t)w.b * d.T + t0 + t) * d.D, at, from_f<T>(y));
-            }
+            for (int v = 0; v < NW; ++v) y += s_y[v][t][lane];
+            if constexpr (Z) y *= silu_f(to_f(cu.z[j]));
+            if (t0 + t < w.len && w.live) st_at((T*)d.y + ((int64_t)w.b * d.T + t0 + t) * d.D, at, from_f<T>(y));
         }
     }
-    if constexpr (ENDS) {                                  // the block's sum of steps: each thread's own frames, then the waves
-        s_y[0][wv][lane] = sum;
-        lds_barrier();
-        sum = 0.f;
-#pragma unroll
-        for (int v = 0; v < NW; ++v) sum += s_y[0][v][lane];
-    }
     if (!w.live) return;
-    if constexpr (ENDS) {
-        float* const e = p.ends + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 1) * d.D + w.ch;
+    for (int t = max(w.i0 * TT, w.len) + wv; t < min((w.i0 + p.tpc) * TT, d.T); t += NW) ((T*)d.y)[((int64_t)w.b * d.T + t) * d.D + w.ch] = from_f<T>(0.f);
+    if (d.h_out && w.ck == p.chunks - 1)
 #pragma unroll
         for (int n = 0; n < NS; ++n)
-            if (n0 + n < d.N) e[(int64_t)(n0 + n) * d.D] = h[n];
-        if (wv == 0) e[(int64_t)d.N * d.D] = sum;
-    } else {
-        for (int t = max(w.i0 * TT, w.len) + wv; t < min((w.i0 + p.tpc) * TT, d.T); t += NW) ((T*)d.y)[((int64_t)w.b * d.T + t) * d.D + w.ch] = from_f<T>(0.f);
-        if (d.h_out && w.ck == p.chunks - 1)
+            if (n0 + n < d.N) d.h_out[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] = h[n];
+}
+
+// Each chunk's own end state (from zero) and the sum of its steps.  No output per frame, so the shared memory holds two tiles: while one is walked the
+// next one is staged and the one after it requested, with one barrier per tile (1 x 48001 x 1536: 278 us; as the kernel above without its output, two
+// barriers, 340 us.  The kernel above gains nothing from the same form: its sums over states then allow only tiles of 8 frames, 97 us against 86 at
+// 8 x 781 x 1536).
+template <typename T, int NW> __global__ __launch_bounds__(64 * NW) void scan_ends_kernel(ScanArgs p) {
+    constexpr int NS = FNS, EP = TT / NW, BC = NS * NW;
+    __shared__ float2 s_dx[2][TT][CH];
+    __shared__ float s_b[2][TT * BC], s_sum[NW][CH];
+    const a8_selective_scan_desc& d = p.d;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = wv * NS;
+    const Where w = locate(p, lane, 0, p.chunks - 1);
+    const float bias = d.dt_bias ? d.dt_bias[w.ch] : 0.f;
+    const bool sp = d.softplus != 0;
+    float A2[NS], h[NS] = {}, sum = 0.f;
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-                if (n0 + n < d.N) d.h_out[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] = h[n];
+    for (int n = 0; n < NS; ++n) A2[n] = n0 + n < d.N ? d.A[(int64_t)w.ch * d.N + n0 + n] * SEQ_LOG2E : 0.f;
+    TileRegs<T, NW, NS, false, false> nx;
+    auto stage = [&](int i) {                              // (the tile behind the chunk's last one is staged like any other, and neither walked nor summed)
+#pragma unroll
+        for (int j = 0; j < EP; ++j) {
+            const int t = wv + NW * j;
+            const float raw = to_f(nx.dt[j]) + bias, s = sp ? softplus_f(raw) : raw, u = to_f(nx.u[j]);
+            const bool in = i < w.i1 && i * TT + t < w.len;
+            s_dx[i & 1][t][lane] = make_float2(in ? s : 0.f, in ? s * u : 0.f);
+            sum += in ? s : 0.f;
+        }
+        nx.template stage_bc<true, false>(d, w, i * TT, s_b[i & 1], nullptr);
+    };
+    if (w.i0 < w.i1) {
+        nx.load(d, w, wv, w.i0 * TT);
+        stage(w.i0);
+        nx.load(d, w, wv, (w.i0 + 1) * TT);
+        lds_barrier();
+    }
+    for (int i = w.i0; i < w.i1; ++i) {
+        const int q = i & 1;
+        stage(i + 1);
+        nx.load(d, w, wv, (i + 2) * TT);
+        float bv[NS];
+        wave_bc<NS, BC>(bv, s_b[q], n0, lane);
+        unroll<TT / 4>([&](auto qc) {
+            constexpr int t4 = 4 * decltype(qc)::value;
+            float hq[4][NS];
+            float2 dx[4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) dx[f] = s_dx[q][t4 + f][lane];
+            row_outer4x2<(t4 % 8) * 2>(hq, bv[t4 / 8], dx[0].y, dx[1].y, dx[2].y, dx[3].y);
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int n = 0; n < NS; ++n) h[n] = fmaf(__builtin_amdgcn_exp2f(dx[f].x * A2[n]), h[n], hq[f][n]);
+        });
+        lds_barrier();
+    }
+    s_sum[wv][lane] = sum;
+    lds_barrier();
+    if (!w.live) return;
+    float* const e = p.ends + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 1) * d.D + w.ch;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+        if (n0 + n < d.N) e[(int64_t)(n0 + n) * d.D] = h[n];
+    if (wv == 0) {
+        sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < NW; ++v) sum += s_sum[v][lane];
+        e[(int64_t)d.N * d.D] = sum;
     }
 }
 
@@ -281,45 +328,41 @@ A8_DEV float rows_sum_scatter4(const float (&v)[4]) {           // row r: the su
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// ENDS: only the adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps.
-template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void scan_bwd_kernel(ScanArgs p) {
+template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void scan_bwd_kernel(ScanArgs p) {
     constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dxs[2][TT][CH];                    // {D, D u}, by tile parity
     __shared__ float s_gs[2][TT][CH];                      // dout silu(z)
     __shared__ float s_b[TT * BC], s_c[TT * BC];
-    __shared__ float2 s_q[ENDS ? 1 : NW][TT][CH];          // a wave's {sum q B, sum A k}
-    __shared__ float s_y[Z && !ENDS ? NW : 1][TT][CH];
+    __shared__ float2 s_q[NW][TT][CH];                     // a wave's {sum q B, sum A k}
+    __shared__ float s_y[Z ? NW : 1][TT][CH];
     const a8_selective_scan_desc& d = p.d;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = wv * NS;
-    const Where w = locate(p, lane, ENDS ? 1 : 0, ENDS ? p.chunks - 1 : p.chunks);
+    const Where w = locate(p, lane, 0, p.chunks);
     const float bias = d.dt_bias ? d.dt_bias[w.ch] : 0.f, skip = d.Dskip ? d.Dskip[w.ch] : 0.f;
     const bool sp = d.softplus != 0;
-    float A[NS], A2[NS], c[NS], dA[NS] = {}, sum = 0.f;
+    float A[NS], A2[NS], c[NS], dA[NS] = {};
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const bool has = n0 + n < d.N;
         A[n] = has ? d.A[(int64_t)w.ch * d.N + n0 + n] : 0.f;
         A2[n] = A[n] * SEQ_LOG2E;
-        c[n] = !ENDS && has && w.live && d.dh_out ? d.dh_out[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
+        c[n] = has && w.live && d.dh_out ? d.dh_out[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
     }
-    if constexpr (!ENDS)
-        for (int k = p.chunks - 1; k > w.ck; --k) {
-            const float* const e = p.ends + ((int64_t)w.b * p.chunks + k) * (d.N + 1) * d.D + w.ch;
-            const float s = e[(int64_t)d.N * d.D];
+    for (int k = p.chunks - 1; k > w.ck; --k) {            // the adjoint that the chunks behind leave
+        const float* const e = p.ends + ((int64_t)w.b * p.chunks + k) * (d.N + 1) * d.D + w.ch;
+        const float s = e[(int64_t)d.N * d.D];
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-                if (n0 + n < d.N && w.live) c[n] = fmaf(__builtin_amdgcn_exp2f(A2[n] * s), c[n], e[(int64_t)(n0 + n) * d.D]);
-        }
+        for (int n = 0; n < NS; ++n)
+            if (n0 + n < d.N && w.live) c[n] = fmaf(__builtin_amdgcn_exp2f(A2[n] * s), c[n], e[(int64_t)(n0 + n) * d.D]);
+    }
     float dskip = 0.f, dbias = 0.f;
     TileRegs<T, NW, NS, Z, true> nx, cu;
     float rh[NS] = {};
     auto load = [&](int i) {
         nx.load(d, w, wv, i * TT);
-        if constexpr (!ENDS) {
-            const float* const ck = d.ckpt + (((int64_t)w.b * p.tiles + i) * d.N + n0) * d.D;
+        const float* const ck = d.ckpt + (((int64_t)w.b * p.tiles + i) * d.N + n0) * d.D;
 #pragma unroll
-            for (int n = 0; n < NS; ++n) rh[n] = n0 + n < d.N ? ck[(int64_t)n * d.D + w.ch] : 0.f;
-        }
+        for (int n = 0; n < NS; ++n) rh[n] = n0 + n < d.N ? ck[(int64_t)n * d.D + w.ch] : 0.f;
     };
     auto stage = [&](int t0) {
 #pragma unroll
@@ -348,18 +391,17 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
         float bv[NS], cv[NS];
         wave_bc<NS, BC>(bv, s_b, n0, lane);
         wave_bc<NS, BC>(cv, s_c, n0, lane);
-        if constexpr (!ENDS)
-            unroll<TT>([&](auto tc) {                      // the tile's states again, from the saved state before it
-                constexpr int t = decltype(tc)::value;
-                const float2 dx = s_dx[t][lane];
-                unroll<NS>([&](auto nc) {
-                    constexpr int n = decltype(nc)::value;
-                    a[t][n] = __builtin_amdgcn_exp2f(dx.x * A2[n]);
-                    h[t + 1][n] = fmaf(a[t][n], h[t][n], dx.y * bc_at<NS, t, n>(bv));
-                });
-                if constexpr (Z) s_y[wv][t][lane] = row_dot<(t % 4) * 4>(cv[t / 4], h[t + 1]);
-                if constexpr (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        unroll<TT>([&](auto tc) {                         // the tile's states again, from the saved state before it
+            constexpr int t = decltype(tc)::value;
+            const float2 dx = s_dx[t][lane];
+            unroll<NS>([&](auto nc) {
+                constexpr int n = decltype(nc)::value;
+                a[t][n] = __builtin_amdgcn_exp2f(dx.x * A2[n]);
+                h[t + 1][n] = fmaf(a[t][n], h[t][n], dx.y * bc_at<NS, t, n>(bv));
             });
+            if constexpr (Z) s_y[wv][t][lane] = row_dot<(t % 4) * 4>(cv[t / 4], h[t + 1]);
+            if constexpr (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        });
         unroll<TT / 4>([&](auto qc) {                      // backwards, 4 frames at a time
             constexpr int t4 = TT - 4 - 4 * decltype(qc)::value;
             float vb[16], vc[16];
@@ -368,109 +410,149 @@ template <typename T, int NW, bool Z, bool ENDS> __global__ __launch_bounds__(64
                 const float2 dx = s_dx[t][lane];
                 const float g = s_g[t][lane];
                 row_axpy<(t % 4) * 4>(c, cv[t / 4], g);    // c is q_t here
-                if constexpr (ENDS) {
-                    sum += dx.x;
+                const float qb = row_dot<(t % 4) * 4>(bv[t / 4], c);
+                float ak = 0.f;
 #pragma unroll
-                    for (int n = 0; n < NS; ++n) c[n] *= __builtin_amdgcn_exp2f(dx.x * A2[n]);
-                } else {
-                    const float qb = row_dot<(t % 4) * 4>(bv[t / 4], c);
-                    float ak = 0.f;
-#pragma unroll
-                    for (int n = 0; n < NS; ++n) {
-                        vb[(t - t4) * 4 + n] = c[n] * dx.y;
-                        vc[(t - t4) * 4 + n] = h[t + 1][n] * g;
-                        c[n] *= a[t][n];
-                        const float k = c[n] * h[t][n];
-                        ak = fmaf(A[n], k, ak);
-                        dA[n] = fmaf(k, dx.x, dA[n]);
-                    }
-                    s_q[wv][t][lane] = make_float2(qb, ak);
+                for (int n = 0; n < NS; ++n) {
+                    vb[(t - t4) * 4 + n] = c[n] * dx.y;
+                    vc[(t - t4) * 4 + n] = h[t + 1][n] * g;
+                    c[n] *= a[t][n];
+                    const float k = c[n] * h[t][n];
+                    ak = fmaf(A[n], k, ak);
+                    dA[n] = fmaf(k, dx.x, dA[n]);
                 }
+                s_q[wv][t][lane] = make_float2(qb, ak);
             });
-            if constexpr (!ENDS) {
-                gb[t4 / 4] = row_sum_scatter16(vb, lane);
-                gc[t4 / 4] = row_sum_scatter16(vc, lane);
-                __builtin_amdgcn_sched_barrier(0);         // (read ahead of here, the next frames' inputs cost more registers than two waves per SIMD have)
-            }
+            gb[t4 / 4] = row_sum_scatter16(vb, lane);
+            gc[t4 / 4] = row_sum_scatter16(vc, lane);
+            __builtin_amdgcn_sched_barrier(0);             // (read ahead of here, the next frames' inputs cost more registers than two waves per SIMD have)
         });
-        float sb = 0.f, sc = 0.f;
-        if constexpr (!ENDS) {
-            sb = rows_sum_scatter4(gb);
-            sc = rows_sum_scatter4(gc);
-        }
+        const float sb = rows_sum_scatter4(gb), sc = rows_sum_scatter4(gc);
         lds_barrier();
         if (i > w.i0) stage(t0 - TT);
-        if constexpr (!ENDS) {
-            {
-                const int t = t0 + (lane >> 2), n = n0 + (lane & 3);
-                if (t < w.len && n < d.N) {
-                    const int64_t at = ((((int64_t)w.ct * d.B + w.b) * d.T + t) * d.G + w.g) * d.N + n;
-                    p.part_b[at] = sb;
-                    p.part_c[at] = sc;
-                }
+        {
+            const int t = t0 + (lane >> 2), n = n0 + (lane & 3);
+            if (t < w.len && n < d.N) {
+                const int64_t at = ((((int64_t)w.ct * d.B + w.b) * d.T + t) * d.G + w.g) * d.N + n;
+                p.part_b[at] = sb;
+                p.part_c[at] = sc;
             }
-            const uint32_t at = lane_bytes<T>(w.ch);
+        }
+        const uint32_t at = lane_bytes<T>(w.ch);
 #pragma unroll
-            for (int j = 0; j < EP; ++j) {
-                const int t = wv + NW * j;
-                const float u = to_f(cu.u[j]), g = s_g[t][lane];
-                float qb = 0.f, ak = 0.f, y = skip * u;
+        for (int j = 0; j < EP; ++j) {
+            const int t = wv + NW * j;
+            const float u = to_f(cu.u[j]), g = s_g[t][lane];
+            float qb = 0.f, ak = 0.f, y = skip * u;
 #pragma unroll
-                for (int k = 0; k < NW; ++k) { const float2 q = s_q[k][t][lane]; qb += q.x; ak += q.y; }
-                float dd = fmaf(u, qb, ak);
-                if (sp) dd *= sigmoid_f(to_f(cu.dt[j]) + bias);
-                float dz = 0.f;
-                if constexpr (Z) {
+            for (int k = 0; k < NW; ++k) { const float2 q = s_q[k][t][lane]; qb += q.x; ak += q.y; }
+            float dd = fmaf(u, qb, ak);
+            if (sp) dd *= sigmoid_f(to_f(cu.dt[j]) + bias);
+            float dz = 0.f;
+            if constexpr (Z) {
 #pragma unroll
-                    for (int k = 0; k < NW; ++k) y += s_y[k][t][lane];
-                    dz = to_f(cu.dy[j]) * y * silu_grad_f(to_f(cu.z[j]));
-                }
-                if (t0 + t < w.len && w.live) {
-                    const int64_t row = ((int64_t)w.b * d.T + t0 + t) * d.D;
-                    dskip = fmaf(g, u, dskip);
-                    dbias += dd;
-                    st_at((T*)d.du + row, at, from_f<T>(fmaf(s_dx[t][lane].x, qb, skip * g)));
-                    st_at((T*)d.ddt + row, at, from_f<T>(dd));
-                    if constexpr (Z) st_at((T*)d.dz + row, at, from_f<T>(dz));
-                }
+                for (int k = 0; k < NW; ++k) y += s_y[k][t][lane];
+                dz = to_f(cu.dy[j]) * y * silu_grad_f(to_f(cu.z[j]));
+            }
+            if (t0 + t < w.len && w.live) {
+                const int64_t row = ((int64_t)w.b * d.T + t0 + t) * d.D;
+                dskip = fmaf(g, u, dskip);
+                dbias += dd;
+                st_at((T*)d.du + row, at, from_f<T>(fmaf(s_dx[t][lane].x, qb, skip * g)));
+                st_at((T*)d.ddt + row, at, from_f<T>(dd));
+                if constexpr (Z) st_at((T*)d.dz + row, at, from_f<T>(dz));
             }
         }
     }
-    if constexpr (ENDS) {
-        if (w.live) {
-            float* const e = p.ends + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 1) * d.D + w.ch;
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-                if (n0 + n < d.N) e[(int64_t)(n0 + n) * d.D] = c[n];
-            if (wv == 0) e[(int64_t)d.N * d.D] = sum;
+    if (w.live)
+        for (int t = max(w.i0 * TT, w.len) + wv; t < min((w.i0 + p.tpc) * TT, d.T); t += NW) {
+            const int64_t at = ((int64_t)w.b * d.T + t) * d.D + w.ch;
+            ((T*)d.du)[at] = from_f<T>(0.f);
+            ((T*)d.ddt)[at] = from_f<T>(0.f);
+            if constexpr (Z) ((T*)d.dz)[at] = from_f<T>(0.f);
         }
-    } else {
-        if (w.live)
-            for (int t = max(w.i0 * TT, w.len) + wv; t < min((w.i0 + p.tpc) * TT, d.T); t += NW) {
-                const int64_t at = ((int64_t)w.b * d.T + t) * d.D + w.ch;
-                ((T*)d.du)[at] = from_f<T>(0.f);
-                ((T*)d.ddt)[at] = from_f<T>(0.f);
-                if constexpr (Z) ((T*)d.dz)[at] = from_f<T>(0.f);
+    lds_barrier();                                         // (s_q is read by the last tile's epilogue above)
+    s_q[wv][0][lane] = make_float2(dskip, dbias);
+    lds_barrier();
+    float* const part = p.part + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 2) * d.D + w.ch;
+    if (w.live) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+            if (n0 + n < d.N) {
+                part[(int64_t)(n0 + n) * d.D] = dA[n];
+                if (d.dh0 && w.ck == 0) d.dh0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] = c[n];
             }
-        lds_barrier();                                     // (s_q is read by the last tile's epilogue above)
-        s_q[wv][0][lane] = make_float2(dskip, dbias);
+        if (wv == 0) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int k = 0; k < NW; ++k) { s0 += s_q[k][0][lane].x; s1 += s_q[k][0][lane].y; }
+            part[(int64_t)d.N * d.D] = s0;
+            part[(int64_t)(d.N + 1) * d.D] = s1;
+        }
+    }
+}
+
+// The adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps: scan_ends_kernel backwards.
+template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void scan_back_ends_kernel(ScanArgs p) {
+    constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
+    __shared__ float2 s_dg[2][TT][CH];                     // {D, dout silu(z)}
+    __shared__ float s_c[2][TT * BC], s_sum[NW][CH];
+    const a8_selective_scan_desc& d = p.d;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = wv * NS;
+    const Where w = locate(p, lane, 1, p.chunks - 1);
+    const float bias = d.dt_bias ? d.dt_bias[w.ch] : 0.f;
+    const bool sp = d.softplus != 0;
+    float A2[NS], c[NS] = {}, sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) A2[n] = n0 + n < d.N ? d.A[(int64_t)w.ch * d.N + n0 + n] * SEQ_LOG2E : 0.f;
+    TileRegs<T, NW, NS, Z, true> nx;
+    auto load = [&](int i) { nx.load(d, w, wv, max(i, 0) * TT); };
+    auto stage = [&](int i) {                              // (the tile in front of the chunk's first one is neither walked nor summed)
+#pragma unroll
+        for (int j = 0; j < EP; ++j) {
+            const int t = wv + NW * j;
+            const float raw = to_f(nx.dt[j]) + bias, s = sp ? softplus_f(raw) : raw;
+            const bool in = i >= w.i0 && i * TT + t < w.len;
+            float g = to_f(nx.dy[j]);
+            if constexpr (Z) g *= silu_f(to_f(nx.z[j]));
+            s_dg[i & 1][t][lane] = make_float2(in ? s : 0.f, in ? g : 0.f);
+            sum += in ? s : 0.f;
+        }
+        nx.template stage_bc<false, true>(d, w, i * TT, nullptr, s_c[i & 1]);
+    };
+    if (w.i0 < w.i1) {
+        load(w.i1 - 1);
+        stage(w.i1 - 1);
+        load(w.i1 - 2);
         lds_barrier();
-        float* const part = p.part + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 2) * d.D + w.ch;
-        if (w.live) {
+    }
+    for (int i = w.i1 - 1; i >= w.i0; --i) {
+        const int q = i & 1;
+        stage(i - 1);
+        load(i - 2);
+        float cv[NS];
+        wave_bc<NS, BC>(cv, s_c[q], n0, lane);
+        unroll<TT>([&](auto tc) {
+            constexpr int t = TT - 1 - decltype(tc)::value;
+            const float2 dg = s_dg[q][t][lane];
+            row_axpy<(t % 4) * 4>(c, cv[t / 4], dg.y);
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-                if (n0 + n < d.N) {
-                    part[(int64_t)(n0 + n) * d.D] = dA[n];
-                    if (d.dh0 && w.ck == 0) d.dh0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] = c[n];
-                }
-            if (wv == 0) {
-                float s0 = 0.f, s1 = 0.f;
+            for (int n = 0; n < NS; ++n) c[n] *= __builtin_amdgcn_exp2f(dg.x * A2[n]);
+        });
+        lds_barrier();
+    }
+    s_sum[wv][lane] = sum;
+    lds_barrier();
+    if (!w.live) return;
+    float* const e = p.ends + ((int64_t)w.b * p.chunks + w.ck) * (d.N + 1) * d.D + w.ch;
 #pragma unroll
-                for (int k = 0; k < NW; ++k) { s0 += s_q[k][0][lane].x; s1 += s_q[k][0][lane].y; }
-                part[(int64_t)d.N * d.D] = s0;
-                part[(int64_t)(d.N + 1) * d.D] = s1;
-            }
-        }
+    for (int n = 0; n < NS; ++n)
+        if (n0 + n < d.N) e[(int64_t)(n0 + n) * d.D] = c[n];
+    if (wv == 0) {
+        sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < NW; ++v) sum += s_sum[v][lane];
+        e[(int64_t)d.N * d.D] = sum;
     }
 }
 
@@ -583,42 +665,35 @@ ScanArgs scan_args(const a8_selective_scan_desc* d, bool backward) {
 int64_t scan_blocks(const ScanArgs& p, int chunks) { return (int64_t)p.d.B * p.d.G * p.tpg * chunks; }
 int64_t ends_floats(const ScanArgs& p) { return p.chunks > 1 ? (int64_t)p.d.B * p.chunks * (p.d.N + 1) * p.d.D : 0; }
 
-#define SCAN_LAUNCH(KERNEL, T, NW, Z, ENDS) hipLaunchKernelGGL((KERNEL<T, NW, Z, ENDS>), grid, dim3(64 * NW), 0, st, p)
-#define FWD_WAVES(T, Z, ENDS)                                                                                     \
-    do {                                                                                                          \
-        if (waves <= 1) SCAN_LAUNCH(scan_fwd_kernel, T, 1, Z, ENDS);                                              \
-        else if (waves <= 2) SCAN_LAUNCH(scan_fwd_kernel, T, 2, Z, ENDS);                                         \
-        else if (waves <= 4) SCAN_LAUNCH(scan_fwd_kernel, T, 4, Z, ENDS);                                         \
-        else if (waves <= 8) SCAN_LAUNCH(scan_fwd_kernel, T, 8, Z, ENDS);                                         \
-        else SCAN_LAUNCH(scan_fwd_kernel, T, 16, Z, ENDS);                                                        \
-    } while (0)
-#define BWD_WAVES(T, Z, ENDS)                                                                                     \
-    do {                                                                                                          \
-        if (waves <= 1) SCAN_LAUNCH(scan_bwd_kernel, T, 1, Z, ENDS);                                              \
-        else if (waves <= 2) SCAN_LAUNCH(scan_bwd_kernel, T, 2, Z, ENDS);                                         \
-        else if (waves <= 4) SCAN_LAUNCH(scan_bwd_kernel, T, 4, Z, ENDS);                                         \
-        else SCAN_LAUNCH(scan_bwd_kernel, T, 8, Z, ENDS);                                                         \
-    } while (0)
+#define FWD_WAVES(KERNEL, ...)                                                                                    \
+    (waves <= 1 ? (KERNEL(1, __VA_ARGS__)) : waves <= 2 ? (KERNEL(2, __VA_ARGS__)) : waves <= 4 ? (KERNEL(4, __VA_ARGS__))      \
+     : waves <= 8 ? (KERNEL(8, __VA_ARGS__)) : (KERNEL(16, __VA_ARGS__)))
+#define FWD_KERNEL(NW, T, Z) scan_fwd_kernel<T, NW, Z>
+#define ENDS_KERNEL(NW, T) scan_ends_kernel<T, NW>
+#define BWD_WAVES(KERNEL, ...)                                                                                    \
+    (waves <= 1 ? (KERNEL(1, __VA_ARGS__)) : waves <= 2 ? (KERNEL(2, __VA_ARGS__)) : waves <= 4 ? (KERNEL(4, __VA_ARGS__)) : (KERNEL(8, __VA_ARGS__)))
+#define BWD_KERNEL(NW, T, Z) scan_bwd_kernel<T, NW, Z>
+#define BACK_ENDS_KERNEL(NW, T, Z) scan_back_ends_kernel<T, NW, Z>
 
-// A chunk's own end does not look at z in the forward; in the backward it does (through dout silu(z)).
 int launch_fwd(const ScanArgs& p, bool ends, hipStream_t st) {
-    const dim3 grid((unsigned)scan_blocks(p, ends ? p.chunks - 1 : p.chunks));
     const int waves = cdiv(p.d.N, FNS);
     const bool bf = p.d.dtype == A8_BF16, z = p.d.z != nullptr;
-    if (ends) { if (bf) FWD_WAVES(bf16, false, true); else FWD_WAVES(float, false, true); }
-    else if (bf) { if (z) FWD_WAVES(bf16, true, false); else FWD_WAVES(bf16, false, false); }
-    else { if (z) FWD_WAVES(float, true, false); else FWD_WAVES(float, false, false); }
+    auto kernel = ends ? (bf ? FWD_WAVES(ENDS_KERNEL, bf16) : FWD_WAVES(ENDS_KERNEL, float))
+                  : bf ? (z ? FWD_WAVES(FWD_KERNEL, bf16, true) : FWD_WAVES(FWD_KERNEL, bf16, false))
+                       : (z ? FWD_WAVES(FWD_KERNEL, float, true) : FWD_WAVES(FWD_KERNEL, float, false));
+    const int block = 64 * (waves <= 1 ? 1 : waves <= 2 ? 2 : waves <= 4 ? 4 : waves <= 8 ? 8 : 16);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)scan_blocks(p, ends ? p.chunks - 1 : p.chunks)), dim3(block), 0, st, p);
     return a8_check_launch("a8_selective_scan_fwd");
 }
 int launch_bwd(const ScanArgs& p, bool ends, hipStream_t st) {
-    const dim3 grid((unsigned)scan_blocks(p, ends ? p.chunks - 1 : p.chunks));
     const int waves = cdiv(p.d.N, BNS);
     const bool bf = p.d.dtype == A8_BF16, z = p.d.z != nullptr;
-    if (ends) {
-        if (bf) { if (z) BWD_WAVES(bf16, true, true); else BWD_WAVES(bf16, false, true); }
-        else { if (z) BWD_WAVES(float, true, true); else BWD_WAVES(float, false, true); }
-    } else if (bf) { if (z) BWD_WAVES(bf16, true, false); else BWD_WAVES(bf16, false, false); }
-    else { if (z) BWD_WAVES(float, true, false); else BWD_WAVES(float, false, false); }
+    auto kernel = ends ? (bf ? (z ? BWD_WAVES(BACK_ENDS_KERNEL, bf16, true) : BWD_WAVES(BACK_ENDS_KERNEL, bf16, false))
+                             : (z ? BWD_WAVES(BACK_ENDS_KERNEL, float, true) : BWD_WAVES(BACK_ENDS_KERNEL, float, false)))
+                       : (bf ? (z ? BWD_WAVES(BWD_KERNEL, bf16, true) : BWD_WAVES(BWD_KERNEL, bf16, false))
+                             : (z ? BWD_WAVES(BWD_KERNEL, float, true) : BWD_WAVES(BWD_KERNEL, float, false)));
+    const int block = 64 * (waves <= 1 ? 1 : waves <= 2 ? 2 : waves <= 4 ? 4 : 8);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)scan_blocks(p, ends ? p.chunks - 1 : p.chunks)), dim3(block), 0, st, p);
     return a8_check_launch("a8_selective_scan_bwd");
 }
 
