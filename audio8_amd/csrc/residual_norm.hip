@@ -6,9 +6,10 @@
 //   dw = sum dn rhat, db = sum dn;  with E1 = sum dR gate ohat, E0 = sum dR gate:  dpw = scale E1, dpb = scale E0, dscale = pw E1 + pb E0
 // (four column sums instead of five: p and dp are columns times ohat and dR gate).
 //
-// Bound by HBM.  A row is held in registers by one wave (C <= 1024) or by a block (wider rows), 8 consecutive channels per lane and round: every
-// tensor is read and written once, statistics are exact two-pass in f32.  The backward walks many rows per wave, the next row's loads in flight, the
-// parameters in LDS, the column sums in registers.
+// Bound by HBM.  A row is held in registers, 8 consecutive channels per lane and round, by one wave (forward up to 1024 channels, backward up to 512),
+// by two (backward up to 1024) or by a block: every tensor is read and written once, statistics are exact two-pass in f32.  The backward walks many
+// rows, the next row's loads in flight, the parameters in LDS, the column sums in registers.  bf16, both norms, a gate per utterance:
+// 32 x 1499 x 1024 forward 81 us (393 MB, 4.8 TB/s), backward 125 us (589 MB, 4.7 TB/s), parameter gradients 12 us.
 #include "a8_seq.h"
 #include "a8hip_internal.h"
 
@@ -192,29 +193,36 @@ template <typename T> struct Raw {
     }
 };
 
-// two row sums at once
-template <int RW> A8_DEV void row_sum2(float& a, float& b, float2* red) {
+// two row sums at once.  Successive calls alternate between two `red`: a wave writes one only behind the barrier of the other's sum, in front of which
+// every wave has read it, so a call has one barrier, and one that leaves the loads of the next row in flight.
+template <int RW> A8_DEV void row_sum2(float& a, float& b, float2 (*red)[RW], int& turn) {
     a = wave_sum(a);
     b = wave_sum(b);
     if constexpr (RW > 1) {
         const int w = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[w] = make_float2(a, b);
-        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[turn][w] = make_float2(a, b);
+        lds_barrier();
         a = b = 0.f;
 #pragma unroll
-        for (int i = 0; i < RW; ++i) { a += red[i].x; b += red[i].y; }
+        for (int i = 0; i < RW; ++i) { a += red[turn][i].x; b += red[turn][i].y; }
+        turn ^= 1;
     }
 }
 
 enum { GATE_NONE = 0, GATE_ROWS, GATE_UTT };
+// one row as loaded
+template <typename T, int NCH, bool GROWS> struct RawRow { Raw<T> o[NCH], x[NCH], dr[NCH], dn[NCH], g[GROWS ? NCH : 1]; float st[4]; };
 // (the kind of gate is a template parameter for its registers: with all three in one kernel a row of 1024 took 314 and one wave per SIMD)
-template <typename T, int RW, int NCH, bool VEC, int GATE> __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void rnorm_bwd_kernel(NormArgs p) {
+template <typename T, int RW, int NCH, bool VEC, int GATE> __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64, VEC && RW <= 4 ? 3 : 1) void rnorm_bwd_kernel(NormArgs p) {
     typedef Row<T, RW, NCH> R;
     constexpr int W = R::NT * NCH * 8;                         // columns a row's threads cover
-    __shared__ float2 red[R::WAVES];
+    // Rows in flight: two, where three waves per SIMD still hold them (32 x 1499 x 1024: 149 us with one row and two waves, 121 with two rows and three;
+    // one wave per row, 512 channels: 123 us with one, 270 with two and the spills of three waves).
+    constexpr int AHEAD = RW == 1 || RW == 16 ? 1 : 2;
+    __shared__ float2 red[2][RW];
     __shared__ __align__(16) float par[4][W];                  // scale, pw, pb, w (1, 1, 0, 1 where there is none); then the waves' column sums
     const a8_residual_norm_desc& d = p.d;
+    int turn = 0;
     R row;
     row.init(d.C, VEC);
     const int rows = d.B * d.T, b = blockIdx.x / p.chunks, ck = blockIdx.x % p.chunks;
@@ -231,56 +239,60 @@ template <typename T, int RW, int NCH, bool VEC, int GATE> __global__ __launch_b
     }
     __syncthreads();
     float acc[PLANES][NCH][8] = {};
-    Raw<T> ug[GATE == GATE_UTT ? NCH : 1], rg[GATE == GATE_ROWS ? NCH : 1];       // the utterance's gate; the row's
-    if constexpr (GATE == GATE_UTT)
+    // the utterance's gate stays in registers, but not in the 128 of a block of 16 waves (32 x 187 x 8192: 246 us with it and its spills, 151 re-read)
+    constexpr bool held = GATE == GATE_UTT && RW < 16;
+    Raw<T> ug[GATE == GATE_UTT ? NCH : 1];
+    auto load_ug = [&]() {
+        if constexpr (GATE == GATE_UTT)
 #pragma unroll
-        for (int j = 0; j < NCH; ++j)
-            if (row.on[j]) ug[j].load((const T*)d.gate + (int64_t)b * d.g_bs + row.col[j], VEC, d.C - row.col[j]);
-    auto gate_of = [&](int j, int k) { return GATE == GATE_ROWS ? to_f(rg[GATE == GATE_ROWS ? j : 0].v[k]) : GATE == GATE_UTT ? to_f(ug[GATE == GATE_UTT ? j : 0].v[k]) : 1.f; };
-    Raw<T> ro[NCH], rx[NCH], rdr[NCH], rdn[NCH];
-    float st[4];
-    auto load = [&](int t) {
+            for (int j = 0; j < NCH; ++j)
+                if (row.on[j]) ug[j].load((const T*)d.gate + (int64_t)b * d.g_bs + row.col[j], VEC, d.C - row.col[j]);
+    };
+    if constexpr (held) load_ug();
+    typedef RawRow<T, NCH, gate_rows> In;
+    auto load = [&](In& in, int t) {
         const int64_t r = (int64_t)b * d.T + t;
 #pragma unroll
         for (int j = 0; j < NCH; ++j)
             if (row.on[j]) {
                 const int c = row.col[j], left = d.C - c;
-                ro[j].load((const T*)d.o + r * d.o_ld + c, VEC, left);
+                in.o[j].load((const T*)d.o + r * d.o_ld + c, VEC, left);
                 if (d.dn) {
-                    rx[j].load((const T*)d.x + r * d.x_ld + c, VEC, left);
-                    rdn[j].load((const T*)d.dn + r * d.C + c, VEC, left);
+                    in.x[j].load((const T*)d.x + r * d.x_ld + c, VEC, left);
+                    in.dn[j].load((const T*)d.dn + r * d.C + c, VEC, left);
                 }
-                if (d.dr) rdr[j].load((const T*)d.dr + r * d.C + c, VEC, left);
-                if constexpr (gate_rows) rg[j].load((const T*)d.gate + (int64_t)b * d.g_bs + (int64_t)t * d.g_ts + c, VEC, left);
+                if (d.dr) in.dr[j].load((const T*)d.dr + r * d.C + c, VEC, left);
+                if constexpr (gate_rows) in.g[j].load((const T*)d.gate + (int64_t)b * d.g_bs + (int64_t)t * d.g_ts + c, VEC, left);
             }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) st[k] = (k < 2 ? d.post != 0 : d.dn != nullptr) ? d.stats[k * (int64_t)rows + r] : k & 1;
+        for (int k = 0; k < 4; ++k) in.st[k] = (k < 2 ? d.post != 0 : d.dn != nullptr) ? d.stats[k * (int64_t)rows + r] : k & 1;
     };
-    if (ta + wv < tb) load(ta + wv);
-    for (int t = ta + wv; t < tb; t += step) {
+    auto walk = [&](In& in, int t) {
+        if constexpr (GATE == GATE_UTT && !held) load_ug();
+        auto gate_of = [&](int j, int k) { return gate_rows ? to_f(in.g[gate_rows ? j : 0].v[k]) : GATE == GATE_UTT ? to_f(ug[GATE == GATE_UTT ? j : 0].v[k]) : 1.f; };
         const int64_t r = (int64_t)b * d.T + t;
         float oh[NCH][8], g[gate_rows ? NCH : 1][8], h[NCH][8], v[NCH][8], dR[NCH][8];     // ohat (or o), the row's gate, rhat, scratch, dr then dR
-        const float mo = st[0], so = st[1], mr = st[2], sr = st[3];
+        const float mo = in.st[0], so = in.st[1], mr = in.st[2], sr = in.st[3];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             const float* const pc = &par[0][row.col[j]];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const bool in = row.has(j, k);
-                const float xh = d.dn ? to_f(rx[j].v[k]) : 0.f;
-                oh[j][k] = in ? (to_f(ro[j].v[k]) - mo) * so : 0.f;         // (mo = 0, so = 1 without a norm)
-                const float gt = in ? gate_of(j, k) : 0.f;
+                const bool on = row.has(j, k);
+                const float xh = d.dn ? to_f(in.x[j].v[k]) : 0.f;
+                oh[j][k] = on ? (to_f(in.o[j].v[k]) - mo) * so : 0.f;         // (mo = 0, so = 1 without a norm)
+                const float gt = on ? gate_of(j, k) : 0.f;
                 if constexpr (gate_rows) g[j][k] = gt;
-                dR[j][k] = in && d.dr ? to_f(rdr[j].v[k]) : 0.f;
+                dR[j][k] = on && d.dr ? to_f(in.dr[j].v[k]) : 0.f;
                 const float pp = fmaf(oh[j][k], pc[W + k], pc[2 * W + k]);
-                h[j][k] = in && d.dn ? (fmaf(pc[k] * gt, pp, xh) - mr) * sr : 0.f;
-                const float dn = in && d.dn ? to_f(rdn[j].v[k]) : 0.f;
+                h[j][k] = on && d.dn ? (fmaf(pc[k] * gt, pp, xh) - mr) * sr : 0.f;
+                const float dn = on && d.dn ? to_f(in.dn[j].v[k]) : 0.f;
                 acc[PLANE_W][j][k] = fmaf(dn, h[j][k], acc[PLANE_W][j][k]);
                 acc[PLANE_B][j][k] += dn;
                 v[j][k] = dn * pc[3 * W + k];
             }
         }
-        if (t + step < tb) load(t + step);
+        if (t + AHEAD * step < tb) load(in, t + AHEAD * step);
         float s1 = 0.f, s2 = 0.f;
         const float inv = 1.0f / (float)d.C;
         if (d.dn) {
@@ -288,7 +300,7 @@ template <typename T, int RW, int NCH, bool VEC, int GATE> __global__ __launch_b
             for (int j = 0; j < NCH; ++j)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) { s1 += v[j][k]; s2 = fmaf(v[j][k], h[j][k], s2); }
-            row_sum2<RW>(s1, s2, red);
+            row_sum2<RW>(s1, s2, red, turn);
             s1 = layer ? s1 * inv : 0.f;
             s2 *= inv;
 #pragma unroll
@@ -316,7 +328,7 @@ template <typename T, int RW, int NCH, bool VEC, int GATE> __global__ __launch_b
         }
         if constexpr (gate_rows) row.store((T*)d.dgate + r * d.C, v);
         if (d.post) {
-            row_sum2<RW>(s1, s2, red);
+            row_sum2<RW>(s1, s2, red, turn);
             s1 = layer ? s1 * inv : 0.f;
             s2 *= inv;
 #pragma unroll
@@ -325,19 +337,30 @@ template <typename T, int RW, int NCH, bool VEC, int GATE> __global__ __launch_b
                 for (int k = 0; k < 8; ++k) h[j][k] = so * (h[j][k] - s1 - oh[j][k] * s2);
         }
         row.store((T*)d.d_o + r * d.C, h);
+    };
+    In in[AHEAD];
+    const int t0 = ta + wv;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (t0 + i * step < tb) load(in[i], t0 + i * step);
+    for (int t = t0; t < tb; t += AHEAD * step) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (t + i * step < tb) walk(in[i], t + i * step);
     }
     // block totals [4 planes][C], and the utterance gate's gradient behind all blocks' planes.  Its terms per frame are dR scale (pw ohat + pb).
     float* const part = d.ws + (int64_t)blockIdx.x * PLANES * d.C;
     float* const partg = d.ws + (int64_t)gridDim.x * PLANES * d.C + (int64_t)blockIdx.x * d.C;
     constexpr bool utt = GATE == GATE_UTT;
     float gd[utt ? NCH : 1][8];
+    if constexpr (utt && !held) load_ug();
     if constexpr (utt)
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             const float* const pc = &par[0][row.col[j]];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float gt = row.has(j, k) ? gate_of(j, k) : 0.f;
+                const float gt = row.has(j, k) ? to_f(ug[j].v[k]) : 0.f;
                 gd[j][k] = pc[k] * fmaf(pc[W + k], acc[PLANE_E1][j][k], pc[2 * W + k] * acc[PLANE_E0][j][k]);
                 acc[PLANE_E1][j][k] *= gt;
                 acc[PLANE_E0][j][k] *= gt;
@@ -429,22 +452,24 @@ NormArgs norm_args(const a8_residual_norm_desc* d) {
     const void* ptrs[] = {d->x, d->o, d->gate, d->r, d->n, d->post_w, d->post_b, d->w, d->b, d->scale, d->dr, d->dn, d->dx, d->d_o, d->dgate, d->ws};
     p.vec = d->C % 8 == 0 && d->x_ld % 8 == 0 && d->o_ld % 8 == 0 && (!d->gate || (d->g_bs % 8 == 0 && (!d->gate_rows || d->g_ts % 8 == 0)));
     for (const void* q : ptrs) p.vec = p.vec && aligned16(q);
-    const int per_b = d->B > 0 ? cdiv(d->C <= 512 ? 512 : 1024, d->B) : 1;       // about two waves per SIMD in all, at least 4 rows per block
+    // the backward's blocks: what the CUs hold at once, three waves per SIMD up to 2048 channels and one block per CU beyond, with at least 4 rows each
+    const int resident = d->C <= 512 ? 768 : d->C <= 1024 ? 1536 : d->C <= 2048 ? 768 : 256;
+    const int per_b = d->B > 0 ? std::max(1, resident / d->B) : 1;
     p.rows_per_chunk = d->T > 0 ? cdiv(d->T, per_b) : 1;
     if (p.rows_per_chunk < 4) p.rows_per_chunk = 4;
     p.chunks = d->T > 0 ? cdiv(d->T, p.rows_per_chunk) : 0;
     return p;
 }
 
-// Forward: a wave per row up to 1024 channels (four rows side by side), a block per row beyond.  Backward: two waves per row from 513 on (a lane with 16
-// channels takes over 250 registers: 32 x 1499 x 1024 with a block count that fits each, 166 us, two waves 153 .. 169, and 8 x 781 x 768 39 us against 29).
-#define NORM_WIDE(KERNEL, T, ...)                                                                                                 \
-    (d->C <= 2048 ? (KERNEL<T, 4, 1, ##__VA_ARGS__>) : d->C <= 4096 ? (KERNEL<T, 8, 1, ##__VA_ARGS__>) : (KERNEL<T, 16, 1, ##__VA_ARGS__>))
-#define NORM_FWD(T) (d->C <= 512 ? (rnorm_fwd_kernel<T, 1, 1>) : d->C <= 1024 ? (rnorm_fwd_kernel<T, 1, 2>) : NORM_WIDE(rnorm_fwd_kernel, T))
+// Forward: a wave per row up to 1024 channels (four rows side by side), a block per row beyond.
+#define NORM_FWD(T)                                                                                                              \
+    (d->C <= 512 ? (rnorm_fwd_kernel<T, 1, 1>) : d->C <= 1024 ? (rnorm_fwd_kernel<T, 1, 2>) : d->C <= 2048 ? (rnorm_fwd_kernel<T, 4, 1>)    \
+     : d->C <= 4096 ? (rnorm_fwd_kernel<T, 8, 1>) : (rnorm_fwd_kernel<T, 16, 1>))
+// Backward: two waves per row from 513 on (a lane with 16 channels takes over 250 registers: 8 x 781 x 768 39 us against 28).
 #define NORM_BWD(T, VEC, GATE)                                                                                                    \
-    (d->C <= 512 ? (rnorm_bwd_kernel<T, 1, 1, VEC, GATE>) : d->C <= 1024 ? (rnorm_bwd_kernel<T, 2, 1, VEC, GATE>) : NORM_WIDE(rnorm_bwd_kernel, T, VEC, GATE))
+    (d->C <= 512 ? (rnorm_bwd_kernel<T, 1, 1, VEC, GATE>) : d->C <= 1024 ? (rnorm_bwd_kernel<T, 2, 1, VEC, GATE>)                 \
+     : d->C <= 2048 ? (rnorm_bwd_kernel<T, 4, 1, VEC, GATE>) : d->C <= 4096 ? (rnorm_bwd_kernel<T, 8, 1, VEC, GATE>) : (rnorm_bwd_kernel<T, 16, 1, VEC, GATE>))
 #define NORM_GATE(T, VEC) (!d->gate ? NORM_BWD(T, VEC, GATE_NONE) : d->gate_rows ? NORM_BWD(T, VEC, GATE_ROWS) : NORM_BWD(T, VEC, GATE_UTT))
-int wide_threads(const a8_residual_norm_desc* d) { return d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024; }
 
 }  // namespace
 
@@ -455,7 +480,7 @@ extern "C" int a8_residual_norm_fwd(const a8_residual_norm_desc* d, void* stream
     const NormArgs p = norm_args(d);
     const int rows = d->B * d->T;
     auto kernel = d->dtype == A8_BF16 ? NORM_FWD(bf16) : NORM_FWD(float);
-    hipLaunchKernelGGL(kernel, dim3(d->C <= 1024 ? cdiv(rows, 4) : rows), dim3(wide_threads(d)), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(kernel, dim3(d->C <= 1024 ? cdiv(rows, 4) : rows), dim3(d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024), 0, (hipStream_t)stream, p);
     return a8_check_launch("a8_residual_norm_fwd");
 }
 
@@ -474,7 +499,7 @@ extern "C" int a8_residual_norm_bwd(const a8_residual_norm_desc* d, void* stream
         A8_REQUIRE(d->x && d->o && d->dx && d->d_o && d->ws && (d->dgate || !d->gate) && (d->stats || !(d->post || d->dn)) && (d->w || !d->dn),
                    "a8_residual_norm_bwd: null operand");
         auto kernel = d->dtype == A8_BF16 ? (p.vec ? NORM_GATE(bf16, true) : NORM_GATE(bf16, false)) : (p.vec ? NORM_GATE(float, true) : NORM_GATE(float, false));
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(d->C <= 512 ? 256 : d->C <= 1024 ? 128 : wide_threads(d)), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(d->C <= 512 ? 256 : d->C <= 1024 ? 128 : d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024), 0, (hipStream_t)stream, p);
         if (int e = a8_check_launch("a8_residual_norm_bwd")) return e;
     }
     A8_REQUIRE((int64_t)d->B * d->C < (1 << 30), "a8_residual_norm_bwd: B x C = %d x %d is too large", d->B, d->C);

@@ -20,7 +20,7 @@ namespace {
 
 constexpr int TT = 16;      // frames of a tile
 constexpr int CH = 64;      // channels of a block
-constexpr int FNS = 2;      // states of a wave, forward: 8 waves for 16 states, two per SIMD (one wave alone issues a VALU operation every ~9 cycles, two every ~5)
+constexpr int FNS = 2;      // states of a wave, forward: 8 waves for 16 states, two per SIMD from one block (with 4: 1 x 781 x 1536 106 us against 88; no difference on a full card)
 constexpr int BNS = 4;      // states of a wave, backward: 16 frames x 4 states of decays and of states live in registers
 
 struct ScanArgs {
@@ -133,6 +133,10 @@ template <int I> A8_DEV void row_axpy(float (&x)[4], float v, float g) {
 // element (t, n) of wave_bc's values
 template <int NS, int T_, int N_> A8_DEV float bc_at(const float (&v)[NS]) { return row_value<(T_ % (16 / NS)) * NS + N_>(v[T_ / (16 / NS)]); }
 
+// The scan of one chunk, from the state that the chunks before it leave.  Bound by VALU issue: a state takes a multiply, an exp2 (two issue slots), a
+// multiply and two multiply-adds, 24 cycles for 64 channels, and a (frame, channel) about 160 for softplus, silu, conversions and the sum over waves.
+// bf16, N = 16, gated, states saved for the backward: 16 x 999 x 2048 175 us (524e6 states: 3.0e12 / s, VALU busy 77 % of the cycles, 0.39 GB at 2.2 TB/s),
+// 8 x 781 x 1536 86 us (192 blocks leave a quarter of the CUs idle; chunks would cost what they win).
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs p) {
     constexpr int NS = FNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dx[TT][CH];                        // {D, D u}
@@ -328,6 +332,10 @@ A8_DEV float rows_sum_scatter4(const float (&v)[4]) {           // row r: the su
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// The gradient of one chunk, from the adjoint that the chunks behind it leave; tiles run backwards, each from its saved state.  Bound by VALU issue: per
+// state the recurrence again (24 cycles), the adjoint with its five products (32), and its share of the two sums over channels (17); 256 registers and
+// 76 KB of LDS allow two blocks of 16 states on a CU, two waves per SIMD.  bf16, N = 16, gated: 16 x 999 x 2048 450 us (1.2e12 states / s, VALU busy
+// 71 %), 8 x 781 x 1536 153 + 37 us in 8 chunks.
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void scan_bwd_kernel(ScanArgs p) {
     constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dxs[2][TT][CH];                    // {D, D u}, by tile parity
@@ -492,7 +500,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >
     }
 }
 
-// The adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps: scan_ends_kernel backwards.
+// The adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps: scan_ends_kernel backwards (8 x 781 x 1536: 37 us of 190).
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void scan_back_ends_kernel(ScanArgs p) {
     constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dg[2][TT][CH];                     // {D, dout silu(z)}
@@ -556,7 +564,8 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void
     }
 }
 
-// dB, dC = the channel tiles' partial sums, in tile order; frames behind an utterance's end are zero
+// dB, dC = the channel tiles' partial sums, in tile order; frames behind an utterance's end are zero.  Bound by HBM: the D / 64 tiles' sums, 8 bytes per
+// frame, state and tile, are read once (8 x 781, 24 tiles, N = 16: 19 MB in 9.6 us; 16 x 999, 32 tiles: 65 MB in 20 us, 3.3 TB/s).
 template <typename T> __global__ __launch_bounds__(256) void scan_bc_kernel(ScanArgs p) {
     const a8_selective_scan_desc& d = p.d;
     const int64_t row = (int64_t)d.G * d.N, total = (int64_t)d.B * d.T * row;
@@ -571,7 +580,7 @@ template <typename T> __global__ __launch_bounds__(256) void scan_bc_kernel(Scan
 }
 
 // One frame: 4 lanes per channel, 4 consecutive states per lane and round; the state is read and written once.  What a launch of one frame costs is
-// latency, so every load is issued before the first use.  VEC: N % 4 = 0 and 16-byte aligned A and state.
+// latency, so every load is issued before the first use.  VEC: N % 4 = 0 and 16-byte aligned A and state.  bf16 32 x 1536, N = 16: 4.0 us, 6.8 MB.
 template <typename T> A8_DEV float ldf(const void* p, int64_t i) { return to_f(((const T*)p)[i]); }
 template <typename T, bool VEC> __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p) {
     const a8_selective_scan_desc& d = p.d;
@@ -634,7 +643,7 @@ int scan_check(const a8_selective_scan_desc* d, const char* what) {
     return A8_OK;
 }
 // Frame chunks.  A launch of n chunks takes ceil-rounds of the blocks that the 256 CUs hold: `part[k - 1]` is the time of a round with k blocks on a
-// CU as a share of a full one, `extra` what the chunks' own ends cost more.  Measured, D = 1536 and 781 frames (us, 1 chunk / the count taken here):
+// CU as a share of a full one, `extra` what the chunks' own ends cost more (forward: 0.7 of the walk itself; 1 leaves near ties to one launch).  Measured, D = 1536 and 781 frames (us, 1 chunk / the count taken here):
 // forward B = 1 85 / 28 (12), B = 4 88 / 62 (8), B = 8 91 / 91 (1; 100 with 4); backward B = 1 256 / 55 (12), B = 4 275 / 119 (12), B = 8 279 / 199 (8);
 // 16 x 999 x 2048 (512 blocks) 180 and 503 with one chunk, 233 and 564 with two.  A chunk has at least 4 tiles: its first loads and its share of
 // the walk over the chunks before it stay small.
