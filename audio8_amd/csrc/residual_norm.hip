@@ -9,7 +9,7 @@
 // Bound by HBM.  A row is held in registers, 8 consecutive channels per lane and round, by one wave (forward up to 1024 channels, backward up to 512),
 // by two (backward up to 1024) or by a block: every tensor is read and written once, statistics are exact two-pass in f32.  The backward walks many
 // rows, the next row's loads in flight, the parameters in LDS, the column sums in registers.  bf16, both norms, a gate per utterance:
-// 32 x 1499 x 1024 forward 81 us (393 MB, 4.8 TB/s), backward 125 us (589 MB, 4.7 TB/s), parameter gradients 12 us.
+// 32 x 1499 x 1024 forward 81 us (393 MB, 4.8 TB/s), backward 142 us (589 MB, 4.1 TB/s), parameter gradients 13 us.
 #include "a8_seq.h"
 #include "a8hip_internal.h"
 
@@ -216,8 +216,8 @@ template <typename T, int NCH, bool GROWS> struct RawRow { Raw<T> o[NCH], x[NCH]
 template <typename T, int RW, int NCH, bool VEC, int GATE> __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64, VEC && RW <= 4 ? 3 : 1) void rnorm_bwd_kernel(NormArgs p) {
     typedef Row<T, RW, NCH> R;
     constexpr int W = R::NT * NCH * 8;                         // columns a row's threads cover
-    // Rows in flight: two, where three waves per SIMD still hold them (32 x 1499 x 1024: 149 us with one row and two waves, 121 with two rows and three;
-    // one wave per row, 512 channels: 123 us with one, 270 with two and the spills of three waves).
+    // Rows in flight: two, where three waves per SIMD still hold them (32 x 1499 x 1024: 169 us with one row and two waves, 156 with one and three, 143 with two and three;
+    // one wave per row, 32 x 2998 x 512: 127 us with one row, 270 with two and the spills of three waves).
     constexpr int AHEAD = RW == 1 || RW == 16 ? 1 : 2;
     __shared__ float2 red[2][RW];
     __shared__ __align__(16) float par[4][W];                  // scale, pw, pb, w (1, 1, 0, 1 where there is none); then the waves' column sums

@@ -135,7 +135,7 @@ template <int NS, int T_, int N_> A8_DEV float bc_at(const float (&v)[NS]) { ret
 
 // The scan of one chunk, from the state that the chunks before it leave.  Bound by VALU issue: a state takes a multiply, an exp2 (two issue slots), a
 // multiply and two multiply-adds, 24 cycles for 64 channels, and a (frame, channel) about 160 for softplus, silu, conversions and the sum over waves.
-// bf16, N = 16, gated, states saved for the backward: 16 x 999 x 2048 175 us (524e6 states: 3.0e12 / s, VALU busy 77 % of the cycles, 0.39 GB at 2.2 TB/s),
+// bf16, N = 16, gated, states saved for the backward: 16 x 999 x 2048 180 us (524e6 states: 2.9e12 / s, VALU busy 78 % of the cycles, 0.39 GB at 2.2 TB/s),
 // 8 x 781 x 1536 86 us (192 blocks leave a quarter of the CUs idle; chunks would cost what they win).
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs p) {
     constexpr int NS = FNS, EP = TT / NW, BC = NS * NW;
@@ -226,7 +226,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void
 }
 
 // Each chunk's own end state (from zero) and the sum of its steps.  No output per frame, so the shared memory holds two tiles: while one is walked the
-// next one is staged and the one after it requested, with one barrier per tile (1 x 48001 x 1536: 278 us; as the kernel above without its output, two
+// next one is staged and the one after it requested, with one barrier per tile (1 x 48001 x 1536: 260 .. 278 us, VALU busy 88 %; as the kernel above without its output, two
 // barriers, 340 us.  The kernel above gains nothing from the same form: its sums over states then allow only tiles of 8 frames, 97 us against 86 at
 // 8 x 781 x 1536).
 template <typename T, int NW> __global__ __launch_bounds__(64 * NW) void scan_ends_kernel(ScanArgs p) {
@@ -334,8 +334,8 @@ A8_DEV float rows_sum_scatter4(const float (&v)[4]) {           // row r: the su
 
 // The gradient of one chunk, from the adjoint that the chunks behind it leave; tiles run backwards, each from its saved state.  Bound by VALU issue: per
 // state the recurrence again (24 cycles), the adjoint with its five products (32), and its share of the two sums over channels (17); 256 registers and
-// 76 KB of LDS allow two blocks of 16 states on a CU, two waves per SIMD.  bf16, N = 16, gated: 16 x 999 x 2048 450 us (1.2e12 states / s, VALU busy
-// 71 %), 8 x 781 x 1536 153 + 37 us in 8 chunks.
+// 76 KB of LDS allow two blocks of 16 states on a CU, two waves per SIMD.  bf16, N = 16, gated: 16 x 999 x 2048 465 us (1.1e12 states / s, VALU busy
+// 78 %), 8 x 781 x 1536 150 + 37 us in 8 chunks.
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void scan_bwd_kernel(ScanArgs p) {
     constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dxs[2][TT][CH];                    // {D, D u}, by tile parity
