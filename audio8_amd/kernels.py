@@ -678,9 +678,14 @@ def _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, what):
         rows = 1 if gate.dim() == 3 and gate.shape[1] == T else 0
         _act("gate", gate, (B, T if rows else 1, Cn), dtype)
         g0, g1, _ = gate.stride()
+    ldx, ldo = _rows_ld("x", x), _rows_ld("o", o)
+    # Without a gate per utterance the rows are one sequence: the backward's blocks, and with them its workspace, are then as many as the card holds,
+    # not one or more per utterance.
+    if B > 1 and B * T < 1 << 30 and (gate is None or (rows and (T == 1 or g0 == T * g1))):
+        B, T, g1 = 1, B * T, g1 if T > 1 else g0
     P = L.ptr
     return L.ResidualNormDesc(L.RNORM_DESC_SIZE, code, B, T, Cn, NORM_KINDS[kind], 1 if post_w is not None else 0, rows, eps,
-                              x.data_ptr(), _rows_ld("x", x), o.data_ptr(), _rows_ld("o", o), P(gate), g0, g1, P(scale), P(w), P(b), P(post_w), P(post_b))
+                              x.data_ptr(), ldx, o.data_ptr(), ldo, P(gate), g0, g1, P(scale), P(w), P(b), P(post_w), P(post_b))
 
 
 @functools.lru_cache(maxsize=1024)

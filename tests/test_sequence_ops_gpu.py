@@ -293,6 +293,36 @@ def test_gated_residual_norm_one_output_used_and_two_axes():
             check(use + " d" + k, got[k].reshape(ref["d" + k].shape), ref["d" + k], mag["d" + k], 4 * (C / 32 + 40) + T)
 
 
+@pytest.mark.parametrize("case", [(7, 1600, 136, "layer", "utterance", True, True, True, True, False), (3, 1700, 640, "rms", "rows", True, True, True, True, True),
+                                  (2, 1201, 1100, "layer", "utterance", True, True, True, True, False), (2, 600, 4104, "layer", "utterance", True, False, True, True, False)], ids=str)
+def test_gated_residual_norm_over_many_rows_per_block(case):
+    test_gated_residual_norm(case, torch.float32)
+
+
+@pytest.mark.parametrize("gate", [None, (4096, 1), (1, 1)])
+def test_norm_backward_of_many_short_utterances_takes_a_bounded_workspace(gate):
+    """4096 utterances of one frame: the workspace follows the card, not the number of utterances."""
+    from audio8_amd import ops
+    B, C = 4096, 256
+    a = dict(x=rnd(B, 1, C, seed=1), o=rnd(B, 1, C, seed=2), w=rnd(C, seed=3), pw=rnd(C, seed=5), scale=rnd(C, seed=8))
+    if gate is not None:
+        a["gate"] = rnd(*gate, C, seed=7)
+    g = {k: cu(t, True) for k, t in a.items()}
+    gt = g["gate"].expand(B, 1, C) if gate is not None else None
+    up = rnd(B, 1, C, seed=9).cuda()
+    r, n = ops.gated_residual_norm(g["x"], g["o"], g["w"], post_weight=g["pw"], gate=gt, scale=g["scale"])
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    # (the gradient of the gate as the operator sees it: torch's own sum over an expanded axis takes eight tensors' memory for its parts)
+    got = dict(zip(g, torch.autograd.grad([r, n], [gt if k == "gate" else t for k, t in g.items()], [up, up])))
+    assert torch.cuda.max_memory_allocated() - before < 6 * up.numel() * 4 + 1536 * 5 * C * 4
+    full = dict(a, gate=a["gate"].expand(B, 1, C) if gate is not None else None, b=None, pb=None)
+    ref, mag = (R.residual_norm(**full, dr=up.cpu(), dn=up.cpu(), mag=m) for m in (False, True))
+    for k in g:
+        check("d" + k, got[k], ref["d" + k], mag["d" + k], 4 * (C / 32 + 40) + B)
+
+
 # ------------------------------------------------------------------------------------------------ empty calls
 def test_no_frames_and_no_utterances():
     from audio8_amd import ops
