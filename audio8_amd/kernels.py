@@ -427,12 +427,12 @@ NORM_KINDS = {"layer": 0, "rms": 1}
 _DT = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 
 
-def _conv_desc(x, w, bias, act, state, lengths, what):
+def _conv_desc(x, w, bias, act, state, lengths, what, step=False):
     if act not in CONV_ACTS:
         raise ValueError(f"a8hip {what}: activation {act!r}, expected None or 'silu'")
-    if x.dim() != 3:
-        raise ValueError(f"a8hip {what}: x has {x.dim()} axes, expected [batch, frames, channels]")
-    B, T, Cn = x.shape
+    if x.dim() != (2 if step else 3):
+        raise ValueError(f"a8hip {what}: x has {x.dim()} axes, expected {'[batch, channels]' if step else '[batch, frames, channels]'}")
+    (B, Cn), T = (x.shape, 1) if step else (x.shape[::2], x.shape[1])
     ws = w.shape
     if len(ws) not in (2, 3) or ws[0] != Cn or (len(ws) == 3 and ws[1] != 1) or not 2 <= ws[-1] <= 4:
         raise ValueError(f"a8hip {what}: weight has shape {tuple(ws)}, expected ({Cn}, taps) or ({Cn}, 1, taps) with 2 to 4 taps")
@@ -441,7 +441,7 @@ def _conv_desc(x, w, bias, act, state, lengths, what):
     code = _DT.get(dtype)
     if code is None:
         code = L.dt(x)
-    bs, ts, cs = x.stride()
+    (bs, cs), ts = (x.stride(), 0) if step else (x.stride()[::2], x.stride(1))
     if cs != 1 and Cn > 1:
         raise RuntimeError("a8hip: x needs contiguous channels")
     _dense("weight", w, ws)
@@ -455,7 +455,7 @@ def causal_conv_fwd(x, w, bias=None, act="silu", state=None, lengths=None, want_
     """x [B,T,C] (channels contiguous, any other strides), w f32 [C,K] or [C,1,K] -> (y [B,T,C], final history [B,K-1,C] or None, descriptor)."""
     d = _conv_desc(x, w, bias, act, state, lengths, "causal_conv_fwd")
     stream = _seq_stream(x, w, bias, state, lengths)
-    y = x.new_empty(x.shape)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     d.y = y.data_ptr()
     out = None
     if want_state:
@@ -489,7 +489,7 @@ def causal_conv_bwd(dy, x, w, bias=None, act="silu", state=None, lengths=None, d
     _dense("dw", dw, w.shape)
     _dense("dbias", dbias, (d.C,))
     stream = _seq_stream(dy, x, dstate_out, dw, dbias)
-    dx = x.new_empty(x.shape)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     d.y = d.state_out = dstate = None
     if want_dstate and d.T == 0:             # no frame: the history is handed on
         dstate = dstate_out.clone() if dstate_out is not None else torch.zeros((d.B, d.K - 1, d.C), device=x.device, dtype=dtype)
@@ -507,35 +507,33 @@ def causal_conv_bwd(dy, x, w, bias=None, act="silu", state=None, lengths=None, d
 
 def causal_conv_step(x, state, w, bias=None, act="silu"):
     """One frame: x [B,C], state [B,K-1,C] (read and updated in place) -> y [B,C]."""
-    if x.dim() != 2:
-        raise ValueError(f"a8hip causal_conv_step: x has {x.dim()} axes, expected [batch, channels]")
     if state is None:
         raise ValueError("a8hip causal_conv_step: a step needs its state")
-    d = _conv_desc(x.unsqueeze(1), w, bias, act, state, None, "causal_conv_step")
+    d = _conv_desc(x, w, bias, act, state, None, "causal_conv_step", True)
     stream = _seq_stream(x, w, bias, state)
-    y = x.new_empty(x.shape)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     d.y, d.state, d.state_out = y.data_ptr(), None, state.data_ptr()
     L.check(L.lib().a8_causal_conv_step(C.byref(d), stream), "a8_causal_conv_step")
     return y
 
 
-def _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, what):
-    if u.dim() != 3:
-        raise ValueError(f"a8hip {what}: u has {u.dim()} axes, expected [batch, frames, channels]")
+def _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, what, step=False):
+    if u.dim() != (2 if step else 3):
+        raise ValueError(f"a8hip {what}: u has {u.dim()} axes, expected {'[batch, channels]' if step else '[batch, frames, channels]'}")
     us = u.shape
-    Bn, T, Dn = us
+    (Bn, Dn), T = (us, 1) if step else (us[::2], us[1])
     if A.dim() != 2 or A.shape[0] != Dn or not 1 <= A.shape[1] <= 32:
         raise ValueError(f"a8hip {what}: A has shape {tuple(A.shape)}, expected ({Dn}, states) with 1 to 32 states")
     N = A.shape[1]
     bs = B.shape
-    if len(bs) != 4 or bs[2] < 1 or Dn % bs[2]:
-        raise ValueError(f"a8hip {what}: B has shape {tuple(bs)}, expected [batch, frames, groups, states] with groups dividing {Dn} channels")
-    G = bs[2]
+    if len(bs) != len(us) + 1 or bs[-2] < 1 or Dn % bs[-2]:
+        raise ValueError(f"a8hip {what}: B has shape {tuple(bs)}, expected [batch, {'' if step else 'frames, '}groups, states] with groups dividing {Dn} channels")
+    G = bs[-2]
     dtype = u.dtype
     code = _DT.get(dtype)
     if code is None:
         code = L.dt(u)
-    want = (Bn, T, G, N)
+    want = (Bn, G, N) if step else (Bn, T, G, N)
     _act("u", u, us, dtype)
     _act("dt", dt, us, dtype)
     _act("z", z, us, dtype)
@@ -546,11 +544,17 @@ def _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, what):
     _dense("dt_bias", dt_bias, (Dn,))
     _dense("state", state, (Bn, Dn, N))
     _dense("lengths", lengths, (Bn,), torch.int32)
-    u0, u1, _ = u.stride()
-    t0, t1, _ = dt.stride()
-    z0, z1 = (0, 0) if z is None else z.stride()[:2]
-    b0, b1, b2, _ = B.stride()
-    c0, c1, c2, _ = Cm.stride()
+    if step:
+        u1 = t1 = z0 = z1 = b1 = c1 = 0
+        u0, t0, (b0, b2, _), (c0, c2, _) = u.stride(0), dt.stride(0), B.stride(), Cm.stride()
+        if z is not None:
+            z0 = z.stride(0)
+    else:
+        u0, u1, _ = u.stride()
+        t0, t1, _ = dt.stride()
+        z0, z1 = (0, 0) if z is None else z.stride()[:2]
+        b0, b1, b2, _ = B.stride()
+        c0, c1, c2, _ = Cm.stride()
     return L.SelectiveScanDesc(L.SCAN_DESC_SIZE, code, Bn, T, Dn, N, G, 1 if softplus else 0, u.data_ptr(), u0, u1, dt.data_ptr(), t0, t1, L.ptr(z), z0, z1,
                                B.data_ptr(), b0, b1, b2, Cm.data_ptr(), c0, c1, c2, A.data_ptr(), L.ptr(D), L.ptr(dt_bias), L.ptr(state), L.ptr(lengths))
 
@@ -570,7 +574,7 @@ def selective_scan_fwd(u, dt, A, B, Cm, D=None, z=None, dt_bias=None, softplus=T
     stream = _seq_stream(u, dt, A, B, Cm, D, z, dt_bias, state, lengths)
     nck, nws = _scan_sizes(d.B, d.T, d.D, d.N, d.G, 0)
     dev = u.device
-    y = u.new_empty(u.shape)
+    y = torch.empty_like(u, memory_format=torch.contiguous_format)
     d.y = y.data_ptr()
     out = ckpt = None
     if want_state:
@@ -627,14 +631,11 @@ def selective_scan_bwd(dy, ckpt, u, dt, A, B, Cm, D=None, z=None, dt_bias=None, 
 
 def selective_scan_step(u, dt, A, B, Cm, state, D=None, z=None, dt_bias=None, softplus=True):
     """One frame: u, dt, z [B,D]; B, Cm [B,G,N]; state f32 [B,D,N] (read and updated in place) -> y [B,D]."""
-    if u.dim() != 2 or B.dim() != 3 or Cm.dim() != 3 or dt.dim() != 2 or (z is not None and z.dim() != 2):
-        raise ValueError("a8hip selective_scan_step: u, dt and z are [batch, channels], B and C [batch, groups, states]")
     if state is None:
         raise ValueError("a8hip selective_scan_step: a step needs its state")
-    d = _scan_desc(u.unsqueeze(1), dt.unsqueeze(1), A, B.unsqueeze(1), Cm.unsqueeze(1), D, z.unsqueeze(1) if z is not None else None, dt_bias,
-                   softplus, state, None, "selective_scan_step")
+    d = _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, None, "selective_scan_step", True)
     stream = _seq_stream(u, dt, A, B, Cm, D, z, dt_bias, state)
-    y = u.new_empty(u.shape)
+    y = torch.empty_like(u, memory_format=torch.contiguous_format)
     d.y, d.h0, d.h_out = y.data_ptr(), None, state.data_ptr()
     L.check(L.lib().a8_selective_scan_step(C.byref(d), stream), "a8_selective_scan_step")
     return y
@@ -702,9 +703,9 @@ def residual_norm_fwd(x, o, w=None, b=None, post_w=None, post_b=None, gate=None,
     stream = _seq_stream(x, o, w, b, post_w, post_b, gate, scale)
     n = stats = None
     if w is not None:
-        n = x.new_empty(x.shape)
+        n = torch.empty_like(x, memory_format=torch.contiguous_format)
         d.n = n.data_ptr()
-    r = x.new_empty(x.shape)
+    r = torch.empty_like(x, memory_format=torch.contiguous_format)
     d.r = r.data_ptr()
     if want_stats:
         stats = torch.empty((4, d.B * d.T), device=x.device, dtype=torch.float32)
@@ -737,7 +738,7 @@ def residual_norm_bwd(dr, dn, stats, x, o, w=None, b=None, post_w=None, post_b=N
         raise ValueError("a8hip residual_norm_bwd: dn without the second norm's weight")
     stream = _seq_stream(dr, dn, stats, x, dw, db, dpost_w, dpost_b, dscale)
     dx, do = x.new_empty((2, *xs)).unbind(0)
-    dgate = x.new_empty(gate.shape) if gate is not None else None
+    dgate = torch.empty_like(gate, memory_format=torch.contiguous_format) if gate is not None else None
     d.r = d.n = None
     d.dr, d.dn, d.dx, d.d_o, d.dgate, d.dw, d.db, d.dpost_w, d.dpost_b, d.dscale = \
         P(dr), P(dn), dx.data_ptr(), do.data_ptr(), P(dgate), P(dw), P(db), P(dpost_w), P(dpost_b), P(dscale)

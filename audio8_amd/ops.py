@@ -522,8 +522,17 @@ def _rows(t):
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _taped(*ts):
+    """Whether the call goes on the tape (whose part of a call is a quarter of a short one)."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _step_only(what, *ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+    if _taped(*ts):
         raise RuntimeError(f"a8hip {what}: a step updates its state in place and has no gradient; call it under torch.no_grad()")
 
 
@@ -555,7 +564,10 @@ def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=
     "silu".  state [B, K - 1, C]: the frames before x (zeros without it).  lengths int32 [B] on the device: frames of each utterance; what lies
     behind is not read, comes out as zero and gets a zero gradient.  return_state: also return the last K - 1 frames of each utterance
     (with `state` in front of short ones), with which the next call or causal_conv_step goes on.  Differentiable in x, weight, bias, state."""
-    y, out = CausalConvFn.apply(_rows(x), weight, bias, state, lengths, activation, return_state)
+    if _taped(x, weight, bias, state):
+        y, out = CausalConvFn.apply(_rows(x), weight, bias, state, lengths, activation, return_state)
+    else:
+        y, out, _ = K.causal_conv_fwd(_rows(x), weight, bias, activation, state, lengths, return_state)
     return (y, out) if return_state else y
 
 
@@ -601,7 +613,10 @@ def selective_scan(u, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=Tru
     Differentiable in everything but lengths; the forward then keeps every 16th frame's states (B Dm N / 16 floats per frame)."""
     if B.dim() == 3 and C.dim() == 3:
         B, C = B.unsqueeze(2), C.unsqueeze(2)
-    y, out = SelectiveScanFn.apply(_rows(u), _rows(dt), A, _rows(B), _rows(C), D, _rows(z), dt_bias, state, lengths, softplus, return_state)
+    if _taped(u, dt, A, B, C, D, z, dt_bias, state):
+        y, out = SelectiveScanFn.apply(_rows(u), _rows(dt), A, _rows(B), _rows(C), D, _rows(z), dt_bias, state, lengths, softplus, return_state)
+    else:
+        y, out, _, _ = K.selective_scan_fwd(_rows(u), _rows(dt), A, _rows(B), _rows(C), D, _rows(z), dt_bias, softplus, state, lengths, return_state)
     return (y, out) if return_state else y
 
 
@@ -656,7 +671,9 @@ def gated_residual_norm(x, o, weight=None, bias=None, *, post_weight=None, post_
         return r[0], n[0] if n is not None else None
     if x.dim() != 3 or o.dim() != 3:
         raise ValueError(f"a8hip gated_residual_norm: x and o have {x.dim()} and {o.dim()} axes, expected [batch, frames, channels]")
-    return GatedResidualNormFn.apply(_even_rows(x), _even_rows(o), weight, bias, post_weight, post_bias, _rows(gate), scale, eps, kind)
+    if _taped(x, o, weight, bias, post_weight, post_bias, gate, scale):
+        return GatedResidualNormFn.apply(_even_rows(x), _even_rows(o), weight, bias, post_weight, post_bias, _rows(gate), scale, eps, kind)
+    return K.residual_norm_fwd(_even_rows(x), _even_rows(o), weight, bias, post_weight, post_bias, _rows(gate), scale, eps, kind)[:2]
 
 
 # ------------------------------------------------------------------ conv feature extractor
