@@ -261,6 +261,7 @@ int conv_check(const a8_causal_conv_desc* d, const char* what) {
     A8_REQUIRE(d != nullptr && d->size == (int)sizeof(a8_causal_conv_desc), "%s: descriptor size %d, expected %d", what, d ? d->size : 0, (int)sizeof(a8_causal_conv_desc));
     A8_REQUIRE(d->dtype == A8_F32 || d->dtype == A8_BF16, "%s: bad dtype %d", what, d->dtype);
     A8_REQUIRE(d->B >= 0 && d->T >= 0 && d->C >= 1 && d->K >= 2 && d->K <= 4, "%s: bad sizes B=%d T=%d C=%d K=%d (2 to 4 taps)", what, d->B, d->T, d->C, d->K);
+    A8_REQUIRE(d->T < (1 << 30), "%s: T = %d is too large", what, d->T);           // (frame indices run up to a block's spans past the end)
     A8_REQUIRE(d->act == A8_CONV_ACT_NONE || d->act == A8_CONV_ACT_SILU, "%s: unknown activation %d", what, d->act);
     A8_REQUIRE(d->w != nullptr, "%s: null weight", what);
     return A8_OK;

@@ -638,6 +638,7 @@ int scan_check(const a8_selective_scan_desc* d, const char* what) {
     A8_REQUIRE(d != nullptr && d->size == (int)sizeof(a8_selective_scan_desc), "%s: descriptor size %d, expected %d", what, d ? d->size : 0, (int)sizeof(a8_selective_scan_desc));
     A8_REQUIRE(d->dtype == A8_F32 || d->dtype == A8_BF16, "%s: bad dtype %d", what, d->dtype);
     A8_REQUIRE(d->B >= 0 && d->T >= 0 && d->D >= 1 && d->N >= 1 && d->N <= 32, "%s: bad sizes B=%d T=%d D=%d N=%d (1 to 32 states)", what, d->B, d->T, d->D, d->N);
+    A8_REQUIRE(d->T < (1 << 30), "%s: T = %d is too large", what, d->T);           // (frame indices run up to three tiles past the end)
     A8_REQUIRE(d->G >= 1 && d->D % d->G == 0, "%s: %d channels do not split into %d groups", what, d->D, d->G);
     A8_REQUIRE(d->A != nullptr, "%s: null A", what);
     return A8_OK;

@@ -117,6 +117,19 @@ def test_entry_points_refuse_bad_descriptors_before_launching():
     assert lib.a8_residual_norm_bwd_workspace(C.byref(r), None) == 1
 
 
+def test_entry_points_refuse_more_frames_than_their_indices_hold():
+    from audio8_amd import _lib as L
+    lib = L.lib()
+    n, m = C.c_int64(), C.c_int64()
+    d, s = L.CausalConvDesc(), L.SelectiveScanDesc()
+    d.size, d.B, d.T, d.C, d.K, d.w = L.CONV_DESC_SIZE, 1, 2 ** 31 - 1, 1, 4, 4096
+    s.size, s.B, s.T, s.D, s.N, s.G, s.A = L.SCAN_DESC_SIZE, 1, 2 ** 31 - 1, 1, 1, 1, 4096
+    for call in (lambda: lib.a8_causal_conv_fwd(C.byref(d), None), lambda: lib.a8_causal_conv_bwd(C.byref(d), None),
+                 lambda: lib.a8_causal_conv_bwd_partial_floats(C.byref(d), C.byref(n)), lambda: lib.a8_selective_scan_fwd(C.byref(s), None),
+                 lambda: lib.a8_selective_scan_bwd(C.byref(s), None), lambda: lib.a8_selective_scan_workspace(C.byref(s), 0, C.byref(m), C.byref(n))):
+        assert call() == 1 and b"too large" in _err(lib)
+
+
 def test_the_python_surface_refuses_wrong_arguments():
     from audio8_amd import ops
     f = lambda *s: torch.zeros(*s)  # noqa: E731
