@@ -335,7 +335,7 @@ A8_DEV float rows_sum_scatter4(const float (&v)[4]) {           // row r: the su
 // The gradient of one chunk, from the adjoint that the chunks behind it leave; tiles run backwards, each from its saved state.  Bound by VALU issue: per
 // state the recurrence again (24 cycles), the adjoint with its five products (32), and its share of the two sums over channels (17); 256 registers and
 // 76 KB of LDS allow two blocks of 16 states on a CU, two waves per SIMD.  bf16, N = 16, gated: 16 x 999 x 2048 465 us (1.1e12 states / s, VALU busy
-// 78 %), 8 x 781 x 1536 150 + 37 us in 8 chunks.
+// 78 %), 8 x 781 x 1536 151 + 35 us in 5 chunks.
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void scan_bwd_kernel(ScanArgs p) {
     constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dxs[2][TT][CH];                    // {D, D u}, by tile parity
@@ -500,7 +500,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >
     }
 }
 
-// The adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps: scan_ends_kernel backwards (8 x 781 x 1536: 37 us of 190).
+// The adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps: scan_ends_kernel backwards (8 x 781 x 1536: 35 us of 186).
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void scan_back_ends_kernel(ScanArgs p) {
     constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dg[2][TT][CH];                     // {D, dout silu(z)}
@@ -643,23 +643,27 @@ int scan_check(const a8_selective_scan_desc* d, const char* what) {
     A8_REQUIRE(d->A != nullptr, "%s: null A", what);
     return A8_OK;
 }
-// Frame chunks.  A launch of n chunks takes ceil-rounds of the blocks that the 256 CUs hold: `part[k - 1]` is the time of a round with k blocks on a
-// CU as a share of a full one, `extra` what the chunks' own ends cost more (forward: 0.7 of the walk itself; 1 leaves near ties to one launch).  Measured, D = 1536 and 781 frames (us, 1 chunk / the count taken here):
-// forward B = 1 85 / 28 (12), B = 4 88 / 62 (8), B = 8 91 / 91 (1; 100 with 4); backward B = 1 256 / 55 (12), B = 4 275 / 119 (12), B = 8 279 / 199 (8);
-// 16 x 999 x 2048 (512 blocks) 180 and 503 with one chunk, 233 and 564 with two.  A chunk has at least 4 tiles: its first loads and its share of
-// the walk over the chunks before it stay small.
+// Frame chunks.  A launch of n chunks takes as many tiles' time as a chunk has tiles, times the rounds of blocks that the 256 CUs hold: `part[k - 1]` is
+// the time of a round with k blocks on a CU as a share of a full one, `extra` what the chunks' own ends (all but one chunk's) cost more, a hundredth per
+// chunk what is left of first loads, partial sums and walks over earlier chunks.  Measured, N = 16 (us with one chunk / with the count taken here):
+//   forward   1 x 781 x 1536 82 / 26 (10), 4 x 781 85 / 57 (7), 8 x 781 89 / 89 (1; with 5: 89), 12 x 781 133 / 127 (7), 16 x 624 110 / 110 (1; with 2: 123),
+//             8 x 999 x 2048 116 / 116 (1; with 3: 131), 16 x 999 180 / 180 (1; with 2: 230)
+//   backward  1 x 781 x 1536 248 / 53 (10), 4 x 781 254 / 114 (5), 8 x 781 263 / 195 (5; with 7: 204), 12 x 781 348 / 279 (7), 16 x 624 288 / 284 (4),
+//             8 x 999 x 2048 341 / 299 (2), 16 x 999 471 / 471 (1; with 2: 538)
+// A chunk has at least 4 tiles.
 int scan_chunks(float blocks, int tiles, const float* part, int resident, float extra) {
     int best = 1;
     float cost = 0.f;
     for (int n = 1; n == 1 || (n <= 32 && n * 4 <= tiles); ++n) {
-        const int per_cu = (int)ceilf(blocks * n / 256.f);
+        const int tpc = cdiv(tiles > 0 ? tiles : 1, n), m = cdiv(tiles > 0 ? tiles : 1, tpc);        // (the chunks that are left when each takes whole tiles)
+        const int per_cu = (int)ceilf(blocks * m / 256.f);
         const int full = per_cu / resident, rest = per_cu % resident;
-        const float c = (full + (rest ? part[rest - 1] : 0.f)) / n * (n > 1 ? 1.f + extra + 0.01f * n : 1.f);
+        const float c = (full + (rest ? part[rest - 1] : 0.f)) * tpc * (m > 1 ? 1.f + extra * (m - 1) / m + 0.01f * m : 1.f);
         if (n == 1 || c < cost) { best = n; cost = c; }
     }
     return best;
 }
-const float FWD_PART[3] = {0.48f, 0.74f, 1.f}, BWD_PART[2] = {0.58f, 1.f};
+const float FWD_PART[3] = {0.44f, 0.74f, 1.f}, BWD_PART[2] = {0.69f, 1.f};
 ScanArgs scan_args(const a8_selective_scan_desc* d, bool backward) {
     ScanArgs p = {};
     p.d = *d;
@@ -667,7 +671,7 @@ ScanArgs scan_args(const a8_selective_scan_desc* d, bool backward) {
     p.tpg = cdiv(p.cpg, CH);
     p.tiles = cdiv(d->T, TT);
     const float blocks = (float)d->B * d->G * p.tpg;         // (in blocks of 16 states: fewer states, shorter blocks)
-    p.chunks = backward ? scan_chunks(blocks * cdiv(d->N, BNS) / 4.f, p.tiles, BWD_PART, 2, 0.13f) : scan_chunks(blocks * cdiv(d->N, FNS) / 8.f, p.tiles, FWD_PART, 3, 1.f);
+    p.chunks = backward ? scan_chunks(blocks * cdiv(d->N, BNS) / 4.f, p.tiles, BWD_PART, 2, 0.3f) : scan_chunks(blocks * cdiv(d->N, FNS) / 8.f, p.tiles, FWD_PART, 3, 0.9f);
     p.tpc = cdiv(p.tiles, p.chunks);
     p.chunks = p.tpc > 0 ? cdiv(p.tiles, p.tpc) : 1;         // (no empty chunks; T = 0: one without tiles)
     return p;
