@@ -39,8 +39,8 @@ A8_DEV void lds_barrier() {
 // minor[i][c]; null targets are skipped.  add = 1 accumulates.  Summed in a fixed order: the same inputs give the same bits.
 struct A8SeqReduce {
     const float* in; int rows, planes, C, np;
-    float* major; float* minor[6];
-    int add_major, add_minor[6];
+    float* major; float* minor[2];
+    int add_major, add_minor[2];
 };
 int a8i_seq_reduce(const A8SeqReduce& r, void* stream);
 

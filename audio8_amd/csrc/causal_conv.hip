@@ -294,6 +294,7 @@ extern "C" int a8_causal_conv_fwd(const a8_causal_conv_desc* d, void* stream) {
     if (int e = conv_check(d, "a8_causal_conv_fwd")) return e;
     if (d->B == 0) return A8_OK;
     A8_REQUIRE((d->x && d->y) || d->T == 0, "a8_causal_conv_fwd: null x or y");
+    A8_REQUIRE(!d->y || d->y != d->x, "a8_causal_conv_fwd: y may not be x");
     A8_REQUIRE(d->state_out == nullptr || d->state_out != d->state, "a8_causal_conv_fwd: state_out may not be the state that is read");
     const bool bf = d->dtype == A8_BF16;
     const int V = conv_vec(d, 4, false) ? 4 : 1;
@@ -316,6 +317,7 @@ extern "C" int a8_causal_conv_bwd(const a8_causal_conv_desc* d, void* stream) {
     if (int e = conv_check(d, "a8_causal_conv_bwd")) return e;
     const int rows = conv_rows(d);
     A8_REQUIRE((d->x && d->dy && d->partials) || rows == 0, "a8_causal_conv_bwd: null x, dy or partials");
+    A8_REQUIRE((!d->dx || (d->dx != d->dy && d->dx != d->x)) && (!d->dstate || d->dstate != d->dstate_out), "a8_causal_conv_bwd: an output may not be an input");
     A8_REQUIRE(d->T > 0 || d->B == 0 || d->dstate == nullptr, "a8_causal_conv_bwd: a history's gradient needs T >= 1");
     if (rows > 0) {
         const bool bf = d->dtype == A8_BF16;

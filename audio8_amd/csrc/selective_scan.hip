@@ -727,6 +727,7 @@ extern "C" int a8_selective_scan_fwd(const a8_selective_scan_desc* d, void* stre
     if (int e = scan_check(d, "a8_selective_scan_fwd")) return e;
     if (d->B == 0) return A8_OK;
     A8_REQUIRE(d->T == 0 || (d->u && d->dt && d->Bm && d->Cm && d->y), "a8_selective_scan_fwd: null u, dt, B, C or y");
+    A8_REQUIRE(!d->h_out || d->h_out != d->h0, "a8_selective_scan_fwd: h_out may not be the state that is read");
     ScanArgs p = scan_args(d, false);
     A8_REQUIRE(scan_blocks(p, p.chunks) < (1 << 21), "a8_selective_scan_fwd: B x D = %d x %d is too large", d->B, d->D);
     A8_REQUIRE(p.chunks == 1 || d->ws, "a8_selective_scan_fwd: null workspace");
@@ -739,6 +740,7 @@ extern "C" int a8_selective_scan_fwd(const a8_selective_scan_desc* d, void* stre
 extern "C" int a8_selective_scan_bwd(const a8_selective_scan_desc* d, void* stream) {
     if (int e = scan_check(d, "a8_selective_scan_bwd")) return e;
     ScanArgs p = scan_args(d, true);
+    A8_REQUIRE(!d->dh0 || d->dh0 != d->dh_out, "a8_selective_scan_bwd: dh0 may not be the gradient that is read");
     A8_REQUIRE(d->B == 0 || d->ws, "a8_selective_scan_bwd: null workspace");
     A8_REQUIRE(d->B == 0 || d->T == 0 || (d->u && d->dt && d->Bm && d->Cm && d->dy && d->ckpt && d->du && d->ddt && d->dBm && d->dCm && (d->dz || !d->z)),
                "a8_selective_scan_bwd: null operand");

@@ -351,7 +351,7 @@ int a8_adamw(float* p, float* g, float* m, float* v, int64_t n, float lr, float 
 
 /* ---- causal sequence operators (streaming encoders): what mixes frames without looking ahead, and the norms around such a block ----
  * Channels-last like everything else: element (b, t, c) of a strided input at b * bs + t * ts + c (strides in elements, channels contiguous:
- * a slice of a wider projection is read in place); outputs are contiguous.  Activations (x, u, dt, z, B, C, o, gate, y ...) are `dtype`;
+ * a slice of a wider projection is read in place); outputs are contiguous and overlap no input (the steps' states excepted).  Activations (x, u, dt, z, B, C, o, gate, y ...) are `dtype`;
  * weights, A, skips, biases, scan states and all parameter gradients are f32.
  * lengths (int32 [B] on the device, or NULL): utterance b has lengths[b] frames (clamped to 0 .. T).  Frames behind its end are not read; their
  * outputs and gradients are zero and the final state is the state at its end.

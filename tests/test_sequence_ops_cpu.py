@@ -130,6 +130,25 @@ def test_entry_points_refuse_more_frames_than_their_indices_hold():
         assert call() == 1 and b"too large" in _err(lib)
 
 
+def test_entry_points_refuse_outputs_that_other_blocks_still_read():
+    from audio8_amd import _lib as L
+    lib = L.lib()
+    d, s = L.CausalConvDesc(), L.SelectiveScanDesc()
+    d.size, d.B, d.T, d.C, d.K, d.w = L.CONV_DESC_SIZE, 1, 4, 8, 4, 4096
+    d.x, d.y = 4096, 4096
+    assert lib.a8_causal_conv_fwd(C.byref(d), None) == 1 and b"y may not be x" in _err(lib)
+    d.dy, d.dx, d.partials = 8192, 8192, 4096
+    assert lib.a8_causal_conv_bwd(C.byref(d), None) == 1 and b"may not be an input" in _err(lib)
+    d.dx, d.dstate, d.dstate_out = 16384, 4096, 4096
+    assert lib.a8_causal_conv_bwd(C.byref(d), None) == 1 and b"may not be an input" in _err(lib)
+    s.size, s.B, s.T, s.D, s.N, s.G, s.A = L.SCAN_DESC_SIZE, 1, 4, 8, 4, 1, 4096
+    s.u = s.dt = s.Bm = s.Cm = s.h0 = s.h_out = 4096
+    s.y = 8192
+    assert lib.a8_selective_scan_fwd(C.byref(s), None) == 1 and b"h_out" in _err(lib)
+    s.dh0 = s.dh_out = 4096
+    assert lib.a8_selective_scan_bwd(C.byref(s), None) == 1 and b"dh0" in _err(lib)
+
+
 def test_the_python_surface_refuses_wrong_arguments():
     from audio8_amd import ops
     f = lambda *s: torch.zeros(*s)  # noqa: E731
