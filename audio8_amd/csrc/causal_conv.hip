@@ -294,8 +294,8 @@ extern "C" int a8_causal_conv_fwd(const a8_causal_conv_desc* d, void* stream) {
     if (int e = conv_check(d, "a8_causal_conv_fwd")) return e;
     if (d->B == 0) return A8_OK;
     A8_REQUIRE((d->x && d->y) || d->T == 0, "a8_causal_conv_fwd: null x or y");
-    A8_REQUIRE(!d->y || d->y != d->x, "a8_causal_conv_fwd: y may not be x");
     A8_REQUIRE(d->state_out == nullptr || d->state_out != d->state, "a8_causal_conv_fwd: state_out may not be the state that is read");
+    A8_REQUIRE(!d->y || d->y != d->x, "a8_causal_conv_fwd: y may not be x");
     const bool bf = d->dtype == A8_BF16;
     const int V = conv_vec(d, 4, false) ? 4 : 1;
     const int cols = cdiv(d->C, 64 * V), quads = conv_quads(d, FWD_SPAN);
