@@ -9,6 +9,7 @@ import time
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import kernels as K
@@ -523,7 +524,7 @@ def _rows(t):
 
 
 def _taped(*ts):
-    """Whether the call goes on the tape (whose part of a call is a quarter of a short one)."""
+    """Whether the tape records the call."""
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
@@ -531,9 +532,19 @@ def _taped(*ts):
     return False
 
 
+def _applied(*ts):
+    """Whether the call goes through its autograd function, whose part of a call is a quarter of a short one: where the tape records it, and where
+    torch knows of the call by its function alone, which forward mode refuses and a trace records (of the launch itself they see nothing)."""
+    return _taped(*ts) or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+
+
 def _step_only(what, *ts):
     if _taped(*ts):
         raise RuntimeError(f"a8hip {what}: a step updates its state in place and has no gradient; call it under torch.no_grad()")
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"a8hip {what}: a step cannot be traced")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError(f"a8hip {what}: a step has no forward-mode gradient")
 
 
 class CausalConvFn(torch.autograd.Function):
@@ -564,7 +575,7 @@ def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=
     "silu".  state [B, K - 1, C]: the frames before x (zeros without it).  lengths int32 [B] on the device: frames of each utterance; what lies
     behind is not read, comes out as zero and gets a zero gradient.  return_state: also return the last K - 1 frames of each utterance
     (with `state` in front of short ones), with which the next call or causal_conv_step goes on.  Differentiable in x, weight, bias, state."""
-    if _taped(x, weight, bias, state):
+    if _applied(x, weight, bias, state):
         y, out = CausalConvFn.apply(_rows(x), weight, bias, state, lengths, activation, return_state)
     else:
         y, out, _ = K.causal_conv_fwd(_rows(x), weight, bias, activation, state, lengths, return_state)
@@ -613,7 +624,7 @@ def selective_scan(u, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=Tru
     Differentiable in everything but lengths; the forward then keeps every 16th frame's states (B Dm N / 16 floats per frame)."""
     if B.dim() == 3 and C.dim() == 3:
         B, C = B.unsqueeze(2), C.unsqueeze(2)
-    if _taped(u, dt, A, B, C, D, z, dt_bias, state):
+    if _applied(u, dt, A, B, C, D, z, dt_bias, state):
         y, out = SelectiveScanFn.apply(_rows(u), _rows(dt), A, _rows(B), _rows(C), D, _rows(z), dt_bias, state, lengths, softplus, return_state)
     else:
         y, out, _, _ = K.selective_scan_fwd(_rows(u), _rows(dt), A, _rows(B), _rows(C), D, _rows(z), dt_bias, softplus, state, lengths, return_state)
@@ -671,7 +682,7 @@ def gated_residual_norm(x, o, weight=None, bias=None, *, post_weight=None, post_
         return r[0], n[0] if n is not None else None
     if x.dim() != 3 or o.dim() != 3:
         raise ValueError(f"a8hip gated_residual_norm: x and o have {x.dim()} and {o.dim()} axes, expected [batch, frames, channels]")
-    if _taped(x, o, weight, bias, post_weight, post_bias, gate, scale):
+    if _applied(x, o, weight, bias, post_weight, post_bias, gate, scale):
         return GatedResidualNormFn.apply(_even_rows(x), _even_rows(o), weight, bias, post_weight, post_bias, _rows(gate), scale, eps, kind)
     return K.residual_norm_fwd(_even_rows(x), _even_rows(o), weight, bias, post_weight, post_bias, _rows(gate), scale, eps, kind)[:2]
 

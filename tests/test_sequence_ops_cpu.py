@@ -190,3 +190,55 @@ def test_the_python_surface_refuses_wrong_arguments():
         ops.gated_residual_norm(f(1, 1, 8200), f(1, 1, 8200), f(8200))
     with pytest.raises(RuntimeError, match="GPU"):
         ops.gated_residual_norm(x, x, f(8))
+
+
+# ------------------------------------------------------------------------------------------------ what torch does with a call by its function
+def _stand_ins(monkeypatch):
+    """The launches replaced by plain copies: y (r, n) = 2 x, whatever the operator."""
+    from audio8_amd import kernels as K
+
+    def twice(x):
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y.detach().numpy()[...] = 2 * x.detach().numpy()
+        return y
+    monkeypatch.setattr(K, "causal_conv_fwd", lambda x, *a: (twice(x), None, None))
+    monkeypatch.setattr(K, "selective_scan_fwd", lambda u, *a: (twice(u), None, None, None))
+    monkeypatch.setattr(K, "residual_norm_fwd", lambda x, *a: (twice(x), twice(x), None, None))
+    monkeypatch.setattr(K, "causal_conv_step", lambda x, *a: twice(x))
+    monkeypatch.setattr(K, "selective_scan_step", lambda u, *a: twice(u))
+
+
+def _calls():
+    from audio8_amd import ops
+    w, A, v = rnd(8, 4, seed=1).float(), rnd(8, 4, seed=2).float(), rnd(8, seed=3).float()
+    return [lambda x: ops.causal_conv(x, w), lambda x: ops.selective_scan(x, x, A, x[..., :4], x[..., :4]), lambda x: ops.gated_residual_norm(x, x, v)[1]]
+
+
+def _steps():
+    from audio8_amd import ops
+    w, A = rnd(8, 4, seed=1).float(), rnd(8, 4, seed=2).float()
+    return [lambda x: ops.causal_conv_step(x, torch.zeros(2, 3, 8), w), lambda x: ops.selective_scan_step(x, x, A, x[:, :4], x[:, :4], torch.zeros(2, 8, 4))]
+
+
+@pytest.mark.parametrize("recording", [False, True])
+def test_a_forward_mode_gradient_is_refused_and_not_dropped(monkeypatch, recording):
+    import torch.autograd.forward_ad as fw
+    _stand_ins(monkeypatch)
+    with torch.set_grad_enabled(recording), fw.dual_level():
+        for call, x in [(c, rnd(2, 5, 8, seed=4).float()) for c in _calls()] + [(c, rnd(2, 8, seed=4).float()) for c in _steps()]:
+            with pytest.raises(NotImplementedError):
+                call(fw.make_dual(x, torch.ones_like(x)))
+            assert torch.equal(call(x), 2 * x)             # without a tangent it is a call like any other
+
+
+@pytest.mark.parametrize("recording", [False, True])
+def test_a_trace_holds_the_operator_and_no_step(monkeypatch, recording):
+    _stand_ins(monkeypatch)
+    with torch.set_grad_enabled(recording):
+        for call in _calls():
+            traced = torch.jit.trace(call, (rnd(2, 5, 8, seed=4).float(),), check_trace=False)
+            x = rnd(2, 5, 8, seed=5).float()
+            assert torch.equal(traced(x), 2 * x)
+        for step in _steps():
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(step, (rnd(2, 8, seed=4).float(),), check_trace=False)

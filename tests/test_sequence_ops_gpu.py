@@ -675,3 +675,16 @@ def test_offsets_past_32_bits():
         # frames before the tail see the tail's gradient through the recurrence and the taps, not the other way round; the scan's frame chunks differ
         assert torch.allclose(dx[:, -tail:].float(), ds.float(), rtol=2.0 ** -7, atol=2.0 ** -14 * float(ds.abs().max()))
         del y, up, dx
+
+
+def test_a_trace_runs_the_operators():
+    from audio8_amd import ops
+    w, A, v = rnd(16, 4, seed=1).cuda(), -rnd(16, 4, seed=2).exp().cuda(), rnd(16, seed=3).cuda()
+
+    def f(x):
+        y = ops.selective_scan(ops.causal_conv(x, w), x, A, x[..., :4].contiguous(), x[..., 4:8].contiguous())
+        return ops.gated_residual_norm(x, y, v)[1]
+    traced = torch.jit.trace(f, (rnd(2, 5, 16, seed=4).cuda(),), check_trace=False)
+    for B, T in ((2, 5), (3, 40)):
+        x = rnd(B, T, 16, seed=5).cuda()
+        assert torch.equal(traced(x), f(x))
