@@ -130,6 +130,23 @@ def test_entry_points_refuse_more_frames_than_their_indices_hold():
         assert call() == 1 and b"too large" in _err(lib)
 
 
+@pytest.mark.parametrize("n", [2 ** 31, 2 ** 32, 2 ** 32 + 5])
+def test_the_python_surface_refuses_sizes_that_a_descriptor_does_not_hold(n):
+    """C ints hold 31 bits: 2^32 + 5 frames would become 5 (views of one element: nothing is allocated)."""
+    from audio8_amd import ops
+    one = torch.ones(1)
+    for B, T in ((1, n), (n, 1)):
+        x, bc = one.expand(B, T, 1), one.expand(B, T, 1, 1)
+        for call in (lambda: ops.causal_conv(x, torch.ones(1, 4)), lambda: ops.selective_scan(x, x, torch.ones(1, 1), bc, bc), lambda: ops.gated_residual_norm(x, x, one)):
+            with pytest.raises(ValueError, match="too large"):
+                call()
+    x = one.expand(n, 1)
+    with pytest.raises(ValueError, match="too large"):
+        ops.causal_conv_step(x, one.expand(n, 3, 1), torch.ones(1, 4))
+    with pytest.raises(ValueError, match="too large"):
+        ops.selective_scan_step(x, x, torch.ones(1, 1), one.expand(n, 1, 1), one.expand(n, 1, 1), one.expand(n, 1, 1))
+
+
 def test_entry_points_refuse_outputs_that_other_blocks_still_read():
     from audio8_amd import _lib as L
     lib = L.lib()
