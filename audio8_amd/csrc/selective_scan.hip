@@ -130,6 +130,12 @@ template <int I> A8_DEV void row_axpy(float (&x)[4], float v, float g) {
         "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
         : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]) : "v"(v), "v"(g), "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3));
 }
+// What a chunk makes of the state (adjoint) in front of it: exp2(x) v plus its own end e.  The factor of a whole chunk may be beyond f32 where the product is
+// not (growing states, with a silent beginning or behind a chunk that decays): it is applied in two halves, and a state of zero stays zero.
+A8_DEV float carry(float x, float v, float e) {
+    const float f = __builtin_amdgcn_exp2f(0.5f * x);
+    return v == 0.f ? e : fmaf(f, f * v, e);
+}
 // element (t, n) of wave_bc's values
 template <int NS, int T_, int N_> A8_DEV float bc_at(const float (&v)[NS]) { return row_value<(T_ % (16 / NS)) * NS + N_>(v[T_ / (16 / NS)]); }
 
@@ -159,7 +165,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void
         const float s = e[(int64_t)d.N * d.D];
 #pragma unroll
         for (int n = 0; n < NS; ++n)
-            if (n0 + n < d.N) h[n] = fmaf(__builtin_amdgcn_exp2f(A2[n] * s), h[n], e[(int64_t)(n0 + n) * d.D]);
+            if (n0 + n < d.N) h[n] = carry(A2[n] * s, h[n], e[(int64_t)(n0 + n) * d.D]);
     }
     TileRegs<T, NW, NS, Z, false> nx, cu;                  // the next tile's inputs, this tile's u and z
     auto stage = [&](int t0) {                             // nx -> LDS
@@ -361,7 +367,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >
         const float s = e[(int64_t)d.N * d.D];
 #pragma unroll
         for (int n = 0; n < NS; ++n)
-            if (n0 + n < d.N && w.live) c[n] = fmaf(__builtin_amdgcn_exp2f(A2[n] * s), c[n], e[(int64_t)(n0 + n) * d.D]);
+            if (n0 + n < d.N && w.live) c[n] = carry(A2[n] * s, c[n], e[(int64_t)(n0 + n) * d.D]);
     }
     float dskip = 0.f, dbias = 0.f;
     TileRegs<T, NW, NS, Z, true> nx, cu;
