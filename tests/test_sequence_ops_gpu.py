@@ -688,3 +688,56 @@ def test_a_trace_runs_the_operators():
     for B, T in ((2, 5), (3, 40)):
         x = rnd(B, T, 16, seed=5).cuda()
         assert torch.equal(traced(x), f(x))
+
+
+def test_steps_in_inference_mode_give_the_definition():
+    from audio8_amd import ops
+    B, D, N, K = 3, 40, 5, 4
+    a = dict(u=rnd(B, 1, D, seed=1), dt=rnd(B, 1, D, seed=2), A=-rnd(D, N, seed=3).exp(), B=rnd(B, 1, 1, N, seed=4), C=rnd(B, 1, 1, N, seed=5), state=rnd(B, D, N, seed=6))
+    w, hist = rnd(D, K, seed=7), rnd(B, K - 1, D, seed=8)
+    with torch.inference_mode():
+        g, c = {k: v.cuda() for k, v in a.items()}, hist.cuda()
+        x = ops.causal_conv_step(g["u"][:, 0], c, w.cuda())
+        y = ops.selective_scan_step(x, g["dt"][:, 0], g["A"], g["B"][:, 0], g["C"][:, 0], g["state"])
+    ref, mag = (R.conv(a["u"], w, state=hist, mag=m) for m in (False, True))
+    check("x", x[:, None], ref["y"], mag["y"], K + 12)
+    assert torch.equal(c.cpu().double(), ref["state"])
+    ref, mag = (R.scan(**{**a, "u": x.cpu()[:, None]}, mag=m) for m in (False, True))
+    check("y", y[:, None], ref["y"], mag["y"], 16 + 40 + N)
+    check("state", g["state"], ref["state"], mag["state"], 16 + 40)
+
+
+@pytest.mark.parametrize("op", ["conv", "scan", "norm"])
+def test_offsets_past_32_bits_against_the_definition(op):
+    """The last frames of 1.1 million frames x 2048 channels, whose offsets pass 2^31 elements: silence before them leaves conv and scan at rest."""
+    from audio8_amd import ops
+    T, C, K, N, tail = 1_100_000, 2048, 4, 4, 80
+    x, bc = rnd(1, tail, C, seed=1, dtype=torch.bfloat16), rnd(1, tail, N, seed=5, dtype=torch.bfloat16)
+    w, A, g = rnd(C, K, seed=2), -rnd(C, N, seed=3).exp(), rnd(C, seed=4)
+    xl = torch.zeros(1, T, C, device="cuda", dtype=torch.bfloat16)
+    xl[:, -tail:] = x.cuda()
+    xl.requires_grad_()
+    bl = torch.zeros(1, T, N, device="cuda", dtype=torch.bfloat16)
+    bl[:, -tail:] = bc.cuda()
+    y = {"conv": lambda: ops.causal_conv(xl, w.cuda()), "scan": lambda: ops.selective_scan(xl, xl, A.cuda(), bl, bl),
+         "norm": lambda: ops.gated_residual_norm(xl, xl, g.cuda(), post_weight=g.cuda(), gate=xl)[1]}[op]()
+    up = torch.zeros_like(y)
+    up[:, -tail:] = 1
+    (dx,) = torch.autograd.grad(y, [xl], [up])
+    one, b4 = torch.ones(1, tail, C), bc[:, :, None]
+    for m in (False, True):
+        if op == "conv":
+            o = R.conv(x, w, dy=one, mag=m)
+            res = o["y"], o["dx"]
+        elif op == "scan":
+            o = R.scan(x, x, A, b4, b4, dy=one, mag=m)
+            res = o["y"], o["du"], o["ddt"]
+        else:
+            o = R.residual_norm(x, x, w=g, pw=g, gate=x, dn=one, mag=m)
+            res = o["n"], o["dx"], o["do"], o["dgate"]
+        ref, mag = (res, None) if not m else (ref, res)
+    F = {"conv": 2 * K + 12, "scan": 16 * tail + 40 + N, "norm": 4 * (C / 32 + 40)}[op]
+    check("y", y[:, -tail:], ref[0], mag[0], 2 * F)
+    # x is several of the arguments: each gradient is rounded to bf16, and so is each sum of two
+    parts = sum(v.abs() for v in ref[1:])
+    check("dx", dx[:, -tail:], sum(ref[1:]), sum(mag[1:]) + parts.max() * len(ref) * 2.0 ** 16 / F, F)
