@@ -259,3 +259,20 @@ def test_a_trace_holds_the_operator_and_no_step(monkeypatch, recording):
         for step in _steps():
             with pytest.raises(RuntimeError, match="traced"):
                 torch.jit.trace(step, (rnd(2, 8, seed=4).float(),), check_trace=False)
+
+
+def test_a_step_refuses_to_drop_a_parameters_gradient(monkeypatch):
+    from audio8_amd import ops
+    _stand_ins(monkeypatch)
+    x, bc = rnd(2, 8, seed=1).float(), rnd(2, 4, seed=2).float()
+    conv = dict(weight=rnd(8, 4, seed=3).float(), bias=rnd(8, seed=4).float())
+    scan = dict(A=rnd(8, 4, seed=5).float(), D=rnd(8, seed=6).float(), dt_bias=rnd(8, seed=7).float())
+    for par, step in ((conv, lambda p: ops.causal_conv_step(x, torch.zeros(2, 3, 8), **p)),
+                      (scan, lambda p: ops.selective_scan_step(x, x, B=bc, C=bc, state=torch.zeros(2, 8, 4), **p))):
+        assert torch.equal(step(par), 2 * x)
+        for k, v in par.items():
+            learnt = {**par, k: v.clone().requires_grad_()}
+            with pytest.raises(RuntimeError, match="no gradient"):
+                step(learnt)
+            with torch.no_grad():
+                assert torch.equal(step(learnt), 2 * x)
