@@ -494,17 +494,18 @@ extern "C" int a8_residual_norm_bwd_workspace(const a8_residual_norm_desc* d, in
 extern "C" int a8_residual_norm_bwd(const a8_residual_norm_desc* d, void* stream) {
     if (int e = norm_check(d, "a8_residual_norm_bwd")) return e;
     const NormArgs p = norm_args(d);
-    const int blocks = d->B * p.chunks;
+    const int blocks = d->B * p.chunks, threads = d->C <= 512 ? 256 : d->C <= 1024 ? 128 : d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024;
+    const int64_t sums = 2 * cdiv(d->C, 16) + (d->gate && !d->gate_rows ? ((int64_t)d->B * d->C + 1023) / 1024 : 0);
+    // (a grid holds less than 2^32 threads; a gate per utterance takes a block per utterance, and a thread per element of its gradient)
+    A8_REQUIRE((int64_t)blocks * threads < (1ll << 32) && sums * 1024 < (1ll << 32), "a8_residual_norm_bwd: B x T x C = %d x %d x %d is too large", d->B, d->T, d->C);
     if (blocks > 0) {
         A8_REQUIRE(d->x && d->o && d->dx && d->d_o && d->ws && (d->dgate || !d->gate) && (d->stats || !(d->post || d->dn)) && (d->w || !d->dn),
                    "a8_residual_norm_bwd: null operand");
         auto kernel = d->dtype == A8_BF16 ? (p.vec ? NORM_GATE(bf16, true) : NORM_GATE(bf16, false)) : (p.vec ? NORM_GATE(float, true) : NORM_GATE(float, false));
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(d->C <= 512 ? 256 : d->C <= 1024 ? 128 : d->C <= 2048 ? 256 : d->C <= 4096 ? 512 : 1024), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, (hipStream_t)stream, p);
         if (int e = a8_check_launch("a8_residual_norm_bwd")) return e;
     }
-    A8_REQUIRE((int64_t)d->B * d->C < (1 << 30), "a8_residual_norm_bwd: B x C = %d x %d is too large", d->B, d->C);
-    const int gate_blocks = d->gate && !d->gate_rows ? cdiv((int64_t)d->B * d->C, 1024) : 0;
-    const dim3 grid(2 * cdiv(d->C, 16) + gate_blocks);
+    const dim3 grid((unsigned)sums);
     if (d->dtype == A8_BF16) hipLaunchKernelGGL(rnorm_reduce_kernel<bf16>, grid, dim3(1024), 0, (hipStream_t)stream, *d, blocks, p.chunks);
     else hipLaunchKernelGGL(rnorm_reduce_kernel<float>, grid, dim3(1024), 0, (hipStream_t)stream, *d, blocks, p.chunks);
     return a8_check_launch("a8_residual_norm_bwd");

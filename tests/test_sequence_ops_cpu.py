@@ -147,6 +147,18 @@ def test_the_python_surface_refuses_sizes_that_a_descriptor_does_not_hold(n):
         ops.selective_scan_step(x, x, torch.ones(1, 1), one.expand(n, 1, 1), one.expand(n, 1, 1), one.expand(n, 1, 1))
 
 
+@pytest.mark.parametrize("B, T, width", [(2 ** 24 + 1, 2, 8), (2 ** 22, 1, 1024), (2 ** 25 + 1, 1, 1024)])
+def test_norm_backward_refuses_grids_beyond_the_launch_limit_before_it_launches(B, T, width):
+    """A gate per utterance: a block per utterance in the backward, a thread per element of the gate's gradient behind it."""
+    from audio8_amd import _lib as L
+    lib = L.lib()
+    r = L.ResidualNormDesc()
+    r.size, r.B, r.T, r.C = L.RNORM_DESC_SIZE, B, T, width
+    r.x = r.o = r.gate = r.w = r.dr = r.dn = r.dx = r.d_o = r.dgate = r.stats = r.ws = 4096
+    r.x_ld = r.o_ld = r.g_bs = width
+    assert lib.a8_residual_norm_bwd(C.byref(r), None) == 1 and b"too large" in _err(lib)
+
+
 def test_entry_points_refuse_outputs_that_other_blocks_still_read():
     from audio8_amd import _lib as L
     lib = L.lib()
