@@ -29,15 +29,14 @@ template <typename T, int V> A8_DEV void stv(T* p, const float (&o)[V]) {
     *reinterpret_cast<W*>(p) = w;
 }
 
-// block -> columns of V channels, utterance, first frame; the column of a lane past the width is the last one (its results are dropped)
-struct Place { int c, b, t0, len; bool on; int64_t row; };
-template <int V, int SPAN> A8_DEV Place place(const a8_causal_conv_desc& d, int cols, int quads) {
+// block and row of spans (quads per utterance) -> columns of V channels, utterance, first frame; the column of a lane past the width is the last one (its results are dropped)
+struct Place { int c, b, t0, len; bool on; };
+template <int V, int SPAN> A8_DEV Place place(const a8_causal_conv_desc& d, int cols, int quads, int64_t row) {
     Place q;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int cb = blockIdx.x % cols;
-    q.row = blockIdx.x / cols;
-    q.b = (int)(q.row / quads);
-    q.t0 = ((int)(q.row % quads) * 4 + wv) * SPAN;
+    q.b = (int)(row / quads);
+    q.t0 = ((int)(row % quads) * 4 + wv) * SPAN;
     const int c = (cb * 64 + lane) * V;
     q.on = c < d.C;
     q.c = q.on ? c : d.C - V;
@@ -55,7 +54,7 @@ template <typename T, int V> A8_DEV void conv_in(float (&o)[V], const a8_causal_
 }
 
 template <typename T, int K, int V> __global__ __launch_bounds__(256) void conv_fwd_kernel(a8_causal_conv_desc d, int cols, int quads) {
-    const Place q = place<V, FWD_SPAN>(d, cols, quads);
+    const Place q = place<V, FWD_SPAN>(d, cols, quads, blockIdx.x / cols);
     if (q.t0 >= d.T && !(q.t0 == 0)) return;                   // (a whole wave)
     float w[K][V], bias[V], e[K - 1][V];
 #pragma unroll
@@ -105,102 +104,107 @@ template <typename T, int K, int V> __global__ __launch_bounds__(256) void conv_
         }
 }
 
-template <typename T, int K, int V> __global__ __launch_bounds__(256) void conv_bwd_kernel(a8_causal_conv_desc d, int cols, int quads) {
+// MANY: more rows of spans than blocks per column, which walk them in turn (a template parameter: as one kernel, 64 x 781 x 1536 took 123 us against 107)
+template <typename T, int K, int V, bool MANY> __global__ __launch_bounds__(256) void conv_bwd_kernel(a8_causal_conv_desc d, int cols, int quads, int64_t items) {
     __shared__ float red[4][K + 1][64 * V];
-    const Place q = place<V, BWD_SPAN>(d, cols, quads);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool silu = d.act == A8_CONV_ACT_SILU;
+    const int slot = blockIdx.x / cols, slots = gridDim.x / cols;
     float dw[K][V] = {}, db[V] = {};
-    if (q.t0 < d.T) {
-        const int t1 = min(q.t0 + BWD_SPAN, d.T);
-        float w[K][V], bias[V], e[K][V], g[K][V] = {};         // e[k], g[k]: input and gradient before the activation of frame t - (K - 1) + k
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            bias[i] = d.bias ? d.bias[q.c + i] : 0.f;
-#pragma unroll
-            for (int k = 0; k < K; ++k) w[k][i] = d.w[(int64_t)(q.c + i) * K + k];
-        }
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k) conv_in<T, V>(e[k + 1], d, q, q.t0 + k);
-        const T* const xp = (const T*)d.x + (q.b * d.x_bs + q.c);
-        const T* const dp = (const T*)d.dy + (q.b * d.dy_bs + q.c);
-        T* const dx = (T*)d.dx + (int64_t)q.b * d.T * d.C + q.c;
-        auto frame = [&](int t, const float (&x)[V], const float (&dy)[V], bool own, bool valid) {
+    for (int64_t row = slot; !MANY || row < items; row += slots) {
+        const Place q = place<V, BWD_SPAN>(d, cols, quads, row);
+        if (q.t0 < d.T) {
+            const int t1 = min(q.t0 + BWD_SPAN, d.T);
+            float w[K][V], bias[V], e[K][V], g[K][V] = {};         // e[k], g[k]: input and gradient before the activation of frame t - (K - 1) + k
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                bias[i] = d.bias ? d.bias[q.c + i] : 0.f;
 #pragma unroll
-                for (int k = 0; k < K - 1; ++k) { e[k][i] = e[k + 1][i]; g[k][i] = g[k + 1][i]; }
-                e[K - 1][i] = x[i];
-                float pre = bias[i];
-#pragma unroll
-                for (int k = 0; k < K; ++k) pre = fmaf(w[k][i], e[k][i], pre);
-                const float gt = valid ? (silu ? dy[i] * silu_grad_f(pre) : dy[i]) : 0.f;
-                g[K - 1][i] = gt;
-                if (own) {
-                    db[i] += gt;
-#pragma unroll
-                    for (int k = 0; k < K; ++k) dw[k][i] = fmaf(gt, e[k][i], dw[k][i]);
-                }
+                for (int k = 0; k < K; ++k) w[k][i] = d.w[(int64_t)(q.c + i) * K + k];
             }
-        };
-        auto emit = [&](int tx) {                              // the input gradient of frame tx, whose last tap was just taken in
-            float de[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                de[i] = 0.f;
+            for (int k = 0; k < K - 1; ++k) conv_in<T, V>(e[k + 1], d, q, q.t0 + k);
+            const T* const xp = (const T*)d.x + (q.b * d.x_bs + q.c);
+            const T* const dp = (const T*)d.dy + (q.b * d.dy_bs + q.c);
+            T* const dx = (T*)d.dx + (int64_t)q.b * d.T * d.C + q.c;
+            auto frame = [&](int t, const float (&x)[V], const float (&dy)[V], bool own, bool valid) {
 #pragma unroll
-                for (int k = 0; k < K; ++k) de[i] = fmaf(w[K - 1 - k][i], g[k][i], de[i]);
-            }
-            if (d.dstate_out && tx < q.len && tx >= q.len - (K - 1)) {
-                float ds[V];
-                ldv<T, V>(ds, (const T*)d.dstate_out + ((int64_t)q.b * (K - 1) + tx + (K - 1) - q.len) * d.C + q.c);
+                for (int i = 0; i < V; ++i) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) de[i] += ds[i];
-            }
-            if (tx >= q.len)
+                    for (int k = 0; k < K - 1; ++k) { e[k][i] = e[k + 1][i]; g[k][i] = g[k + 1][i]; }
+                    e[K - 1][i] = x[i];
+                    float pre = bias[i];
 #pragma unroll
-                for (int i = 0; i < V; ++i) de[i] = 0.f;
-            if (q.on && d.dx) stv<T, V>(dx + (int64_t)tx * d.C, de);
-        };
-        // g runs K - 1 frames past the span's end; the input gradient lags it by as many
-        auto slow = [&](int t) {
-            float x[V] = {}, dy[V] = {};
-            const bool valid = t < q.len;
-            if (valid) { ldv<T, V>(x, xp + t * d.x_ts); ldv<T, V>(dy, dp + t * d.dy_ts); }
-            frame(t, x, dy, t < t1, valid);
-            if (t - q.t0 >= K - 1) emit(t - (K - 1));
-        };
-        int t = q.t0;
-        for (; t < min(q.t0 + K - 1, t1 + K - 1); ++t) slow(t);
-        for (; t + 4 <= min(t1, q.len); t += 4) {              // four frames' loads in flight
-            float x[4][V], dy[4][V];
+                    for (int k = 0; k < K; ++k) pre = fmaf(w[k][i], e[k][i], pre);
+                    const float gt = valid ? (silu ? dy[i] * silu_grad_f(pre) : dy[i]) : 0.f;
+                    g[K - 1][i] = gt;
+                    if (own) {
+                        db[i] += gt;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) { ldv<T, V>(x[s], xp + (t + s) * d.x_ts); ldv<T, V>(dy[s], dp + (t + s) * d.dy_ts); }
-#pragma unroll
-            for (int s = 0; s < 4; ++s) { frame(t + s, x[s], dy[s], true, true); emit(t + s - (K - 1)); }
-        }
-        for (; t < t1 + K - 1; ++t) slow(t);
-    }
-    if (q.t0 == 0 && q.on && d.dstate)                         // the history's gradient: e indexes 0 .. K - 2, read by frames t <= j at tap j - t
-        for (int j = 0; j < K - 1; ++j)
-            for (int i = 0; i < V; ++i) {
-                const int c = q.c + i;
-                float de = 0.f;
-                for (int t = 0; t <= min(j, q.len - 1); ++t) {
-                    float pre = d.bias ? d.bias[c] : 0.f;
-                    for (int k = 0; k < K; ++k) {
-                        const int f = t + k - (K - 1);
-                        const float v = f >= 0 ? to_f(((const T*)d.x)[q.b * d.x_bs + f * d.x_ts + c])
-                                               : d.state ? to_f(((const T*)d.state)[((int64_t)q.b * (K - 1) + t + k) * d.C + c]) : 0.f;
-                        pre = fmaf(d.w[(int64_t)c * K + k], v, pre);
+                        for (int k = 0; k < K; ++k) dw[k][i] = fmaf(gt, e[k][i], dw[k][i]);
                     }
-                    float gt = to_f(((const T*)d.dy)[q.b * d.dy_bs + t * d.dy_ts + c]);
-                    if (silu) gt *= silu_grad_f(pre);
-                    de = fmaf(d.w[(int64_t)c * K + j - t], gt, de);
                 }
-                if (d.dstate_out && j >= q.len) de += to_f(((const T*)d.dstate_out)[((int64_t)q.b * (K - 1) + j - q.len) * d.C + c]);
-                ((T*)d.dstate)[((int64_t)q.b * (K - 1) + j) * d.C + c] = from_f<T>(de);
+            };
+            auto emit = [&](int tx) {                              // the input gradient of frame tx, whose last tap was just taken in
+                float de[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    de[i] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) de[i] = fmaf(w[K - 1 - k][i], g[k][i], de[i]);
+                }
+                if (d.dstate_out && tx < q.len && tx >= q.len - (K - 1)) {
+                    float ds[V];
+                    ldv<T, V>(ds, (const T*)d.dstate_out + ((int64_t)q.b * (K - 1) + tx + (K - 1) - q.len) * d.C + q.c);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) de[i] += ds[i];
+                }
+                if (tx >= q.len)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) de[i] = 0.f;
+                if (q.on && d.dx) stv<T, V>(dx + (int64_t)tx * d.C, de);
+            };
+            // g runs K - 1 frames past the span's end; the input gradient lags it by as many
+            auto slow = [&](int t) {
+                float x[V] = {}, dy[V] = {};
+                const bool valid = t < q.len;
+                if (valid) { ldv<T, V>(x, xp + t * d.x_ts); ldv<T, V>(dy, dp + t * d.dy_ts); }
+                frame(t, x, dy, t < t1, valid);
+                if (t - q.t0 >= K - 1) emit(t - (K - 1));
+            };
+            int t = q.t0;
+            for (; t < min(q.t0 + K - 1, t1 + K - 1); ++t) slow(t);
+            for (; t + 4 <= min(t1, q.len); t += 4) {              // four frames' loads in flight
+                float x[4][V], dy[4][V];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) { ldv<T, V>(x[s], xp + (t + s) * d.x_ts); ldv<T, V>(dy[s], dp + (t + s) * d.dy_ts); }
+#pragma unroll
+                for (int s = 0; s < 4; ++s) { frame(t + s, x[s], dy[s], true, true); emit(t + s - (K - 1)); }
             }
+            for (; t < t1 + K - 1; ++t) slow(t);
+        }
+        if (q.t0 == 0 && q.on && d.dstate)                         // the history's gradient: e indexes 0 .. K - 2, read by frames t <= j at tap j - t
+            for (int j = 0; j < K - 1; ++j)
+                for (int i = 0; i < V; ++i) {
+                    const int c = q.c + i;
+                    float de = 0.f;
+                    for (int t = 0; t <= min(j, q.len - 1); ++t) {
+                        float pre = d.bias ? d.bias[c] : 0.f;
+                        for (int k = 0; k < K; ++k) {
+                            const int f = t + k - (K - 1);
+                            const float v = f >= 0 ? to_f(((const T*)d.x)[q.b * d.x_bs + f * d.x_ts + c])
+                                                   : d.state ? to_f(((const T*)d.state)[((int64_t)q.b * (K - 1) + t + k) * d.C + c]) : 0.f;
+                            pre = fmaf(d.w[(int64_t)c * K + k], v, pre);
+                        }
+                        float gt = to_f(((const T*)d.dy)[q.b * d.dy_bs + t * d.dy_ts + c]);
+                        if (silu) gt *= silu_grad_f(pre);
+                        de = fmaf(d.w[(int64_t)c * K + j - t], gt, de);
+                    }
+                    if (d.dstate_out && j >= q.len) de += to_f(((const T*)d.dstate_out)[((int64_t)q.b * (K - 1) + j - q.len) * d.C + c]);
+                    ((T*)d.dstate)[((int64_t)q.b * (K - 1) + j) * d.C + c] = from_f<T>(de);
+                }
+        if constexpr (!MANY) break;
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
@@ -211,7 +215,7 @@ template <typename T, int K, int V> __global__ __launch_bounds__(256) void conv_
     const int c0 = (blockIdx.x % cols) * 64 * V;
     for (int i = threadIdx.x; i < (K + 1) * 64 * V; i += 256) {
         const int p = i / (64 * V), l = i % (64 * V);
-        if (c0 + l < d.C) d.partials[(q.row * (K + 1) + p) * d.C + c0 + l] = (red[0][p][l] + red[1][p][l]) + (red[2][p][l] + red[3][p][l]);
+        if (c0 + l < d.C) d.partials[((int64_t)slot * (K + 1) + p) * d.C + c0 + l] = (red[0][p][l] + red[1][p][l]) + (red[2][p][l] + red[3][p][l]);
     }
 }
 
@@ -279,9 +283,18 @@ bool conv_vec(const a8_causal_conv_desc* d, int V, bool backward) {
     }
     return ok;
 }
-#define CONV_TAPS(KERNEL, T, V) (d->K == 2 ? (KERNEL<T, 2, V>) : d->K == 3 ? (KERNEL<T, 3, V>) : (KERNEL<T, 4, V>))
+#define CONV_FWD(T, V) (d->K == 2 ? (conv_fwd_kernel<T, 2, V>) : d->K == 3 ? (conv_fwd_kernel<T, 3, V>) : (conv_fwd_kernel<T, 4, V>))
+#define CONV_BWD(T, V, MANY) (d->K == 2 ? (conv_bwd_kernel<T, 2, V, MANY>) : d->K == 3 ? (conv_bwd_kernel<T, 3, V, MANY>) : (conv_bwd_kernel<T, 4, V, MANY>))
 int conv_quads(const a8_causal_conv_desc* d, int span) { return cdiv(d->T > 0 ? d->T : 1, 4 * span); }        // blocks along an utterance (T = 0 still hands the history on)
-int conv_rows(const a8_causal_conv_desc* d) { return d->T > 0 ? d->B * conv_quads(d, BWD_SPAN) : 0; }
+// The backward's rows of spans, and the blocks per column that walk them: one each (8 x 781: 56), unless that is more than eight per CU and their partial
+// sums (K + 1 floats per channel) would be more than twice the frames themselves, as with many utterances of a few frames; then as many as keep them
+// below the frames (4096 x 1 x 1536: 126 -> 12 MB, 79 + 7 us against 76 + 39; 4096 x 8 x 768 stays at one each: 84 + 20 us against 113 + 17).
+int64_t conv_items(const a8_causal_conv_desc* d) { return d->T > 0 ? (int64_t)d->B * conv_quads(d, BWD_SPAN) : 0; }
+int conv_slots(const a8_causal_conv_desc* d) {
+    const int cols = cdiv(d->C, 64);
+    const int64_t most = std::max<int64_t>(cdiv(4096, cols), (int64_t)d->B * d->T / (2 * (d->K + 1)));
+    return (int)std::min(conv_items(d) <= 2 * most ? conv_items(d) : most, (int64_t)std::max(1, (1 << 23) / cols));
+}
 
 }  // namespace
 
@@ -300,8 +313,8 @@ extern "C" int a8_causal_conv_fwd(const a8_causal_conv_desc* d, void* stream) {
     const int V = conv_vec(d, 4, false) ? 4 : 1;
     const int cols = cdiv(d->C, 64 * V), quads = conv_quads(d, FWD_SPAN);
     A8_REQUIRE((int64_t)cols * d->B * quads < (1 << 24), "a8_causal_conv_fwd: B x T x C = %d x %d x %d is too large", d->B, d->T, d->C);
-    auto kernel = bf ? (V == 4 ? CONV_TAPS(conv_fwd_kernel, bf16, 4) : CONV_TAPS(conv_fwd_kernel, bf16, 1))
-                     : (V == 4 ? CONV_TAPS(conv_fwd_kernel, float, 4) : CONV_TAPS(conv_fwd_kernel, float, 1));
+    auto kernel = bf ? (V == 4 ? CONV_FWD(bf16, 4) : CONV_FWD(bf16, 1))
+                     : (V == 4 ? CONV_FWD(float, 4) : CONV_FWD(float, 1));
     hipLaunchKernelGGL(kernel, dim3(cols * d->B * quads), dim3(256), 0, (hipStream_t)stream, *d, cols, quads);
     return a8_check_launch("a8_causal_conv_fwd");
 }
@@ -309,13 +322,13 @@ extern "C" int a8_causal_conv_fwd(const a8_causal_conv_desc* d, void* stream) {
 extern "C" int a8_causal_conv_bwd_partial_floats(const a8_causal_conv_desc* d, int64_t* floats) {
     if (int e = conv_check(d, "a8_causal_conv_bwd_partial_floats")) return e;
     A8_REQUIRE(floats != nullptr, "a8_causal_conv_bwd_partial_floats: null result");
-    *floats = (int64_t)conv_rows(d) * (d->K + 1) * d->C;
+    *floats = (int64_t)conv_slots(d) * (d->K + 1) * d->C;
     return A8_OK;
 }
 
 extern "C" int a8_causal_conv_bwd(const a8_causal_conv_desc* d, void* stream) {
     if (int e = conv_check(d, "a8_causal_conv_bwd")) return e;
-    const int rows = conv_rows(d);
+    const int rows = conv_slots(d);
     A8_REQUIRE((d->x && d->dy && d->partials) || rows == 0, "a8_causal_conv_bwd: null x, dy or partials");
     A8_REQUIRE((!d->dx || (d->dx != d->dy && d->dx != d->x)) && (!d->dstate || d->dstate != d->dstate_out), "a8_causal_conv_bwd: an output may not be an input");
     A8_REQUIRE(d->T > 0 || d->B == 0 || d->dstate == nullptr, "a8_causal_conv_bwd: a history's gradient needs T >= 1");
@@ -323,10 +336,10 @@ extern "C" int a8_causal_conv_bwd(const a8_causal_conv_desc* d, void* stream) {
         const bool bf = d->dtype == A8_BF16;
         const int V = conv_vec(d, 2, true) ? 2 : 1;
         const int cols = cdiv(d->C, 64 * V), quads = conv_quads(d, BWD_SPAN);
-        A8_REQUIRE((int64_t)cols * rows < (1 << 24), "a8_causal_conv_bwd: B x T x C = %d x %d x %d is too large", d->B, d->T, d->C);
-        auto kernel = bf ? (V == 2 ? CONV_TAPS(conv_bwd_kernel, bf16, 2) : CONV_TAPS(conv_bwd_kernel, bf16, 1))
-                         : (V == 2 ? CONV_TAPS(conv_bwd_kernel, float, 2) : CONV_TAPS(conv_bwd_kernel, float, 1));
-        hipLaunchKernelGGL(kernel, dim3(cols * rows), dim3(256), 0, (hipStream_t)stream, *d, cols, quads);
+        const bool many = conv_items(d) > rows;
+        auto kernel = many ? (bf ? (V == 2 ? CONV_BWD(bf16, 2, true) : CONV_BWD(bf16, 1, true)) : (V == 2 ? CONV_BWD(float, 2, true) : CONV_BWD(float, 1, true)))
+                           : (bf ? (V == 2 ? CONV_BWD(bf16, 2, false) : CONV_BWD(bf16, 1, false)) : (V == 2 ? CONV_BWD(float, 2, false) : CONV_BWD(float, 1, false)));
+        hipLaunchKernelGGL(kernel, dim3(cols * rows), dim3(256), 0, (hipStream_t)stream, *d, cols, quads, conv_items(d));
         if (int e = a8_check_launch("a8_causal_conv_bwd")) return e;
     }
     A8SeqReduce r = {d->partials, rows, d->K + 1, d->C, d->K, d->dw, {d->dbias}, d->add_dw, {d->add_dbias}};

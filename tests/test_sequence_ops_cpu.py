@@ -159,6 +159,16 @@ def test_norm_backward_refuses_grids_beyond_the_launch_limit_before_it_launches(
     assert lib.a8_residual_norm_bwd(C.byref(r), None) == 1 and b"too large" in _err(lib)
 
 
+@pytest.mark.parametrize("B, T", [(4096, 1), (2 ** 20, 1), (2 ** 26, 2 ** 13), (1, 1), (8, 781), (1, 2 ** 30 - 1)])
+def test_conv_backward_partial_sums_follow_the_frames(B, T):
+    """At most the size of x or 8192 blocks' partial sums (64 channels each), and never fewer than one block's."""
+    from audio8_amd import _lib as L
+    n, d = C.c_int64(), L.CausalConvDesc()
+    d.size, d.B, d.T, d.C, d.K, d.w = L.CONV_DESC_SIZE, B, T, 1536, 4, 4096
+    assert L.lib().a8_causal_conv_bwd_partial_floats(C.byref(d), C.byref(n)) == 0
+    assert 5 * 1536 <= n.value <= 2 * max(4096 * 64 * 5 + 5 * 1536, B * T * 1536 // 2)
+
+
 def test_entry_points_refuse_outputs_that_other_blocks_still_read():
     from audio8_amd import _lib as L
     lib = L.lib()

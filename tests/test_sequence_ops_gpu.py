@@ -741,3 +741,31 @@ def test_offsets_past_32_bits_against_the_definition(op):
     # x is several of the arguments: each gradient is rounded to bf16, and so is each sum of two
     parts = sum(v.abs() for v in ref[1:])
     check("dx", dx[:, -tail:], sum(ref[1:]), sum(mag[1:]) + parts.max() * len(ref) * 2.0 ** 16 / F, F)
+
+
+def test_conv_backward_of_many_short_utterances_takes_a_bounded_workspace():
+    """4096 utterances of one frame: partial sums follow the frames, not the number of utterances.  Rounding: 10 utterances summed in a block, the waves
+    and the blocks' sums behind them (below 100), with the magnitude of an element's own terms."""
+    from audio8_amd import ops
+    B, C, K = 4096, 768, 4
+    x, w, b, state = rnd(B, 1, C, seed=1), rnd(C, K, seed=2), rnd(C, seed=3), rnd(B, K - 1, C, seed=4)
+    dy, dst = rnd(B, 1, C, seed=5), rnd(B, K - 1, C, seed=6)
+    g = [cu(t, True) for t in (x, w, b, state)]
+    up = dy.cuda(), dst.cuda()
+    y, out = ops.causal_conv(g[0], g[1], g[2], state=g[3], return_state=True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = torch.autograd.grad([y, out], g, up)
+    assert torch.cuda.max_memory_allocated() - before < (1 + K - 1 + 1) * x.numel() * 4 + 2 ** 20      # dx, dstate, partial sums as large as x at most
+    ref, mag = (R.conv(x, w, b, state=state, dy=dy, dstate_out=dst, mag=m) for m in (False, True))
+    for k, v in zip(("dx", "dw", "dbias", "dstate"), got):
+        F = K + 12 + (K if k in ("dx", "dstate") else 110)
+        assert ((v.double().cpu() - ref[k]).abs() <= 2.0 ** -24 * (ref[k].abs() + F * mag[k])).all(), k
+
+
+@pytest.mark.parametrize("case", [(5000, 3, 130, 4, "silu", True, [3, 0, 1, 2] * 1250, True), (9000, 1, 64, 2, None, False, None, False), (2000, 5, 257, 3, "silu", True, [5, 2] * 1000, False)],
+                         ids=lambda c: str(c[:6]))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_causal_conv_of_many_short_utterances(case, dtype):
+    test_causal_conv(case, dtype)
