@@ -42,6 +42,7 @@ struct A8SeqReduce {
     float* major; float* minor[2];
     int add_major, add_minor[2];
 };
+constexpr int SEQ_REDUCE_MAX = 1 << 26;      // C stays below: a block of 1024 threads per 16 columns, a grid of less than 2^32 (callers refuse before they launch)
 int a8i_seq_reduce(const A8SeqReduce& r, void* stream);
 
 // a descriptor's frame count of utterance b: lengths[b] clamped to [0, T]

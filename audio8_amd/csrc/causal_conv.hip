@@ -328,6 +328,7 @@ extern "C" int a8_causal_conv_bwd_partial_floats(const a8_causal_conv_desc* d, i
 
 extern "C" int a8_causal_conv_bwd(const a8_causal_conv_desc* d, void* stream) {
     if (int e = conv_check(d, "a8_causal_conv_bwd")) return e;
+    A8_REQUIRE(d->C < SEQ_REDUCE_MAX, "a8_causal_conv_bwd: C = %d is too large", d->C);
     const int rows = conv_slots(d);
     A8_REQUIRE((d->x && d->dy && d->partials) || rows == 0, "a8_causal_conv_bwd: null x, dy or partials");
     A8_REQUIRE((!d->dx || (d->dx != d->dy && d->dx != d->x)) && (!d->dstate || d->dstate != d->dstate_out), "a8_causal_conv_bwd: an output may not be an input");

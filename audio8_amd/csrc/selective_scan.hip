@@ -746,6 +746,7 @@ extern "C" int a8_selective_scan_fwd(const a8_selective_scan_desc* d, void* stre
 extern "C" int a8_selective_scan_bwd(const a8_selective_scan_desc* d, void* stream) {
     if (int e = scan_check(d, "a8_selective_scan_bwd")) return e;
     ScanArgs p = scan_args(d, true);
+    A8_REQUIRE(d->D < SEQ_REDUCE_MAX, "a8_selective_scan_bwd: D = %d is too large", d->D);
     A8_REQUIRE(!d->dh0 || d->dh0 != d->dh_out, "a8_selective_scan_bwd: dh0 may not be the gradient that is read");
     A8_REQUIRE(d->B == 0 || d->ws, "a8_selective_scan_bwd: null workspace");
     A8_REQUIRE(d->B == 0 || d->T == 0 || (d->u && d->dt && d->Bm && d->Cm && d->dy && d->ckpt && d->du && d->ddt && d->dBm && d->dCm && (d->dz || !d->z)),

@@ -169,6 +169,17 @@ def test_conv_backward_partial_sums_follow_the_frames(B, T):
     assert 5 * 1536 <= n.value <= 2 * max(4096 * 64 * 5 + 5 * 1536, B * T * 1536 // 2)
 
 
+def test_backwards_refuse_more_channels_than_their_column_sums_take_before_they_launch():
+    from audio8_amd import _lib as L
+    lib = L.lib()
+    d, s = L.CausalConvDesc(), L.SelectiveScanDesc()
+    d.size, d.B, d.T, d.C, d.K, d.w, d.x, d.dy, d.dx, d.partials = L.CONV_DESC_SIZE, 1, 1, 2 ** 26, 4, 4096, 4096, 8192, 16384, 4096
+    assert lib.a8_causal_conv_bwd(C.byref(d), None) == 1 and b"too large" in _err(lib)
+    s.size, s.B, s.T, s.D, s.N, s.G, s.A = L.SCAN_DESC_SIZE, 1, 1, 2 ** 26, 1, 1, 4096
+    s.u = s.dt = s.Bm = s.Cm = s.dy = s.ckpt = s.du = s.ddt = s.dBm = s.dCm = s.ws = 4096
+    assert lib.a8_selective_scan_bwd(C.byref(s), None) == 1 and b"too large" in _err(lib)
+
+
 def test_entry_points_refuse_outputs_that_other_blocks_still_read():
     from audio8_amd import _lib as L
     lib = L.lib()
