@@ -130,6 +130,11 @@ template <int I> A8_DEV void row_axpy(float (&x)[4], float v, float g) {
         "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n\tv_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
         : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]) : "v"(v), "v"(g), "n"(I), "n"(I + 1), "n"(I + 2), "n"(I + 3));
 }
+// A as exp2 takes it, kept finite where A is -inf or its product is: a step of zero (frames behind the end) leaves such a state as it is, 0 x inf does not.
+A8_DEV float log2_rate(float A) {
+    const float r = A * SEQ_LOG2E;
+    return r < -3.4028235e38f ? -3.4028235e38f : r;
+}
 // What a chunk makes of the state (adjoint) in front of it: exp2(x) v plus its own end e.  The factor of a whole chunk may be beyond f32 where the product is
 // not (growing states, with a silent beginning or behind a chunk that decays): it is applied in two halves, and a state of zero stays zero.
 A8_DEV float carry(float x, float v, float e) {
@@ -157,7 +162,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const bool has = n0 + n < d.N;
-        A2[n] = has ? d.A[(int64_t)w.ch * d.N + n0 + n] * SEQ_LOG2E : 0.f;
+        A2[n] = has ? log2_rate(d.A[(int64_t)w.ch * d.N + n0 + n]) : 0.f;
         h[n] = has && d.h0 ? d.h0[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
     }
     for (int k = 0; k < w.ck; ++k) {                       // the states that the chunks before leave: at most a few dozen, each two loads away
@@ -246,7 +251,7 @@ template <typename T, int NW> __global__ __launch_bounds__(64 * NW) void scan_en
     const bool sp = d.softplus != 0;
     float A2[NS], h[NS] = {}, sum = 0.f;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) A2[n] = n0 + n < d.N ? d.A[(int64_t)w.ch * d.N + n0 + n] * SEQ_LOG2E : 0.f;
+    for (int n = 0; n < NS; ++n) A2[n] = n0 + n < d.N ? log2_rate(d.A[(int64_t)w.ch * d.N + n0 + n]) : 0.f;
     TileRegs<T, NW, NS, false, false> nx;
     auto stage = [&](int i) {                              // (the tile behind the chunk's last one is staged like any other, and neither walked nor summed)
 #pragma unroll
@@ -359,7 +364,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >
     for (int n = 0; n < NS; ++n) {
         const bool has = n0 + n < d.N;
         A[n] = has ? d.A[(int64_t)w.ch * d.N + n0 + n] : 0.f;
-        A2[n] = A[n] * SEQ_LOG2E;
+        A2[n] = log2_rate(A[n]);
         c[n] = has && w.live && d.dh_out ? d.dh_out[((int64_t)w.b * d.D + w.ch) * d.N + n0 + n] : 0.f;
     }
     for (int k = p.chunks - 1; k > w.ck; --k) {            // the adjoint that the chunks behind leave
@@ -518,7 +523,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void
     const bool sp = d.softplus != 0;
     float A2[NS], c[NS] = {}, sum = 0.f;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) A2[n] = n0 + n < d.N ? d.A[(int64_t)w.ch * d.N + n0 + n] * SEQ_LOG2E : 0.f;
+    for (int n = 0; n < NS; ++n) A2[n] = n0 + n < d.N ? log2_rate(d.A[(int64_t)w.ch * d.N + n0 + n]) : 0.f;
     TileRegs<T, NW, NS, Z, true> nx;
     auto load = [&](int i) { nx.load(d, w, wv, max(i, 0) * TT); };
     auto stage = [&](int i) {                              // (the tile in front of the chunk's first one is neither walked nor summed)

@@ -769,3 +769,17 @@ def test_conv_backward_of_many_short_utterances_takes_a_bounded_workspace():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_causal_conv_of_many_short_utterances(case, dtype):
     test_causal_conv(case, dtype)
+
+
+@pytest.mark.parametrize("T", [5, 30, 600])
+def test_a_state_that_decays_at_once(T):
+    """A = -inf keeps nothing of a state from one frame to the next; frames behind an utterance's end (steps of zero) leave it as it is."""
+    from audio8_amd import ops
+    case = (3, T, 70, 16, 1, True, True, True, True, [T, T // 2, 0], False)
+    a, n = scan_inputs(case, torch.float32)
+    a["A"][:, 3], a["A"][::3, 11] = -3.0e38, -float("inf")
+    g = {k: v.cuda() for k, v in a.items()}
+    y, out = ops.selective_scan(*(g[k] for k in ("u", "dt", "A", "B", "C")), **{k: g[k] for k in ("D", "z", "dt_bias", "state")}, lengths=cu(n), return_state=True)
+    ref, mag = (R.scan(**a, lengths=n, mag=m) for m in (False, True))
+    check("y", y, ref["y"], mag["y"], 16 * T + 40 + 16)
+    check("state", out, ref["state"], mag["state"], 16 * T + 40)
