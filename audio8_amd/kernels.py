@@ -394,11 +394,11 @@ def gelu_bwd_bias(dy, z, dbias):
 # replacement may even lie at the old address): these calls are short, and the host's share of them counts.
 def _seq_stream(*ts):
     """The current stream of the current device, on which every tensor of the call has to live."""
-    dev = torch.cuda.current_device() if torch.cuda.is_initialized() else None
+    dev = None
     for t in ts:
         if t is not None and t.get_device() != dev:
-            L.require_cuda(t)
-            dev = torch.cuda.current_device()
+            L.require_cuda(t)              # (from here on the runtime is up, which torch.cuda.current_device() would ask every time)
+            dev = torch._C._cuda_getDevice()
             if t.get_device() != dev:
                 raise RuntimeError(f"a8hip: a tensor lives on cuda:{t.get_device()}, the current device is cuda:{dev}")
     return torch._C._cuda_getCurrentRawStream(dev)
@@ -422,10 +422,11 @@ def _dense(name, t, shape, dtype=torch.float32):
     raise RuntimeError(f"a8hip: {name} has to be contiguous")
 
 
-def _fits(what, *sizes):
-    """Sizes are C ints in the descriptors, and ctypes cuts off what does not fit without a word."""
-    if max(sizes) > 0x7FFFFFFF:
-        raise ValueError(f"a8hip {what}: sizes {' x '.join(str(int(n)) for n in sizes)} are too large")
+_INT_MAX = 0x7FFFFFFF      # sizes are C ints in the descriptors, and ctypes cuts off what does not fit without a word
+
+
+def _too_large(what, *sizes):
+    raise ValueError(f"a8hip {what}: sizes {' x '.join(str(int(n)) for n in sizes)} are too large")
 
 
 CONV_ACTS = {None: 0, "silu": 1}
@@ -439,7 +440,8 @@ def _conv_desc(x, w, bias, act, state, lengths, what, step=False):
     if x.dim() != (2 if step else 3):
         raise ValueError(f"a8hip {what}: x has {x.dim()} axes, expected {'[batch, channels]' if step else '[batch, frames, channels]'}")
     (B, Cn), T = (x.shape, 1) if step else (x.shape[::2], x.shape[1])
-    _fits(what, B, T, Cn)
+    if B > _INT_MAX or T > _INT_MAX or Cn > _INT_MAX:
+        _too_large(what, B, T, Cn)
     ws = w.shape
     if len(ws) not in (2, 3) or ws[0] != Cn or (len(ws) == 3 and ws[1] != 1) or not 2 <= ws[-1] <= 4:
         raise ValueError(f"a8hip {what}: weight has shape {tuple(ws)}, expected ({Cn}, taps) or ({Cn}, 1, taps) with 2 to 4 taps")
@@ -529,7 +531,8 @@ def _scan_desc(u, dt, A, B, Cm, D, z, dt_bias, softplus, state, lengths, what, s
         raise ValueError(f"a8hip {what}: u has {u.dim()} axes, expected {'[batch, channels]' if step else '[batch, frames, channels]'}")
     us = u.shape
     (Bn, Dn), T = (us, 1) if step else (us[::2], us[1])
-    _fits(what, Bn, T, Dn)
+    if Bn > _INT_MAX or T > _INT_MAX or Dn > _INT_MAX:
+        _too_large(what, Bn, T, Dn)
     if A.dim() != 2 or A.shape[0] != Dn or not 1 <= A.shape[1] <= 32:
         raise ValueError(f"a8hip {what}: A has shape {tuple(A.shape)}, expected ({Dn}, states) with 1 to 32 states")
     N = A.shape[1]
@@ -668,7 +671,8 @@ def _rnorm_desc(x, o, w, b, post_w, post_b, gate, scale, eps, kind, what):
     if x.dim() != 3:
         raise ValueError(f"a8hip {what}: x has {x.dim()} axes, expected [batch, frames, channels]")
     B, T, Cn = x.shape
-    _fits(what, B, T)
+    if B > _INT_MAX or T > _INT_MAX:
+        _too_large(what, B, T, Cn)
     if not 1 <= Cn <= 8192:
         raise ValueError(f"a8hip {what}: {Cn} channels, expected 1 to 8192")
     if (b is not None and w is None) or (post_b is not None and post_w is None):

@@ -532,16 +532,19 @@ def _taped(*ts):
     return False
 
 
+_tracing = torch._C._get_tracing_state
+
+
 def _applied(*ts):
     """Whether the call goes through its autograd function, whose part of a call is a quarter of a short one: where the tape records it, and where
     torch knows of the call by its function alone, which forward mode refuses and a trace records (of the launch itself they see nothing)."""
-    return _taped(*ts) or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+    return _taped(*ts) or forward_ad._current_level >= 0 or _tracing() is not None
 
 
 def _step_only(what, *ts):
     if _taped(*ts):
         raise RuntimeError(f"a8hip {what}: a step updates its state in place and has no gradient; call it under torch.no_grad()")
-    if torch._C._get_tracing_state() is not None:
+    if _tracing() is not None:
         raise RuntimeError(f"a8hip {what}: a step cannot be traced")
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         raise NotImplementedError(f"a8hip {what}: a step has no forward-mode gradient")
