@@ -9,7 +9,7 @@
 // Bound by HBM.  A row is held in registers, 8 consecutive channels per lane and round, by one wave (forward up to 1024 channels, backward up to 512),
 // by two (backward up to 1024) or by a block: every tensor is read and written once, statistics are exact two-pass in f32.  The backward walks many
 // rows, the next row's loads in flight, the parameters in LDS, the column sums in registers.  bf16, both norms, a gate per utterance:
-// 32 x 1499 x 1024 forward 81 us (393 MB, 4.8 TB/s), backward 142 us (589 MB, 4.1 TB/s), parameter gradients 13 us.
+// 32 x 1499 x 1024 forward 83 us (393 MB, 4.8 TB/s), backward 142 us (589 MB, 4.1 TB/s), parameter gradients 13 us.
 #include "a8_seq.h"
 #include "a8hip_internal.h"
 

@@ -147,7 +147,7 @@ template <int NS, int T_, int N_> A8_DEV float bc_at(const float (&v)[NS]) { ret
 // The scan of one chunk, from the state that the chunks before it leave.  Bound by VALU issue: a state takes a multiply, an exp2 (two issue slots), a
 // multiply and two multiply-adds, 24 cycles for 64 channels, and a (frame, channel) about 160 for softplus, silu, conversions and the sum over waves.
 // bf16, N = 16, gated, states saved for the backward: 16 x 999 x 2048 180 us (524e6 states: 2.9e12 / s, VALU busy 78 % of the cycles, 0.39 GB at 2.2 TB/s),
-// 8 x 781 x 1536 86 us (192 blocks leave a quarter of the CUs idle; chunks would cost what they win).
+// 8 x 781 x 1536 85 us (192 blocks leave a quarter of the CUs idle; chunks would cost what they win).
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs p) {
     constexpr int NS = FNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dx[TT][CH];                        // {D, D u}
@@ -237,8 +237,8 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void
 }
 
 // Each chunk's own end state (from zero) and the sum of its steps.  No output per frame, so the shared memory holds two tiles: while one is walked the
-// next one is staged and the one after it requested, with one barrier per tile (1 x 48001 x 1536: 260 .. 278 us, VALU busy 88 %; as the kernel above without its output, two
-// barriers, 340 us.  The kernel above gains nothing from the same form: its sums over states then allow only tiles of 8 frames, 97 us against 86 at
+// next one is staged and the one after it requested, with one barrier per tile (1 x 48001 x 1536: 250 .. 278 us, VALU busy 88 %; as the kernel above without its output, two
+// barriers, 340 us.  The kernel above gains nothing from the same form: its sums over states then allow only tiles of 8 frames, 97 us against 86 in one session at
 // 8 x 781 x 1536).
 template <typename T, int NW> __global__ __launch_bounds__(64 * NW) void scan_ends_kernel(ScanArgs p) {
     constexpr int NS = FNS, EP = TT / NW, BC = NS * NW;
@@ -345,8 +345,8 @@ A8_DEV float rows_sum_scatter4(const float (&v)[4]) {           // row r: the su
 
 // The gradient of one chunk, from the adjoint that the chunks behind it leave; tiles run backwards, each from its saved state.  Bound by VALU issue: per
 // state the recurrence again (24 cycles), the adjoint with its five products (32), and its share of the two sums over channels (17); 256 registers and
-// 76 KB of LDS allow two blocks of 16 states on a CU, two waves per SIMD.  bf16, N = 16, gated: 16 x 999 x 2048 465 us (1.1e12 states / s, VALU busy
-// 78 %), 8 x 781 x 1536 151 + 35 us in 5 chunks.
+// 76 KB of LDS allow two blocks of 16 states on a CU, two waves per SIMD.  bf16, N = 16, gated: 16 x 999 x 2048 457 us (1.1e12 states / s, VALU busy
+// 78 %), 8 x 781 x 1536 142 + 33 us in 5 chunks.
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void scan_bwd_kernel(ScanArgs p) {
     constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dxs[2][TT][CH];                    // {D, D u}, by tile parity
@@ -511,7 +511,7 @@ template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW, NW >
     }
 }
 
-// The adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps: scan_ends_kernel backwards (8 x 781 x 1536: 35 us of 186).
+// The adjoint at each chunk's beginning, from zero behind its end, and the sum of its steps: scan_ends_kernel backwards (8 x 781 x 1536: 33 us of 175).
 template <typename T, int NW, bool Z> __global__ __launch_bounds__(64 * NW) void scan_back_ends_kernel(ScanArgs p) {
     constexpr int NS = BNS, EP = TT / NW, BC = NS * NW;
     __shared__ float2 s_dg[2][TT][CH];                     // {D, dout silu(z)}
@@ -656,11 +656,12 @@ int scan_check(const a8_selective_scan_desc* d, const char* what) {
 }
 // Frame chunks.  A launch of n chunks takes as many tiles' time as a chunk has tiles, times the rounds of blocks that the 256 CUs hold: `part[k - 1]` is
 // the time of a round with k blocks on a CU as a share of a full one, `extra` what the chunks' own ends (all but one chunk's) cost more, a hundredth per
-// chunk what is left of first loads, partial sums and walks over earlier chunks.  Measured, N = 16 (us with one chunk / with the count taken here):
-//   forward   1 x 781 x 1536 82 / 26 (10), 4 x 781 85 / 57 (7), 8 x 781 89 / 89 (1; with 5: 89), 12 x 781 133 / 127 (7), 16 x 624 110 / 110 (1; with 2: 123),
-//             8 x 999 x 2048 116 / 116 (1; with 3: 131), 16 x 999 180 / 180 (1; with 2: 230)
-//   backward  1 x 781 x 1536 248 / 53 (10), 4 x 781 254 / 114 (5), 8 x 781 263 / 195 (5; with 7: 204), 12 x 781 348 / 279 (7), 16 x 624 288 / 284 (4),
-//             8 x 999 x 2048 341 / 299 (2), 16 x 999 471 / 471 (1; with 2: 538)
+// chunk what is left of first loads, partial sums and walks over earlier chunks.  Measured in one session, N = 16, kernels alone (us with one chunk / with
+// the count taken here; to be compared with one another: the sweep holds one set of inputs, where a program's calls take turns):
+//   forward   1 x 781 x 1536 83 / 26 (10), 4 x 781 86 / 58 (7), 8 x 781 90 / 90 (1; with 5: 90), 12 x 781 134 / 128 (7), 16 x 624 110 / 110 (1; with 2: 123),
+//             8 x 999 x 2048 117 / 117 (1; with 3: 131), 16 x 999 178 / 178 (1; with 2: 221)
+//   backward  1 x 781 x 1536 249 / 53 (10), 4 x 781 252 / 113 (5), 8 x 781 261 / 193 (5; with 7: 199), 12 x 781 344 / 275 (7), 16 x 624 285 / 281 (4),
+//             8 x 999 x 2048 338 / 295 (2), 16 x 999 454 / 454 (1; with 2: 512)
 // A chunk has at least 4 tiles.
 int scan_chunks(float blocks, int tiles, const float* part, int resident, float extra) {
     int best = 1;

@@ -586,7 +586,8 @@ def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=
 
 
 def causal_conv_step(x, state, weight, bias=None, *, activation="silu"):
-    """One frame of causal_conv for each utterance: x [B, C], state [B, K - 1, C] updated in place -> y [B, C].  No gradient."""
+    """One frame of causal_conv for each utterance: x [B, C], state [B, K - 1, C] updated in place -> y [B, C].
+    No gradient: refused where one would be recorded, for a parameter too."""
     _step_only("causal_conv_step", x, state, weight, bias)
     y = K.causal_conv_step(_rows(x), state, weight, bias, activation)
     torch.autograd.graph.increment_version(state)
@@ -636,7 +637,7 @@ def selective_scan(u, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=Tru
 
 def selective_scan_step(u, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, softplus=True):
     """One frame of selective_scan for each utterance: u, dt, z [B, Dm], B and C [B, G, N] (or [B, N]), state f32 [B, Dm, N] updated in place
-    -> y [B, Dm].  No gradient."""
+    -> y [B, Dm].  No gradient: refused where one would be recorded, for a parameter too."""
     _step_only("selective_scan_step", u, dt, A, B, C, state, D, z, dt_bias)
     if B.dim() == 2 and C.dim() == 2:
         B, C = B.unsqueeze(1), C.unsqueeze(1)
